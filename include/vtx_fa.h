@@ -380,6 +380,162 @@ typedef struct vtx_out_proj_args {
 } vtx_out_proj_args;
 VTX_API int vtx_attn_out_proj(const vtx_out_proj_args *args, void *stream);
 
+/* ---- paged decoder cache ---------------------------------------------------- */
+
+/* A decoder KV cache kept in pages, and one step's ragged batch of new tokens
+ * over it.  No counterpart in the reference, whose cache is one buffer per
+ * context (src/voxtral.cpp:1126-1136): pages let many streams share one pool.
+ * - k, v: the pools, [head_dim, page_size, n_head_kv, n_pages]: nb[1] is the
+ *   stride between the rows (tokens) of a page, nb[2] between KV heads, nb[3]
+ *   between pages.  F16 with 16-byte aligned base and strides (heads inside a
+ *   token or rows inside a head, either order), or Q8_0 with the rows of one
+ *   head contiguous (nb[1] = head_dim / 32 * 34) and base, nb[2] and nb[3]
+ *   multiples of 16.  k and v have the same type, sizes and strides.
+ *   head_dim 64 or 128; page_size a power of two from 16 to 256.
+ * - page_table: row r of stream s is row r % page_size of page
+ *   page_table[s * max_pages + r / page_size].  An entry that a call needs and
+ *   that is outside [0, n_pages) is reported through vtx_read_device_error;
+ *   reads then take page 0 and writes are dropped.
+ * - kv_len[s]: rows of stream s, this step's new ones included; at most
+ *   max_pages * page_size (a longer one is reported and cut there).
+ * - q_start: stream s brings the tokens [q_start[s], q_start[s+1]) of the
+ *   packed token arrays, possibly none; n of them go to (append) or stand in
+ *   (the other calls) its rows kv_len[s] - n ... kv_len[s] - 1.  A token whose
+ *   row would be negative is written nowhere and sees nothing.
+ * - n_tokens: tokens of the packed arrays (q_start's entries are cut there).
+ *   max_new and max_kv_len bound every stream's new tokens and kv_len: they
+ *   size grids and workspaces.  A stream above a bound is reported and what
+ *   exceeds it is not served (vtx_flash_attn_paged serves a longer kv_len
+ *   exactly).
+ * page_table, kv_len and q_start are device memory, read by the kernels only:
+ * a captured call may be replayed after they changed within the bounds. */
+typedef struct vtx_paged_kv {
+    vtx_tensor k, v;
+    const int32_t *page_table;          /* [n_seq][max_pages] */
+    const int32_t *kv_len;              /* [n_seq] */
+    const int32_t *q_start;             /* [n_seq + 1] */
+    int32_t n_seq, max_pages;
+    int32_t n_tokens, max_new, max_kv_len;
+    int32_t reserved;
+} vtx_paged_kv;
+
+/* vtx_kv_append into a paged cache: RoPE of Q and K (adjacent pairs, as
+ * vtx_kv_append), then K and V of every new token written to its row.  The
+ * angle pos * freq_base^(-2i/head_dim) is reduced in double, so far positions
+ * keep full accuracy (vtx_kv_append follows ggml's float recurrence).
+ * - q / k / v: n_tokens rows of heads x head_dim F32 (heads contiguous, token
+ *   stride *_nb1 bytes).  q_out: F32 or F16 rows of n_head_q x head_dim (NULL:
+ *   only K and V); an F32 q_out may be q itself.
+ * - positions[t]: the RoPE position of token t (not its row: an evicted
+ *   cache has fewer rows than positions).
+ * - row_pos / score (each optional): [n_seq][n_head_kv][row_cap] arrays; the
+ *   new rows' entries are set to positions[t] and to 0.  Needs
+ *   row_cap >= max_kv_len.
+ * Two streams of a call must not hold the same page where both write. */
+typedef struct vtx_kv_append_paged_args {
+    const vtx_paged_kv *kv;
+    int32_t n_head_q;
+    int32_t q_out_type;                 /* VTX_TYPE_F32 or VTX_TYPE_F16 */
+    float freq_base;
+    int32_t row_cap;
+    const float *q; size_t q_nb1;
+    void *q_out; size_t q_out_nb1;
+    const float *k; size_t k_nb1;
+    const float *v; size_t v_nb1;
+    const int32_t *positions;
+    int32_t *row_pos;
+    float *score;
+} vtx_kv_append_paged_args;
+VTX_API int vtx_kv_append_paged(const vtx_kv_append_paged_args *args, void *stream);
+
+/* vtx_flash_attn_ext for a ragged batch of new tokens over a paged cache: the
+ * decoder's attention node (src/voxtral.cpp:1802) for decode steps (one token
+ * per stream), chunks of prompts, and both in one call.
+ *   q    [head_dim, n_tokens, n_head_q, 1]  F32 or F16 (rounded to half)
+ *   dst  [head_dim, n_head_q, n_tokens, 1]  F32 or F16
+ *   lse  optional F32 [n_tokens][n_head_q]: ln(sum_j exp(x_j)) of each row's
+ *        scores x, -inf for a row that sees nothing (whose dst is 0)
+ * params: scale, logit_softcap, causal and window as in vtx_flash_attn_ext
+ * (causal: new token i of n sees row j iff j <= kv_len - n + i; window W:
+ * additionally j > kv_len - n + i - W; rows of an evicted cache are not
+ * positions, so a window does not fit there).  max_bias must be 0.
+ * Hq / Hkv <= 16; base and strides of q and dst multiples of 16 bytes.
+ * Rows at or behind kv_len may hold anything, NaN included.  P and V (and a
+ * F32 q) are rounded to half, everything else is F32.
+ * workspace: 256-byte aligned, vtx_flash_attn_paged_workspace bytes (they
+ * depend on kv's sizes and bounds and on n_head_q alone); calls that share
+ * one must not overlap on the GPU. */
+typedef struct vtx_flash_attn_paged_args {
+    const vtx_paged_kv *kv;
+    const vtx_tensor *q;
+    vtx_tensor *dst;
+    float *lse;
+    const vtx_fa_params *params;
+} vtx_flash_attn_paged_args;
+VTX_API size_t vtx_flash_attn_paged_workspace(const vtx_paged_kv *kv, int32_t n_head_q);
+VTX_API int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *args, void *workspace, size_t workspace_bytes,
+                                 void *stream);
+
+/* Accumulated attention weight of the rows of a paged cache: for every row j
+ * of stream s and KV head g
+ *   score_out[s][g][j] = decay * score[s][g][j]
+ *                      + sum over observed new tokens i and the query heads h
+ *                        of the group of exp(x_hij - lse[i][h])
+ * with the scores x, the visibility and lse of vtx_flash_attn_paged.  observe
+ * = n counts only the last n new tokens of each stream (0: all).  score and
+ * score_out: F32 [n_seq][n_head_kv][row_cap], the same array or two disjoint
+ * ones; with decay 0 score may be NULL.  Entries at or behind kv_len are left
+ * alone.  A token whose lse is -inf counts nothing. */
+typedef struct vtx_kv_score_paged_args {
+    const vtx_paged_kv *kv;
+    const vtx_tensor *q;                /* as in vtx_flash_attn_paged */
+    const float *lse;
+    const vtx_fa_params *params;
+    const float *score;
+    float *score_out;
+    int32_t row_cap;                    /* >= max_kv_len */
+    int32_t observe;
+    float decay;
+    int32_t reserved;
+} vtx_kv_score_paged_args;
+VTX_API int vtx_kv_score_paged(const vtx_kv_score_paged_args *args, void *stream);
+
+/* Evicts rows of a paged cache by score, each KV head for itself, and closes
+ * the gaps in place.  Of the n = kv_len[s] rows of a (stream, KV head),
+ * m = min(n, keep) stay: first the protected ones (position < n_sink, or
+ * >= next_pos[s] - n_recent), then those with the highest score (a NaN counts
+ * as -inf); between equals the lower row stays.  Kept rows below m do not
+ * move; the i-th gap below m takes the i-th kept row behind it, K and V.
+ * Attention does not depend on the order of cached rows.  Pages behind m rows
+ * are free afterwards.  The evicted pages of a stream must not be shared with
+ * another stream, nor be read by work that runs at the same time.
+ * - score: F32 [n_seq][n_head_kv][row_cap].
+ * - row_pos: optional int32, same shape: each row's position; NULL: its row
+ *   index.  next_pos: int32 [n_seq], the position that follows the newest
+ *   row's; NULL (only without row_pos): kv_len.
+ * - score_out / pos_out / src_out (each optional): [n_seq][n_head_kv][out_cap]
+ *   (out_cap >= keep): score, position and old row index of the m rows;
+ *   entries behind m are left alone.  score_out may be score and pos_out
+ *   row_pos (then out_cap = row_cap), no other overlap.
+ * - kv_len_out: [n_seq], receives m (may be kv_len).
+ * q_start is not used.  n_sink + n_recent <= keep. */
+typedef struct vtx_kv_evict_paged_args {
+    const vtx_paged_kv *kv;
+    const float *score;
+    const int32_t *row_pos;
+    const int32_t *next_pos;
+    float *score_out;
+    int32_t *pos_out;
+    int32_t *src_out;
+    int32_t *kv_len_out;
+    int32_t keep, n_sink, n_recent;
+    int32_t row_cap, out_cap;
+    int32_t reserved;
+} vtx_kv_evict_paged_args;
+VTX_API size_t vtx_kv_evict_paged_workspace(const vtx_paged_kv *kv);
+VTX_API int vtx_kv_evict_paged(const vtx_kv_evict_paged_args *args, void *workspace, size_t workspace_bytes,
+                               void *stream);
+
 /* Diagnostic: synchronises `stream`, returns and clears the device-side error
  * word of the current device (0 = none).  Kernels set it instead of hanging
  * when a bounded pipeline wait runs out, or when a batched-decode stream base

@@ -39,7 +39,7 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> str:
     if not force and not stale():
         return LIB
     cmd = [NVCC, "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-           "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared",
+           "--expt-relaxed-constexpr", "--threads", "0", "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared",
            "-I", os.path.join(ROOT, "include"), "-o", LIB + ".tmp"]
     if verbose_ptxas:
         cmd += ["-Xptxas", "-v"]

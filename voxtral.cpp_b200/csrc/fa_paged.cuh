@@ -1,0 +1,217 @@
+// fa_paged.cuh — attention of ragged chunks of new tokens over a paged cache
+// with mma.sync, any shape: the decoder node of src/voxtral.cpp:1802 over pages.
+//
+//   x_ij = scale * q_i . k_j  (softcap c: c * tanh(x / c)),  j visible to i
+//   O_i  = sum_j e^(x_ij - m_i) v_j / sum_j e^(x_ij - m_i)
+//
+// in one pass over the keys with the running maximum m and sum l of each row
+// in registers.  A CTA owns 64 query rows (row = token * G + head of the group,
+// so every K/V row is read once for the whole group) of one KV head: 4 warps of
+// 16 rows, tiles of 32 keys in shared memory.  F16 rows as they are.  Q8_0: K
+// as its integers (exact halves) with each block's scale applied to that
+// block's f32 sum, so scores and lse carry no rounding of K; V as d * q rounded
+// to half, like P.
+#pragma once
+#include <cuda_fp16.h>
+#include <cstdint>
+#include "vtx_ptx.cuh"
+#include "paged_kv.cuh"
+#include "fa_prefill_sm100.cuh"
+#include "fa_decode_mma.cuh"
+
+namespace vtx {
+
+struct PagedAttnArgs {
+    PagedView kv;
+    const char *q; int q_f16; long long q_nbt, q_nbh;       // token and head strides (bytes)
+    char *dst; int d_f16; long long d_nbt, d_nbh;
+    float *lse;
+    int Hq, G;
+    float scale, softcap;                                   // logits: scale * s, or softcap * tanh(scale / softcap * s)
+    int causal, window;
+};
+
+// Logit in log2 units of a dot product.
+__device__ __forceinline__ float paged_logit(float s, float scale, float softcap) {
+    return softcap != 0.0f ? softcap * kLog2e * tanhf(s * (scale / softcap)) : s * (scale * kLog2e);
+}
+
+// Two adjacent columns (d even) of a query row, rounded to half.
+__device__ __forceinline__ uint32_t paged_q2(const char *row, int f16, int d) {
+    if (f16) return *reinterpret_cast<const uint32_t *>(row + d * 2);
+    const float2 x = *reinterpret_cast<const float2 *>(row + d * 4);
+    return pack_half2(x.x, x.y);
+}
+
+// Scale of the Q8_0 block that holds column d of a cache row.
+__device__ __forceinline__ float q8_scale(const char *row, int d) {
+    return __half2float(*reinterpret_cast<const __half *>(row + (d >> 5) * 34));
+}
+// 8 consecutive values of a cache row as halves.  Q8_0: s * q rounded once,
+// exact for s = 1 (the bare integers).
+template <int KVT>
+__device__ __forceinline__ uint4 paged_load8(const char *row, int d, float s) {
+    if (KVT == 1) return *reinterpret_cast<const uint4 *>(row + d * 2);
+    const unsigned short *w = reinterpret_cast<const unsigned short *>(row + (d >> 5) * 34 + 2 + (d & 31));
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned short u = w[i];
+        r[i] = pack_half2(s * (float)(int8_t)(u & 0xff), s * (float)(int8_t)(u >> 8));
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// Writes two adjacent columns of an output row.
+__device__ __forceinline__ void paged_store2(const PagedAttnArgs &a, int tok, int head, int d, float x, float y) {
+    char *p = a.dst + (long long)tok * a.d_nbt + (long long)head * a.d_nbh;
+    if (a.d_f16) *reinterpret_cast<uint32_t *>(p + d * 2) = pack_half2(x, y);
+    else *reinterpret_cast<float2 *>(p + d * 4) = make_float2(x, y);
+}
+
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <int D, int KVT>
+__global__ void __launch_bounds__(128)
+fa_paged_kernel(const PagedAttnArgs a)
+{
+    grid_dep_wait();
+    grid_dep_launch();
+    constexpr int KEYS = 32, P = D + 8, KC = D / 16, NB = D / 8;
+    __shared__ __align__(16) __half ks[KEYS * P];
+    __shared__ __align__(16) __half vs[KEYS * P];
+    __shared__ float kd[KVT == 8 ? D / 32 : 1][KEYS];       // Q8_0: scales of K
+    const int b = blockIdx.z, g = blockIdx.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const PagedSeq s = paged_seq(a.kv, b);
+    if (blockIdx.x == 0 && s.n_new > a.kv.max_new) paged_report(a.kv, VTX_KERR_BOUND);
+    const int rows = min(s.n_new, a.kv.max_new) * a.G;
+    const int r_first = blockIdx.x * 64;
+    if (r_first >= rows) return;
+
+    const int off = s.len - s.n_new;                        // row of token 0
+    int row[2], tok[2], lo[2], hi[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        row[u] = r_first + warp * 16 + (lane >> 2) + 8 * u;
+        tok[u] = row[u] / a.G;
+        hi[u] = row[u] < rows ? (a.causal ? off + tok[u] : s.len - 1) : -1;
+        lo[u] = a.window > 0 ? off + tok[u] - a.window + 1 : 0;
+    }
+    const int t_first = r_first / a.G, t_last = (min(r_first + 64, rows) - 1) / a.G;
+    const int k_hi = a.causal ? off + t_last : s.len - 1;
+    const int k_lo = a.window > 0 ? max(0, off + t_first - a.window + 1) : 0;
+
+    uint32_t qa[KC][4];
+    {
+        const char *q0 = a.q + (long long)(s.q0 + tok[0]) * a.q_nbt + (long long)(g * a.G + row[0] % a.G) * a.q_nbh;
+        const char *q1 = a.q + (long long)(s.q0 + tok[1]) * a.q_nbt + (long long)(g * a.G + row[1] % a.G) * a.q_nbh;
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) {
+            const int c = kc * 16 + 2 * (lane & 3);
+            qa[kc][0] = row[0] < rows ? paged_q2(q0, a.q_f16, c) : 0u;
+            qa[kc][1] = row[1] < rows ? paged_q2(q1, a.q_f16, c) : 0u;
+            qa[kc][2] = row[0] < rows ? paged_q2(q0, a.q_f16, c + 8) : 0u;
+            qa[kc][3] = row[1] < rows ? paged_q2(q1, a.q_f16, c + 8) : 0u;
+        }
+    }
+    float o[NB][4];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    const int lrow = lane & 7, lmat = lane >> 3;
+
+    for (int k0 = k_lo & ~(KEYS - 1); k0 <= k_hi; k0 += KEYS) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < KEYS * (D / 8); i += 128) {
+            const int r = i / (D / 8), c = (i % (D / 8)) * 8;
+            uint4 kx = make_uint4(0u, 0u, 0u, 0u), vx = kx;
+            if (k0 + r >= k_lo && k0 + r <= k_hi) {         // other rows may hold anything: zeros instead
+                const long long at = paged_row(a.kv, b, k0 + r, g);
+                kx = paged_load8<KVT>(a.kv.k + at, c, 1.0f);
+                vx = paged_load8<KVT>(a.kv.v + at, c, KVT == 8 ? q8_scale(a.kv.v + at, c) : 1.0f);
+                if (KVT == 8 && (c & 31) == 0) kd[c >> 5][r] = q8_scale(a.kv.k + at, c);
+            }
+            *reinterpret_cast<uint4 *>(ks + r * P + c) = kx;
+            *reinterpret_cast<uint4 *>(vs + r * P + c) = vx;
+        }
+        __syncthreads();
+        float x[KEYS / 8][4];
+#pragma unroll
+        for (int nt = 0; nt < KEYS / 8; ++nt) {
+            x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
+#pragma unroll
+            for (int kc = 0; kc < KC; kc += 2) {
+                uint32_t bk[4];
+                ldsm_x4(bk, ks + (nt * 8 + lrow) * P + kc * 16 + lmat * 8);
+                if constexpr (KVT == 1) {
+                    mma16816(x[nt], qa[kc], bk[0], bk[1]);
+                    mma16816(x[nt], qa[kc + 1], bk[2], bk[3]);
+                } else {                                    // a block of 32 dims, then its scale
+                    float y[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma16816(y, qa[kc], bk[0], bk[1]);
+                    mma16816(y, qa[kc + 1], bk[2], bk[3]);
+                    const float2 d = *reinterpret_cast<const float2 *>(&kd[kc / 2][nt * 8 + 2 * (lane & 3)]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[nt][i] = fmaf(i & 1 ? d.y : d.x, y[i], x[nt][i]);
+                }
+            }
+        }
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int nt = 0; nt < KEYS / 8; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int u = i >> 1, key = k0 + nt * 8 + 2 * (lane & 3) + (i & 1);
+                x[nt][i] = key >= lo[u] && key <= hi[u] ? paged_logit(x[nt][i], a.scale, a.softcap) : -INFINITY;
+                mx[u] = fmaxf(mx[u], x[nt][i]);
+            }
+        float mu[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 1));
+            mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 2));
+            const float mn = fmaxf(m[u], mx[u]);
+            mu[u] = mn == -INFINITY ? 0.f : mn;
+            const float al = ex2(m[u] - mu[u]);
+            m[u] = mn;
+            l[u] *= al;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) { o[i][2 * u] *= al; o[i][2 * u + 1] *= al; }
+        }
+        uint32_t pa[KEYS / 16][4];
+#pragma unroll
+        for (int nt = 0; nt < KEYS / 8; ++nt) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[nt][i] = ex2(x[nt][i] - mu[i >> 1]);
+            l[0] += x[nt][0] + x[nt][1];
+            l[1] += x[nt][2] + x[nt][3];
+            pa[nt / 2][(nt & 1) * 2] = pack_half2(x[nt][0], x[nt][1]);
+            pa[nt / 2][(nt & 1) * 2 + 1] = pack_half2(x[nt][2], x[nt][3]);
+        }
+#pragma unroll
+        for (int kk = 0; kk < KEYS / 16; ++kk)
+#pragma unroll
+            for (int nb = 0; nb < NB; nb += 2) {
+                uint32_t bv[4];
+                ldsm_x4_t(bv, vs + (kk * 16 + (lmat & 1) * 8 + lrow) * P + nb * 8 + (lmat >> 1) * 8);
+                mma16816(o[nb], pa[kk], bv[0], bv[1]);
+                mma16816(o[nb + 1], pa[kk], bv[2], bv[3]);
+            }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+        if (row[u] >= rows) continue;
+        const float inv = l[u] == 0.f ? 0.f : 1.f / l[u];
+        const int head = g * a.G + row[u] % a.G, t = s.q0 + tok[u];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+            paged_store2(a, t, head, nb * 8 + 2 * (lane & 3), o[nb][2 * u] * inv, o[nb][2 * u + 1] * inv);
+        if (a.lse && (lane & 3) == 0)
+            a.lse[(long long)t * a.Hq + head] = l[u] == 0.f ? -INFINITY : (m[u] + log2f(l[u])) * kLn2;
+    }
+}
+
+}  // namespace vtx

@@ -25,6 +25,7 @@
 
 #include "../../include/vtx_fa.h"
 #include "vtx_ptx.cuh"
+#include "vtx_host.cuh"
 #include "fa_splitkv.cuh"
 #include "fa_prefill_sm100.cuh"
 #include "fa_encoder_sk.cuh"
@@ -44,22 +45,17 @@ __device__ int g_vtx_kernel_err;
 
 namespace {
 
-constexpr int kMaxDevices = 64;
-
-struct DeviceState {
-    int ok = 0;
-    int sms = 148;
-    int *err = nullptr;
-};
 DeviceState g_dev[kMaxDevices];
 std::once_flag g_dev_once[kMaxDevices];
 std::once_flag g_encode_once;
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 
+}  // namespace
+
 // Per-device set-up runs exactly once (std::call_once), so concurrent first
 // calls from several host threads are ordered: every caller sees the state
 // the one initialising call wrote.
-int ensure_device(DeviceState **out) {
+int vtx::ensure_device(DeviceState **out) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return VTX_ERR_NO_DEVICE;
     DeviceState &s = g_dev[dev];
@@ -88,9 +84,9 @@ int ensure_device(DeviceState **out) {
     return VTX_OK;
 }
 
-inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
-inline int elem_size(int t) { return t == VTX_TYPE_F32 ? 4 : 2; }
-inline int row_bytes(int t, int64_t d) { return t == VTX_TYPE_Q8_0 ? (int)(d / 32 * 34) : (int)(d * elem_size(t)); }
+PFN_cuTensorMapEncodeTiled_v12000 vtx::tensor_map_encoder() { return g_encode; }
+
+namespace {
 
 // ---- operand checks ----------------------------------------------------------
 
@@ -382,24 +378,6 @@ __global__ void convert_kv_f16_kernel(const char *src, long long nb1, long long 
         }
         dst[i] = __float2half_rn(x);
     }
-}
-
-// Every kernel is launched with programmatic stream serialisation (PDL): it
-// may be scheduled while the previous kernel on the stream drains, and waits
-// for it in-kernel (grid_dep_wait) before touching global memory.
-template <typename... KArgs, typename... Args>
-int launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args &&...args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...) == cudaSuccess ? VTX_OK : VTX_ERR_CUDA;
 }
 
 // The same with the grid in clusters of `cs` CTAs along x.

@@ -1,0 +1,310 @@
+// vtx_paged.cu — C ABI entry points of the paged decoder cache: append,
+// attention over ragged chunks, accumulated attention weight, eviction.
+// Operand checks, launch geometry and workspace accounting; nothing here
+// allocates, synchronises or aborts.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <cuda_fp16.h>
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "../../include/vtx_fa.h"
+#include "vtx_ptx.cuh"
+#include "vtx_host.cuh"
+#include "fa_prefill_sm100.cuh"
+#include "paged_kv.cuh"
+#include "fa_paged.cuh"
+#include "kv_score.cuh"
+#include "kv_evict.cuh"
+
+using namespace vtx;
+
+namespace {
+
+constexpr int kMaxGroup = 16;             // query heads per KV head
+
+int check_pool(const vtx_tensor &t, int row) {
+    if (!t.data) return VTX_ERR_NULL;
+    if (t.nb[1] < (size_t)row) return VTX_ERR_STRIDE;
+    if (reinterpret_cast<uintptr_t>(t.data) % 16 || t.nb[2] % 16 || t.nb[3] % 16) return VTX_ERR_STRIDE;
+    if (t.type == VTX_TYPE_Q8_0) return t.nb[0] == 34 && t.nb[1] == (size_t)row ? VTX_OK : VTX_ERR_STRIDE;
+    return t.nb[0] == 2 && t.nb[1] % 16 == 0 ? VTX_OK : VTX_ERR_STRIDE;
+}
+
+// Sizes and strides of a paged cache, as every call needs them.
+int check_paged(const vtx_paged_kv *p) {
+    if (!p) return VTX_ERR_NULL;
+    const vtx_tensor &k = p->k, &v = p->v;
+    if (k.type != v.type || (k.type != VTX_TYPE_F16 && k.type != VTX_TYPE_Q8_0)) return VTX_ERR_TYPE;
+    for (int i = 0; i < 4; ++i)
+        if (k.ne[i] != v.ne[i] || k.ne[i] < 1) return VTX_ERR_SHAPE;
+    if (k.ne[0] != 64 && k.ne[0] != 128) return VTX_ERR_UNSUPPORTED;
+    if (k.ne[1] < 16 || k.ne[1] > 256 || (k.ne[1] & (k.ne[1] - 1))) return VTX_ERR_UNSUPPORTED;
+    if (k.ne[2] > 65535 || k.ne[3] > INT32_MAX) return VTX_ERR_SHAPE;
+    if (p->n_seq < 0 || p->n_seq > 65535 || p->max_pages < 0 || p->n_tokens < 0 || p->max_new < 0 ||
+        p->max_kv_len < 0)
+        return VTX_ERR_SHAPE;
+    if ((long long)p->max_pages * k.ne[1] > INT32_MAX || p->n_tokens > (1 << 24)) return VTX_ERR_SHAPE;
+    if (p->max_kv_len > (long long)p->max_pages * k.ne[1] || p->max_new > p->n_tokens) return VTX_ERR_SHAPE;
+    for (int i = 1; i < 4; ++i)
+        if (k.nb[i] != v.nb[i] || k.nb[i] >= (1ULL << 40)) return VTX_ERR_STRIDE;
+    const int row = row_bytes(k.type, k.ne[0]);
+    int rc = check_pool(k, row);
+    if (rc == VTX_OK) rc = check_pool(v, row);
+    if (rc != VTX_OK) return rc;
+    if (p->n_seq > 0 && (!p->kv_len || (p->max_pages > 0 && !p->page_table))) return VTX_ERR_NULL;
+    return VTX_OK;
+}
+
+PagedView view_of(const vtx_paged_kv *p, const DeviceState *ds) {
+    PagedView v{};
+    v.k = static_cast<char *>(p->k.data);
+    v.v = static_cast<char *>(p->v.data);
+    v.nb1 = (long long)p->k.nb[1]; v.nb2 = (long long)p->k.nb[2]; v.nb3 = (long long)p->k.nb[3];
+    v.table = p->page_table; v.kv_len = p->kv_len; v.q_start = p->q_start;
+    v.n_seq = p->n_seq; v.n_tokens = p->n_tokens; v.max_new = p->max_new; v.max_kv = p->max_kv_len;
+    v.max_pages = p->max_pages; v.n_pages = (int)p->k.ne[3];
+    while ((1 << v.shift) < (int)p->k.ne[1]) ++v.shift;
+    v.Hkv = (int)p->k.ne[2];
+    v.err = ds->err;
+    return v;
+}
+
+// q [D, n_tokens, Hq, 1] of the attention and score calls.
+int check_q(const vtx_paged_kv *p, const vtx_tensor *q) {
+    if (!q) return VTX_ERR_NULL;
+    if (q->type != VTX_TYPE_F32 && q->type != VTX_TYPE_F16) return VTX_ERR_TYPE;
+    if (q->ne[0] != p->k.ne[0] || q->ne[1] != p->n_tokens || q->ne[3] != 1) return VTX_ERR_SHAPE;
+    if (q->ne[2] < 1 || q->ne[2] % p->k.ne[2]) return VTX_ERR_SHAPE;
+    if (q->ne[2] / p->k.ne[2] > kMaxGroup) return VTX_ERR_UNSUPPORTED;
+    if (q->nb[0] != (size_t)elem_size(q->type)) return VTX_ERR_STRIDE;
+    if (p->n_tokens == 0) return VTX_OK;
+    if (!q->data || !p->q_start) return VTX_ERR_NULL;
+    if (reinterpret_cast<uintptr_t>(q->data) % 16 || q->nb[1] % 16 || q->nb[2] % 16) return VTX_ERR_STRIDE;
+    return VTX_OK;
+}
+
+int check_params(const vtx_fa_params *p) {
+    if (!p) return VTX_ERR_NULL;
+    if (p->window < 0 || (p->window > 0 && !p->causal) || p->max_bias != 0.0f) return VTX_ERR_UNSUPPORTED;
+    if (!std::isfinite(p->scale) || !std::isfinite(p->logit_softcap)) return VTX_ERR_UNSUPPORTED;
+    return VTX_OK;
+}
+
+template <typename K>
+int set_smem(K kernel, int bytes) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess
+               ? VTX_OK : VTX_ERR_CUDA;
+}
+
+template <int D, int KVT>
+int launch_attn(const PagedAttnArgs &a, cudaStream_t st) {
+    const long long tiles = ((long long)a.kv.max_new * a.G + 63) / 64;
+    return launch_pdl(fa_paged_kernel<D, KVT>, dim3((unsigned)tiles, (unsigned)a.kv.Hkv, (unsigned)a.kv.n_seq),
+                      dim3(128), 0, st, a);
+}
+
+template <int D, int KVT>
+int launch_score(const PagedScoreArgs &a, cudaStream_t st) {
+    return launch_pdl(kv_score_kernel<D, KVT>,
+                      dim3((unsigned)((a.kv.max_kv + 127) / 128), (unsigned)a.kv.Hkv, (unsigned)a.kv.n_seq), dim3(128),
+                      0, st, a);
+}
+
+struct EvictPlan {
+    long long items;
+    int max_moves;
+    size_t moves_bytes, bytes;
+};
+
+EvictPlan plan_evict(const vtx_paged_kv *p) {
+    EvictPlan e{};
+    e.items = (long long)p->n_seq * p->k.ne[2];
+    e.max_moves = std::max(1, p->max_kv_len / 2);        // min(m, n - m) rows move at most
+    e.moves_bytes = align_up((size_t)e.items * e.max_moves * sizeof(int2), 256);
+    e.bytes = e.moves_bytes + align_up((size_t)e.items * sizeof(int2), 256);
+    return e;
+}
+
+}  // namespace
+
+extern "C" {
+
+int vtx_kv_append_paged(const vtx_kv_append_paged_args *p, void *stream) {
+    if (!p) return VTX_ERR_NULL;
+    int rc = check_paged(p->kv);
+    if (rc != VTX_OK) return rc;
+    const vtx_paged_kv *kv = p->kv;
+    const int D = (int)kv->k.ne[0];
+    if (p->q_out && p->q_out_type != VTX_TYPE_F32 && p->q_out_type != VTX_TYPE_F16) return VTX_ERR_TYPE;
+    if (p->q_out && p->n_head_q < 1) return VTX_ERR_SHAPE;
+    if (!(p->freq_base > 0.0f) || !std::isfinite(p->freq_base)) return VTX_ERR_UNSUPPORTED;
+    if ((p->row_pos || p->score) && p->row_cap < kv->max_kv_len) return VTX_ERR_SHAPE;
+    if (kv->n_tokens == 0 || kv->n_seq == 0) return VTX_OK;
+    if (!p->k || !p->v || !p->positions || !kv->q_start || (p->q_out && !p->q)) return VTX_ERR_NULL;
+    const size_t kvrow = (size_t)kv->k.ne[2] * D * 4, qrow = (size_t)p->n_head_q * D;
+    if (p->k_nb1 < kvrow || p->v_nb1 < kvrow) return VTX_ERR_STRIDE;
+    const unsigned long long rows =
+        reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v) | p->k_nb1 | p->v_nb1 |
+        (p->q_out ? reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->q_out) | p->q_nb1 |
+                        p->q_out_nb1 : 0);
+    if (rows % 8) return VTX_ERR_STRIDE;
+    if (p->q_out && (p->q_nb1 < qrow * 4 || p->q_out_nb1 < qrow * elem_size(p->q_out_type))) return VTX_ERR_STRIDE;
+    DeviceState *ds = nullptr;
+    rc = ensure_device(&ds);
+    if (rc != VTX_OK) return rc;
+    KvAppendPagedArgs a{};
+    a.kv = view_of(kv, ds);
+    a.Hq = p->q_out ? p->n_head_q : 0;
+    a.q8 = kv->k.type == VTX_TYPE_Q8_0;
+    a.qo_f16 = p->q_out_type == VTX_TYPE_F16;
+    a.q = p->q; a.q_nb1 = (long long)(p->q_nb1 / 4);
+    a.k = p->k; a.k_nb1 = (long long)(p->k_nb1 / 4);
+    a.v = p->v; a.v_nb1 = (long long)(p->v_nb1 / 4);
+    a.q_out = p->q_out; a.qo_nb1 = (long long)(p->q_out_nb1 / (a.qo_f16 ? 2 : 4));
+    a.positions = p->positions;
+    a.row_pos = p->row_pos; a.score = p->score; a.row_cap = p->row_cap;
+    for (int i = 0; i < D / 2; ++i)
+        a.turns[i] = std::pow((double)p->freq_base, -2.0 * i / D) / (2.0 * 3.14159265358979323846);
+    // few tokens: 8 rows (one per warp) per CTA, so that all rows are in flight
+    // together; many tokens: one CTA and one cos/sin table per token
+    const int per_tok = a.Hq + 2 * a.kv.Hkv;
+    a.rows_per_cta = kv->n_tokens >= 2 * ds->sms ? per_tok : 8;
+    const dim3 grid((unsigned)kv->n_tokens, (unsigned)((per_tok + a.rows_per_cta - 1) / a.rows_per_cta));
+    if (grid.y > 65535) return VTX_ERR_SHAPE;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return D == 64 ? launch_pdl(kv_append_paged_kernel<64>, grid, dim3(256), 0, st, a)
+                   : launch_pdl(kv_append_paged_kernel<128>, grid, dim3(256), 0, st, a);
+}
+
+size_t vtx_flash_attn_paged_workspace(const vtx_paged_kv *kv, int32_t n_head_q) {
+    if (check_paged(kv) != VTX_OK || n_head_q < 1 || n_head_q % kv->k.ne[2] ||
+        n_head_q / kv->k.ne[2] > kMaxGroup)
+        return (size_t)-1;
+    return 0;
+}
+
+int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, size_t workspace_bytes, void *stream) {
+    if (!p) return VTX_ERR_NULL;
+    int rc = check_paged(p->kv);
+    if (rc == VTX_OK) rc = check_q(p->kv, p->q);
+    if (rc == VTX_OK) rc = check_params(p->params);
+    if (rc != VTX_OK) return rc;
+    const vtx_paged_kv *kv = p->kv;
+    const vtx_tensor *q = p->q, *d = p->dst;
+    if (!d) return VTX_ERR_NULL;
+    if (d->type != VTX_TYPE_F32 && d->type != VTX_TYPE_F16) return VTX_ERR_TYPE;
+    if (d->ne[0] != q->ne[0] || d->ne[1] != q->ne[2] || d->ne[2] != q->ne[1] || d->ne[3] != 1) return VTX_ERR_SHAPE;
+    if (d->nb[0] != (size_t)elem_size(d->type)) return VTX_ERR_STRIDE;
+    if (kv->n_tokens == 0 || kv->n_seq == 0) return VTX_OK;
+    if (!d->data) return VTX_ERR_NULL;
+    if (reinterpret_cast<uintptr_t>(d->data) % 16 || d->nb[1] % 16 || d->nb[2] % 16) return VTX_ERR_STRIDE;
+    const int Hq = (int)q->ne[2];
+    const size_t need = vtx_flash_attn_paged_workspace(kv, Hq);
+    if (workspace_bytes < need || (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256)))
+        return VTX_ERR_WORKSPACE;
+    DeviceState *ds = nullptr;
+    rc = ensure_device(&ds);
+    if (rc != VTX_OK) return rc;
+    PagedAttnArgs a{};
+    a.kv = view_of(kv, ds);
+    a.q = static_cast<const char *>(q->data); a.q_f16 = q->type == VTX_TYPE_F16;
+    a.q_nbt = (long long)q->nb[1]; a.q_nbh = (long long)q->nb[2];
+    a.dst = static_cast<char *>(d->data); a.d_f16 = d->type == VTX_TYPE_F16;
+    a.d_nbt = (long long)d->nb[2]; a.d_nbh = (long long)d->nb[1];
+    a.lse = p->lse;
+    a.Hq = Hq; a.G = Hq / a.kv.Hkv;
+    a.scale = p->params->scale; a.softcap = p->params->logit_softcap;
+    a.causal = p->params->causal != 0; a.window = p->params->window;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool f16 = kv->k.type == VTX_TYPE_F16;
+    if (kv->k.ne[0] == 64) return f16 ? launch_attn<64, 1>(a, st) : launch_attn<64, 8>(a, st);
+    return f16 ? launch_attn<128, 1>(a, st) : launch_attn<128, 8>(a, st);
+}
+
+int vtx_kv_score_paged(const vtx_kv_score_paged_args *p, void *stream) {
+    if (!p) return VTX_ERR_NULL;
+    int rc = check_paged(p->kv);
+    if (rc == VTX_OK) rc = check_q(p->kv, p->q);
+    if (rc == VTX_OK) rc = check_params(p->params);
+    if (rc != VTX_OK) return rc;
+    const vtx_paged_kv *kv = p->kv;
+    if (!std::isfinite(p->decay)) return VTX_ERR_UNSUPPORTED;
+    if (p->observe < 0 || p->row_cap < kv->max_kv_len) return VTX_ERR_SHAPE;
+    if (kv->n_seq == 0 || kv->max_kv_len == 0) return VTX_OK;
+    if (!p->score_out || !kv->q_start || (kv->n_tokens > 0 && !p->lse) || (p->decay != 0.0f && !p->score))
+        return VTX_ERR_NULL;
+    DeviceState *ds = nullptr;
+    rc = ensure_device(&ds);
+    if (rc != VTX_OK) return rc;
+    PagedScoreArgs a{};
+    a.kv = view_of(kv, ds);
+    a.q = static_cast<const char *>(p->q->data); a.q_f16 = p->q->type == VTX_TYPE_F16;
+    a.q_nbt = (long long)p->q->nb[1]; a.q_nbh = (long long)p->q->nb[2];
+    a.lse = p->lse; a.score = p->score; a.score_out = p->score_out; a.row_cap = p->row_cap;
+    a.decay = p->decay; a.observe = p->observe;
+    a.Hq = (int)p->q->ne[2]; a.G = a.Hq / a.kv.Hkv;
+    a.scale = p->params->scale; a.softcap = p->params->logit_softcap;
+    a.causal = p->params->causal != 0; a.window = p->params->window;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool f16 = kv->k.type == VTX_TYPE_F16;
+    if (kv->k.ne[0] == 64) return f16 ? launch_score<64, 1>(a, st) : launch_score<64, 8>(a, st);
+    return f16 ? launch_score<128, 1>(a, st) : launch_score<128, 8>(a, st);
+}
+
+size_t vtx_kv_evict_paged_workspace(const vtx_paged_kv *kv) {
+    return check_paged(kv) == VTX_OK ? plan_evict(kv).bytes : (size_t)-1;
+}
+
+int vtx_kv_evict_paged(const vtx_kv_evict_paged_args *p, void *workspace, size_t workspace_bytes, void *stream) {
+    if (!p) return VTX_ERR_NULL;
+    int rc = check_paged(p->kv);
+    if (rc != VTX_OK) return rc;
+    const vtx_paged_kv *kv = p->kv;
+    if (p->keep < 0 || p->n_sink < 0 || p->n_recent < 0 || (long long)p->n_sink + p->n_recent > p->keep)
+        return VTX_ERR_SHAPE;
+    if (p->row_cap < kv->max_kv_len) return VTX_ERR_SHAPE;
+    if ((p->score_out || p->pos_out || p->src_out) && p->out_cap < p->keep) return VTX_ERR_SHAPE;
+    if (((p->score_out && p->score_out == p->score) || (p->pos_out && p->pos_out == p->row_pos)) &&
+        p->out_cap != p->row_cap)
+        return VTX_ERR_SHAPE;
+    if (kv->n_seq == 0) return VTX_OK;
+    if (!p->kv_len_out || (kv->max_kv_len > 0 && !p->score) || (p->row_pos && !p->next_pos)) return VTX_ERR_NULL;
+    const EvictPlan e = plan_evict(kv);
+    if (e.items > (1 << 24)) return VTX_ERR_UNSUPPORTED;
+    if (workspace_bytes < e.bytes || !workspace || reinterpret_cast<uintptr_t>(workspace) % 256)
+        return VTX_ERR_WORKSPACE;
+    DeviceState *ds = nullptr;
+    rc = ensure_device(&ds);
+    if (rc != VTX_OK) return rc;
+    PagedEvictArgs a{};
+    a.kv = view_of(kv, ds);
+    a.score = p->score; a.row_pos = p->row_pos; a.next_pos = p->next_pos;
+    a.score_out = p->score_out; a.pos_out = p->pos_out; a.src_out = p->src_out; a.kv_len_out = p->kv_len_out;
+    a.keep = p->keep; a.n_sink = p->n_sink; a.n_recent = p->n_recent;
+    a.row_cap = p->row_cap; a.out_cap = p->out_cap;
+    a.max_moves = e.max_moves;
+    a.moves = static_cast<int2 *>(workspace);
+    a.counts = reinterpret_cast<int2 *>(static_cast<char *>(workspace) + e.moves_bytes);
+    a.row_bytes = row_bytes(kv->k.type, kv->k.ne[0]);
+    a.vec = kv->k.type == VTX_TYPE_F16 ? 16 : 4;
+    // about eight CTAs per SM over all items, at most one per 64 possible moves
+    a.slices = (int)std::max<long long>(1, std::min<long long>((8LL * ds->sms + e.items - 1) / e.items,
+                                                               (e.max_moves + 63) / 64));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int keys = std::min(kv->max_kv_len, kEvictKeysInSmem) * 4;
+    if (kv->max_kv_len <= kEvictKeysInSmem) {
+        if (keys > 32 * 1024) {
+            rc = set_smem(kv_evict_select_kernel<true>, kEvictKeysInSmem * 4);
+            if (rc != VTX_OK) return rc;
+        }
+        rc = launch_pdl(kv_evict_select_kernel<true>, dim3((unsigned)e.items), dim3(kEvictThreads), (size_t)keys, st, a);
+    } else {
+        rc = launch_pdl(kv_evict_select_kernel<false>, dim3((unsigned)e.items), dim3(kEvictThreads), 0, st, a);
+    }
+    if (rc != VTX_OK) return rc;
+    return launch_pdl(kv_evict_move_kernel, dim3((unsigned)(e.items * a.slices)), dim3(256), 0, st, a);
+}
+
+}  // extern "C"

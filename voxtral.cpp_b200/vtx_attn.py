@@ -93,6 +93,47 @@ class OutProjArgs(ctypes.Structure):
                 ("residual", ctypes.c_void_p), ("dst", ctypes.c_void_p)]
 
 
+class VtxPagedKv(ctypes.Structure):
+    """vtx_paged_kv (include/vtx_fa.h)."""
+    _fields_ = [("k", VtxTensor), ("v", VtxTensor), ("page_table", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
+                ("q_start", ctypes.c_void_p), ("n_seq", ctypes.c_int32), ("max_pages", ctypes.c_int32),
+                ("n_tokens", ctypes.c_int32), ("max_new", ctypes.c_int32), ("max_kv_len", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
+class KvAppendPagedArgs(ctypes.Structure):
+    """vtx_kv_append_paged_args (include/vtx_fa.h)."""
+    _fields_ = [("kv", ctypes.c_void_p), ("n_head_q", ctypes.c_int32), ("q_out_type", ctypes.c_int32),
+                ("freq_base", ctypes.c_float), ("row_cap", ctypes.c_int32),
+                ("q", ctypes.c_void_p), ("q_nb1", ctypes.c_size_t),
+                ("q_out", ctypes.c_void_p), ("q_out_nb1", ctypes.c_size_t),
+                ("k", ctypes.c_void_p), ("k_nb1", ctypes.c_size_t),
+                ("v", ctypes.c_void_p), ("v_nb1", ctypes.c_size_t),
+                ("positions", ctypes.c_void_p), ("row_pos", ctypes.c_void_p), ("score", ctypes.c_void_p)]
+
+
+class FlashAttnPagedArgs(ctypes.Structure):
+    """vtx_flash_attn_paged_args (include/vtx_fa.h)."""
+    _fields_ = [("kv", ctypes.c_void_p), ("q", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+                ("params", ctypes.c_void_p)]
+
+
+class KvScorePagedArgs(ctypes.Structure):
+    """vtx_kv_score_paged_args (include/vtx_fa.h)."""
+    _fields_ = [("kv", ctypes.c_void_p), ("q", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("params", ctypes.c_void_p),
+                ("score", ctypes.c_void_p), ("score_out", ctypes.c_void_p), ("row_cap", ctypes.c_int32),
+                ("observe", ctypes.c_int32), ("decay", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
+class KvEvictPagedArgs(ctypes.Structure):
+    """vtx_kv_evict_paged_args (include/vtx_fa.h)."""
+    _fields_ = [("kv", ctypes.c_void_p), ("score", ctypes.c_void_p), ("row_pos", ctypes.c_void_p),
+                ("next_pos", ctypes.c_void_p), ("score_out", ctypes.c_void_p), ("pos_out", ctypes.c_void_p),
+                ("src_out", ctypes.c_void_p), ("kv_len_out", ctypes.c_void_p), ("keep", ctypes.c_int32),
+                ("n_sink", ctypes.c_int32), ("n_recent", ctypes.c_int32), ("row_cap", ctypes.c_int32),
+                ("out_cap", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
 class EncChunk(ctypes.Structure):
     """vtx_enc_chunk (include/vtx_fa.h): one chunk of the realtime encoder run."""
     _fields_ = [("mel_offset", ctypes.c_int32), ("mel_frames", ctypes.c_int32), ("n_tokens", ctypes.c_int32),
@@ -150,6 +191,18 @@ def load(path: str = LIB_PATH):
     L.vtx_decode_layer.restype = ctypes.c_int
     L.vtx_decode_layer_workspace.argtypes = [P(DecodeLayerArgs)]
     L.vtx_decode_layer_workspace.restype = ctypes.c_size_t
+    L.vtx_kv_append_paged.argtypes = [P(KvAppendPagedArgs), ctypes.c_void_p]
+    L.vtx_kv_append_paged.restype = ctypes.c_int
+    L.vtx_flash_attn_paged_workspace.argtypes = [P(VtxPagedKv), ctypes.c_int32]
+    L.vtx_flash_attn_paged_workspace.restype = ctypes.c_size_t
+    L.vtx_flash_attn_paged.argtypes = [P(FlashAttnPagedArgs), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+    L.vtx_flash_attn_paged.restype = ctypes.c_int
+    L.vtx_kv_score_paged.argtypes = [P(KvScorePagedArgs), ctypes.c_void_p]
+    L.vtx_kv_score_paged.restype = ctypes.c_int
+    L.vtx_kv_evict_paged_workspace.argtypes = [P(VtxPagedKv)]
+    L.vtx_kv_evict_paged_workspace.restype = ctypes.c_size_t
+    L.vtx_kv_evict_paged.argtypes = [P(KvEvictPagedArgs), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+    L.vtx_kv_evict_paged.restype = ctypes.c_int
     _lib = L
     return L
 
@@ -378,6 +431,221 @@ class DecodeLayerPlan:
         _check(load().vtx_decode_layer(ctypes.byref(a), self.workspace.data_ptr(), self.workspace.numel(),
                                        ctypes.c_void_p(s.cuda_stream)), "vtx_decode_layer")
         return out
+
+
+# ---- paged decoder cache ------------------------------------------------------
+
+class PagedKv:
+    """A decoder cache in pages with one step's ragged batch of new tokens
+    (vtx_paged_kv), and the calls over it: append, attend, score, evict.
+
+    k_pool, v_pool: (n_pages, n_head_kv, page_size, D) float16 views, or uint8
+    with Q8_0 blocks on the last axis (rows of a head contiguous).  page_table:
+    int32 (n_seq, max_pages), kv_len: int32 (n_seq,), q_start: int32
+    (n_seq + 1,), contiguous on the pools' device: the kernels read them, so
+    they may change between calls (and between replays of a captured call)
+    within n_tokens, max_new and max_kv_len (default: the table's capacity).
+    Workspaces are made here once; calls on one PagedKv must not overlap on
+    the GPU.  Inputs and outputs stay the caller's and are not copied."""
+
+    def __init__(self, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor,
+                 q_start: torch.Tensor, n_head_q: int, *, n_tokens: int, max_new: int,
+                 max_kv_len: Optional[int] = None):
+        if k_pool.dim() != 4 or v_pool.shape != k_pool.shape or v_pool.dtype != k_pool.dtype:
+            raise VtxError(-3, "k_pool and v_pool must be (n_pages, n_head_kv, page_size, D) alike")
+        if k_pool.dtype not in (torch.float16, torch.uint8):
+            raise VtxError(-2, "pools must be float16 or Q8_0 bytes")
+        self.dev = k_pool.device
+        n_seq = kv_len.shape[0]
+        for t, shape in ((page_table, (n_seq, page_table.shape[-1])), (kv_len, (n_seq,)), (q_start, (n_seq + 1,))):
+            if t.dtype != torch.int32 or not t.is_contiguous() or t.device != self.dev or tuple(t.shape) != shape:
+                raise VtxError(-3, "page_table, kv_len and q_start must be contiguous int32 on the pools' device")
+        self.k_pool, self.v_pool, self.page_table, self.kv_len, self.q_start = k_pool, v_pool, page_table, kv_len, q_start
+        self.n_seq, self.n_head_q, self.n_head_kv = n_seq, n_head_q, k_pool.shape[1]
+        kvt = Q8_0 if k_pool.dtype == torch.uint8 else F16
+        self.head_dim = k_pool.shape[3] // Q8_0_BLOCK * QK8_0 if kvt == Q8_0 else k_pool.shape[3]
+        self.n_tokens = n_tokens
+        c = VtxPagedKv()
+        c.k, c.v = self._pool(k_pool, kvt), self._pool(v_pool, kvt)
+        c.page_table, c.kv_len, c.q_start = page_table.data_ptr(), kv_len.data_ptr(), q_start.data_ptr()
+        c.n_seq, c.max_pages, c.n_tokens, c.max_new = n_seq, page_table.shape[1], n_tokens, max_new
+        c.max_kv_len = page_table.shape[1] * k_pool.shape[2] if max_kv_len is None else max_kv_len
+        self.c = c
+        self.max_kv_len = c.max_kv_len
+        self._lib = load()
+        need = [self._lib.vtx_flash_attn_paged_workspace(ctypes.byref(c), n_head_q),
+                self._lib.vtx_kv_evict_paged_workspace(ctypes.byref(c))]
+        if ctypes.c_size_t(-1).value in need:
+            raise VtxError(-3, "paged cache rejected")
+        # one buffer for every call: they follow one another
+        self.workspace = torch.empty(max(max(need), 256), dtype=torch.uint8, device=self.dev)
+        self._ws = (ctypes.c_void_p(self.workspace.data_ptr()), ctypes.c_size_t(self.workspace.numel()))
+        # argument blocks, made once: a call only sets its tensors
+        self._q, self._dst, self._params = VtxTensor(), VtxTensor(), FaParams()
+        for d in (self._q, self._dst):
+            d.ne[0], d.ne[3] = self.head_dim, 1
+        self._q.ne[1], self._q.ne[2] = n_tokens, n_head_q
+        self._dst.ne[1], self._dst.ne[2] = n_head_q, n_tokens
+        at, adr = ctypes.addressof, ctypes.addressof(c)
+        self._append, self._attend = KvAppendPagedArgs(), FlashAttnPagedArgs()
+        self._score, self._evict = KvScorePagedArgs(), KvEvictPagedArgs()
+        for a in (self._append, self._attend, self._score, self._evict):
+            a.kv = adr
+        self._attend.q, self._attend.dst, self._attend.params = at(self._q), at(self._dst), at(self._params)
+        self._score.q, self._score.params = at(self._q), at(self._params)
+
+    @staticmethod
+    def _pool(t: torch.Tensor, kvt: int) -> VtxTensor:
+        d = VtxTensor()
+        es, s = t.element_size(), t.stride()
+        if s[3] != 1:
+            raise VtxError(-4, "the last axis of a pool must be contiguous")
+        d.type = kvt
+        row = t.shape[3] * es
+        # an axis of one element: any legal stride
+        nb = [34 if kvt == Q8_0 else es, s[2] * es, s[1] * es if t.shape[1] > 1 else row * t.shape[2], s[0] * es]
+        if t.shape[0] == 1:
+            nb[3] = max(nb[1] * t.shape[2], nb[2] * t.shape[1])
+        ne = [t.shape[3] // Q8_0_BLOCK * QK8_0 if kvt == Q8_0 else t.shape[3], t.shape[2], t.shape[1], t.shape[0]]
+        for i in range(4):
+            d.ne[i], d.nb[i] = ne[i], nb[i]
+        d.data = t.data_ptr()
+        return d
+
+    def _rows(self, t: torch.Tensor, heads: int, what: str, d: VtxTensor, token: int, head: int) -> None:
+        """Puts a (n_tokens, heads, D) float32 / float16 view into descriptor d."""
+        if tuple(t.shape) != (self.n_tokens, heads, self.head_dim) or t.stride(2) != 1 or t.device != self.dev:
+            raise VtxError(-3, f"{what} must be ({self.n_tokens}, {heads}, {self.head_dim}), last axis contiguous")
+        es = t.element_size()
+        d.type = _ggml_type(t, None)
+        d.nb[0], d.nb[token], d.nb[head], d.data = es, t.stride(0) * es, t.stride(1) * es, t.data_ptr()
+
+    def _array(self, t: Optional[torch.Tensor], dtype: torch.dtype, what: str, cap: Optional[int]) -> Optional[int]:
+        """Checks a (n_seq, n_head_kv, cap) row array; returns its cap."""
+        if t is None:
+            return cap
+        if t.dtype != dtype or t.dim() != 3 or t.shape[0] != self.n_seq or t.shape[1] != self.n_head_kv or \
+                not t.is_contiguous() or t.device != self.dev or (cap is not None and t.shape[2] != cap):
+            raise VtxError(-3, f"{what} must be a contiguous ({self.n_seq}, {self.n_head_kv}, rows) {dtype} tensor")
+        return t.shape[2]
+
+    def _set_params(self, scale, causal, window, softcap) -> None:
+        p = self._params
+        p.scale = self.head_dim ** -0.5 if scale is None else scale
+        p.logit_softcap, p.causal, p.window = softcap, 1 if causal else 0, window
+
+    def _call(self, fn, args, stream: Optional[torch.cuda.Stream], *ws) -> None:
+        if self.dev.type != "cuda":
+            raise VtxError(-8, "the pools are not on a GPU")
+        s = stream.cuda_stream if stream is not None else torch.cuda.current_stream(self.dev).cuda_stream
+        if torch.cuda.current_device() != self.dev.index:
+            with torch.cuda.device(self.dev):
+                rc = fn(ctypes.byref(args), *ws, ctypes.c_void_p(s))
+        else:
+            rc = fn(ctypes.byref(args), *ws, ctypes.c_void_p(s))
+        if rc != 0:
+            raise VtxError(rc, fn.__name__)
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, freq_base: float = 1e6, *,
+               q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
+               row_pos: Optional[torch.Tensor] = None, score: Optional[torch.Tensor] = None,
+               stream: Optional[torch.cuda.Stream] = None) -> Optional[torch.Tensor]:
+        """vtx_kv_append_paged: k, v (n_tokens, n_head_kv, D) float32 into the new
+        tokens' rows, K rotated to positions (int32 (n_tokens,)); q (n_tokens,
+        n_head_q, D) float32 rotated into q_out (float32 or float16; made as
+        float16 when not given).  row_pos (int32) and score (float32),
+        (n_seq, n_head_kv, rows): the new rows' entries are set."""
+        T, Hq, Hkv, D = self.n_tokens, self.n_head_q, self.n_head_kv, self.head_dim
+        for t, h in ((k, Hkv), (v, Hkv)) + (((q, Hq),) if q is not None else ()):
+            if t.dtype != torch.float32 or tuple(t.shape) != (T, h, D) or t.stride(2) != 1 or t.stride(1) != D:
+                raise VtxError(-4, f"q/k/v must be ({T}, heads, {D}) float32 with heads contiguous")
+        if positions.dtype != torch.int32 or positions.shape != (T,) or not positions.is_contiguous():
+            raise VtxError(-3, "positions must be contiguous int32, one per token")
+        if q is not None and q_out is None:
+            q_out = torch.empty(q.shape, dtype=torch.float16, device=q.device)
+        a = self._append
+        if q_out is not None:
+            if q is None:
+                raise VtxError(-1, "q_out without q")
+            if tuple(q_out.shape) != (T, Hq, D) or q_out.stride(2) != 1 or q_out.stride(1) != D:
+                raise VtxError(-4, f"q_out must be ({T}, {Hq}, {D}) with heads contiguous")
+            a.n_head_q, a.q_out_type = Hq, _ggml_type(q_out, None)
+            a.q, a.q_nb1 = q.data_ptr(), q.stride(0) * 4
+            a.q_out, a.q_out_nb1 = q_out.data_ptr(), q_out.stride(0) * q_out.element_size()
+        else:
+            a.q = a.q_out = None
+        a.freq_base = freq_base
+        a.k, a.k_nb1, a.v, a.v_nb1 = k.data_ptr(), k.stride(0) * 4, v.data_ptr(), v.stride(0) * 4
+        a.positions = positions.data_ptr()
+        cap = self._array(score, torch.float32, "score", self._array(row_pos, torch.int32, "row_pos", None))
+        a.row_cap = cap or 0
+        a.row_pos = row_pos.data_ptr() if row_pos is not None else None
+        a.score = score.data_ptr() if score is not None else None
+        self._call(self._lib.vtx_kv_append_paged, a, stream)
+        return q_out
+
+    def attend(self, q: torch.Tensor, out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, *,
+               scale: Optional[float] = None, causal: bool = True, window: int = 0, logit_softcap: float = 0.0,
+               stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+        """vtx_flash_attn_paged: q (n_tokens, n_head_q, D) float16 / float32 ->
+        out, same shape (float32, or the type of the given tensor).  lse:
+        optional float32 (n_tokens, n_head_q) that receives ln sum exp.  scale
+        defaults to D ** -0.5."""
+        if out is None:
+            out = torch.empty((self.n_tokens, self.n_head_q, self.head_dim), dtype=torch.float32, device=self.dev)
+        self._rows(q, self.n_head_q, "q", self._q, 1, 2)
+        self._rows(out, self.n_head_q, "out", self._dst, 2, 1)
+        self._set_params(scale, causal, window, logit_softcap)
+        self._attend.lse = self._check_lse(lse) if lse is not None else None
+        self._call(self._lib.vtx_flash_attn_paged, self._attend, stream, *self._ws)
+        return out
+
+    def _check_lse(self, lse: torch.Tensor) -> int:
+        if lse.dtype != torch.float32 or tuple(lse.shape) != (self.n_tokens, self.n_head_q) or not lse.is_contiguous():
+            raise VtxError(-3, "lse must be a contiguous float32 (n_tokens, n_head_q) tensor")
+        return lse.data_ptr()
+
+    def score(self, q: torch.Tensor, lse: torch.Tensor, score: torch.Tensor, score_out: Optional[torch.Tensor] = None,
+              *, scale: Optional[float] = None, causal: bool = True, window: int = 0, logit_softcap: float = 0.0,
+              observe: int = 0, decay: float = 1.0, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+        """vtx_kv_score_paged: adds the attention weight that the new tokens (the
+        last ``observe`` of each stream; 0: all) gave every cached row to
+        decay * score, float32 (n_seq, n_head_kv, rows); in place, or into
+        score_out.  q and lse as attend read and wrote them."""
+        out = score if score_out is None else score_out
+        cap = self._array(out, torch.float32, "score_out", self._array(score, torch.float32, "score", None))
+        self._rows(q, self.n_head_q, "q", self._q, 1, 2)
+        self._set_params(scale, causal, window, logit_softcap)
+        a = self._score
+        a.lse, a.score, a.score_out = self._check_lse(lse), score.data_ptr(), out.data_ptr()
+        a.row_cap, a.observe, a.decay = cap, observe, decay
+        self._call(self._lib.vtx_kv_score_paged, a, stream)
+        return out
+
+    def evict(self, score: torch.Tensor, keep: int, kv_len_out: Optional[torch.Tensor] = None, *, n_sink: int = 0,
+              n_recent: int = 0, row_pos: Optional[torch.Tensor] = None, next_pos: Optional[torch.Tensor] = None,
+              score_out: Optional[torch.Tensor] = None, pos_out: Optional[torch.Tensor] = None,
+              src_out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+        """vtx_kv_evict_paged: every (stream, KV head) keeps its ``keep`` best rows,
+        moved together in place; kv_len_out (default: kv_len itself) receives
+        the new lengths.  score_out, pos_out, src_out: optional
+        (n_seq, n_head_kv, >= keep) arrays of the kept rows' scores, positions
+        and old row indices; score_out may be score and pos_out row_pos."""
+        if kv_len_out is None:
+            kv_len_out = self.kv_len
+        for t, what in ((kv_len_out, "kv_len_out"), (next_pos, "next_pos")):
+            if t is not None and (t.dtype != torch.int32 or t.shape != (self.n_seq,) or not t.is_contiguous()):
+                raise VtxError(-3, f"{what} must be contiguous int32, one per stream")
+        a = self._evict
+        a.row_cap = self._array(row_pos, torch.int32, "row_pos", self._array(score, torch.float32, "score", None))
+        cap = self._array(pos_out, torch.int32, "pos_out", self._array(score_out, torch.float32, "score_out", None))
+        a.out_cap = self._array(src_out, torch.int32, "src_out", cap) or 0
+        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        a.score, a.row_pos, a.next_pos, a.kv_len_out = score.data_ptr(), ptr(row_pos), ptr(next_pos), kv_len_out.data_ptr()
+        a.score_out, a.pos_out, a.src_out = ptr(score_out), ptr(pos_out), ptr(src_out)
+        a.keep, a.n_sink, a.n_recent = keep, n_sink, n_recent
+        self._call(self._lib.vtx_kv_evict_paged, a, stream, *self._ws)
+        return kv_len_out
 
 
 # ---- realtime encoder: chunk plan and device-side stitch ---------------------
