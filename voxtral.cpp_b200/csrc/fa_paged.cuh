@@ -29,6 +29,7 @@ struct PagedAttnArgs {
     int Hq, G;
     float scale, softcap;                                   // logits: scale * s, or softcap * tanh(scale / softcap * s)
     int causal, window;
+    int min_rows;             // streams with at most so many query rows per KV head are another kernel's
 };
 
 // Logit in log2 units of a dot product.
@@ -87,7 +88,7 @@ fa_paged_kernel(const PagedAttnArgs a)
     if (blockIdx.x == 0 && s.n_new > a.kv.max_new) paged_report(a.kv, VTX_KERR_BOUND);
     const int rows = min(s.n_new, a.kv.max_new) * a.G;
     const int r_first = blockIdx.x * 64;
-    if (r_first >= rows) return;
+    if (r_first >= rows || rows <= a.min_rows) return;
 
     const int off = s.len - s.n_new;                        // row of token 0
     int row[2], tok[2], lo[2], hi[2];

@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <cuda_fp16.h>
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
@@ -15,6 +16,7 @@
 #include "fa_prefill_sm100.cuh"
 #include "paged_kv.cuh"
 #include "fa_paged.cuh"
+#include "fa_paged_decode.cuh"
 #include "kv_score.cuh"
 #include "kv_evict.cuh"
 
@@ -92,10 +94,78 @@ int check_params(const vtx_fa_params *p) {
     return VTX_OK;
 }
 
+// Allows a kernel its shared memory, once per device (`done`: one flag each).
 template <typename K>
-int set_smem(K kernel, int bytes) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess
-               ? VTX_OK : VTX_ERR_CUDA;
+int allow_smem(K kernel, int bytes, std::atomic<int> (&done)[kMaxDevices]) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (done[dev].load(std::memory_order_acquire)) return VTX_OK;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+        return VTX_ERR_CUDA;
+    done[dev].store(1, std::memory_order_release);
+    return VTX_OK;
+}
+
+int current_sms() {
+    int sms = 148, dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    cudaGetLastError();
+    return sms;
+}
+
+// Streams of at most kFewRows query rows per KV head go to the streaming kernel.
+constexpr int kFewRows = 16;
+
+struct DecodePlan {
+    bool use;                 // the streaming kernel is launched
+    int rows;                 // its row count, 8 or 16
+    PagedSplit split;
+    size_t o_bytes, bytes;
+};
+
+// Splits: about two waves of two CTAs per SM over (streams x KV heads), at
+// most 128 tiles (2048 keys) each so that ragged lengths spread evenly, and at
+// least one tile per warp.
+DecodePlan plan_decode(const vtx_paged_kv *p, int G, int sms) {
+    DecodePlan d{};
+    // the only stream may bring more tokens than fit: then all go one way
+    d.use = p->max_new * (long long)G <= kFewRows || p->n_seq > 1;
+    if (!d.use || G > kFewRows || p->n_seq == 0) {
+        d.use = false;
+        return d;
+    }
+    d.rows = p->max_new * (long long)G <= 8 ? 8 : 16;
+    const long long base = (long long)p->n_seq * p->k.ne[2];
+    const int tiles = std::max(1, (p->max_kv_len + 15) / 16);
+    long long want = std::max<long long>((4LL * sms + base - 1) / base, (tiles + 127) / 128);
+    want = std::min<long long>(want, (tiles + 3) / 4);
+    d.split.n_splits = (int)want;
+    d.split.tiles = (int)((tiles + want - 1) / want);
+    if (want > 1) {
+        const size_t rows = (size_t)base * want * d.rows;
+        d.o_bytes = align_up(rows * p->k.ne[0] * 4, 256);
+        d.bytes = d.o_bytes + align_up(rows * 8, 256);
+    }
+    return d;
+}
+
+template <int D, int KVT, int ROWS>
+int launch_decode(const PagedAttnArgs &a, const PagedSplit &sp, cudaStream_t st) {
+    using C = PagedDecodeCfg<D, KVT>;
+    static std::atomic<int> done[kMaxDevices];
+    int rc = allow_smem(fa_paged_decode_kernel<D, KVT, ROWS>, C::SMEM, done);
+    if (rc != VTX_OK) return rc;
+    const long long ctas = (long long)a.kv.n_seq * a.kv.Hkv * sp.n_splits;
+    if (ctas > 0x7fffffffLL) return VTX_ERR_UNSUPPORTED;
+    rc = launch_pdl(fa_paged_decode_kernel<D, KVT, ROWS>, dim3((unsigned)ctas), dim3(128), C::SMEM, st, a, sp);
+    if (rc != VTX_OK || sp.n_splits == 1) return rc;
+    return launch_pdl(fa_paged_combine_kernel<D, ROWS>, dim3((unsigned)a.kv.Hkv, (unsigned)a.kv.n_seq), dim3(128), 0,
+                      st, a, sp);
+}
+
+template <int D, int KVT>
+int launch_decode_rows(const PagedAttnArgs &a, const DecodePlan &d, cudaStream_t st) {
+    return d.rows == 8 ? launch_decode<D, KVT, 8>(a, d.split, st) : launch_decode<D, KVT, 16>(a, d.split, st);
 }
 
 template <int D, int KVT>
@@ -182,7 +252,7 @@ size_t vtx_flash_attn_paged_workspace(const vtx_paged_kv *kv, int32_t n_head_q) 
     if (check_paged(kv) != VTX_OK || n_head_q < 1 || n_head_q % kv->k.ne[2] ||
         n_head_q / kv->k.ne[2] > kMaxGroup)
         return (size_t)-1;
-    return 0;
+    return plan_decode(kv, n_head_q / (int)kv->k.ne[2], current_sms()).bytes;
 }
 
 int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, size_t workspace_bytes, void *stream) {
@@ -201,12 +271,12 @@ int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, si
     if (!d->data) return VTX_ERR_NULL;
     if (reinterpret_cast<uintptr_t>(d->data) % 16 || d->nb[1] % 16 || d->nb[2] % 16) return VTX_ERR_STRIDE;
     const int Hq = (int)q->ne[2];
-    const size_t need = vtx_flash_attn_paged_workspace(kv, Hq);
-    if (workspace_bytes < need || (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256)))
-        return VTX_ERR_WORKSPACE;
     DeviceState *ds = nullptr;
     rc = ensure_device(&ds);
     if (rc != VTX_OK) return rc;
+    DecodePlan dp = plan_decode(kv, Hq / (int)kv->k.ne[2], ds->sms);
+    if (workspace_bytes < dp.bytes || (dp.bytes && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256)))
+        return VTX_ERR_WORKSPACE;
     PagedAttnArgs a{};
     a.kv = view_of(kv, ds);
     a.q = static_cast<const char *>(q->data); a.q_f16 = q->type == VTX_TYPE_F16;
@@ -218,8 +288,16 @@ int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, si
     a.scale = p->params->scale; a.softcap = p->params->logit_softcap;
     a.causal = p->params->causal != 0; a.window = p->params->window;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool f16 = kv->k.type == VTX_TYPE_F16;
-    if (kv->k.ne[0] == 64) return f16 ? launch_attn<64, 1>(a, st) : launch_attn<64, 8>(a, st);
+    const bool f16 = kv->k.type == VTX_TYPE_F16, d64 = kv->k.ne[0] == 64;
+    if (dp.use) {
+        dp.split.part_o = static_cast<float *>(workspace);
+        dp.split.part_ml = reinterpret_cast<float *>(static_cast<char *>(workspace) + dp.o_bytes);
+        rc = d64 ? (f16 ? launch_decode_rows<64, 1>(a, dp, st) : launch_decode_rows<64, 8>(a, dp, st))
+                 : (f16 ? launch_decode_rows<128, 1>(a, dp, st) : launch_decode_rows<128, 8>(a, dp, st));
+        if (rc != VTX_OK || kv->max_new * (long long)a.G <= kFewRows) return rc;
+        a.min_rows = dp.rows;
+    }
+    if (d64) return f16 ? launch_attn<64, 1>(a, st) : launch_attn<64, 8>(a, st);
     return f16 ? launch_attn<128, 1>(a, st) : launch_attn<128, 8>(a, st);
 }
 
@@ -295,10 +373,9 @@ int vtx_kv_evict_paged(const vtx_kv_evict_paged_args *p, void *workspace, size_t
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int keys = std::min(kv->max_kv_len, kEvictKeysInSmem) * 4;
     if (kv->max_kv_len <= kEvictKeysInSmem) {
-        if (keys > 32 * 1024) {
-            rc = set_smem(kv_evict_select_kernel<true>, kEvictKeysInSmem * 4);
-            if (rc != VTX_OK) return rc;
-        }
+        static std::atomic<int> done[kMaxDevices];
+        rc = allow_smem(kv_evict_select_kernel<true>, kEvictKeysInSmem * 4, done);
+        if (rc != VTX_OK) return rc;
         rc = launch_pdl(kv_evict_select_kernel<true>, dim3((unsigned)e.items), dim3(kEvictThreads), (size_t)keys, st, a);
     } else {
         rc = launch_pdl(kv_evict_select_kernel<false>, dim3((unsigned)e.items), dim3(kEvictThreads), 0, st, a);
