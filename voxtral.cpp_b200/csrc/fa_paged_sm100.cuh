@@ -1,0 +1,560 @@
+// fa_paged_sm100.cuh — tensor-core attention of chunks of new tokens over a
+// paged F16 cache (tcgen05 / TMEM / TMA): the decoder prefill node of
+// src/voxtral.cpp:1802 for ragged batches, bound by the tensor core and the
+// exponentials (4 D flops and one exp per query row and visible key).
+//
+// A CTA owns a group of two 128-row Q tiles of one stream and KV head (row =
+// token * G + head of the group, T = 128 / G tokens a tile) and one split of
+// its key tiles of 128.  Two softmax warpgroups, one per Q tile (a thread per
+// row = TMEM lane), take turns on the tensor core; a third warpgroup holds the
+// TMA and the MMA warp and gives its registers away (setmaxnreg).  Per key tile
+// and Q tile: S = Q K^T into TMEM, P = 2^(x - m) over S's first half columns,
+// O += P V with P read from TMEM.  Shared memory: both Q tiles, and a ring of K
+// and V tiles, all in the 128-byte swizzle.
+//
+// Pages: a tensor map (dim, row, head, page) per pool; a key tile is one box of
+// 64 dims x min(page, 128) rows per page and half row, a lane of the TMA warp
+// each.  Pages without a row that the group sees are not touched; rows of the
+// other pages outside the group's key range may hold anything, so the softmax
+// warps clear those V rows in shared memory before P V (masked P is 0, and
+// 0 * NaN is not), while masked scores are replaced.
+//
+// Part of the exponentials runs on the FMA pipe: 2^x = 2^j p(f), j = round(x),
+// with p the degree-4 polynomial of least relative error (2.6e-6) on
+// [-1/2, 1/2], fitted here by an exchange.  The row sums are taken of the f32
+// P, so lse carries neither P's rounding to half nor more than that error.
+//
+// Splits: with few groups the key tiles of a group are cut into up to n_splits
+// ranges; their (m, l, O) are merged by fa_paged_tile_combine_kernel.
+#pragma once
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cstdint>
+#include "vtx_ptx.cuh"
+#include "paged_kv.cuh"
+#include "fa_paged.cuh"
+#include "fa_prefill_sm100.cuh"
+
+namespace vtx {
+
+struct PagedTile {
+    int T;                    // tokens per Q tile: 128 / G
+    int groups;               // bound on the groups of all streams
+    int n_splits, min_tiles;  // splits of a group's key tiles at most, key tiles per split at least
+    float *part_o, *part_ml;  // [n_splits][n_tokens][Hq][D], ... [2] (m, l)
+};
+
+template <int D> struct PagedTileCfg {
+    static constexpr int BN = 128, SUB = D / 64;
+    static constexpr int TILE = 128 * D * 2;
+    static constexpr int STAGES = D == 64 ? 4 : 2;
+    static constexpr int Q_OFF = 0, K_OFF = 2 * TILE, V_OFF = K_OFF + STAGES * TILE;
+    static constexpr int BAR_OFF = V_OFF + STAGES * TILE;
+    static constexpr int NBARS = 1 + 3 * STAGES + 6;
+    static constexpr int SMEM = BAR_OFF + NBARS * 8 + 32 + 1024;       // + alignment slack
+    static constexpr int NTHREADS = 384, TMA_WARP = 8, MMA_WARP = 9;
+    static constexpr int REG_SOFTMAX = 224, REG_PRODUCER = 56;         // 256 x 224 + 128 x 56 = 384 x 168
+    __host__ __device__ static constexpr int s_col(int t) { return t * 128; }
+    __host__ __device__ static constexpr int o_col(int t) { return 256 + t * D; }
+};
+
+// 2^x of a pair on the FMA pipe, x <= ~8; below -125 the result is about 2^-125.
+__device__ __forceinline__ void paged_exp2_pair(float &a, float &b) {
+    const float kRound = 12582912.0f;                    // 1.5 * 2^23
+    a = fmaxf(a, -125.0f);
+    b = fmaxf(b, -125.0f);
+    const uint64_t x = pk2(a, b);
+    const uint64_t t = fadd2(x, pk2(kRound, kRound));
+    const uint64_t f = fsub2(x, fadd2(t, pk2(-kRound, -kRound)));
+    uint64_t p = ffma2(pk2(0.00957010191f, 0.00957010191f), f, pk2(0.0559178603f, 0.0559178603f));
+    p = ffma2(p, f, pk2(0.240247448f, 0.240247448f));
+    p = ffma2(p, f, pk2(0.693121815f, 0.693121815f));
+    p = ffma2(p, f, pk2(0.999999261f, 0.999999261f));
+    float pa, pb, ta, tb;
+    upk2(p, pa, pb);
+    upk2(t, ta, tb);
+    a = __int_as_float(__float_as_int(pa) + (__float_as_int(ta) << 23));
+    b = __int_as_float(__float_as_int(pb) + (__float_as_int(tb) << 23));
+}
+
+// Groups (pairs of Q tiles) of a stream with n_new tokens.
+__device__ __forceinline__ int paged_groups(int n_new, const PagedAttnArgs &a, const PagedTile &tl) {
+    return n_new * a.G > a.min_rows ? (n_new + 2 * tl.T - 1) / (2 * tl.T) : 0;
+}
+
+// Key tiles [j0, j1) of a group whose first token is tok0, and their splits.
+struct PagedRange {
+    int lo, hi;               // keys some token of the group sees
+    int j0, j1, per, n;
+};
+__device__ __forceinline__ PagedRange paged_range(const PagedSeq &s, int tok0, const PagedAttnArgs &a,
+                                                  const PagedTile &tl) {
+    PagedRange r;
+    const int off = s.len - s.n_new, last = min(s.n_new, tok0 + 2 * tl.T) - 1;
+    r.hi = a.causal ? off + last : s.len - 1;
+    r.lo = a.window > 0 ? max(0, off + tok0 - a.window + 1) : 0;
+    r.j0 = r.hi >= r.lo ? r.lo >> 7 : 0;
+    r.j1 = r.hi >= r.lo ? (r.hi >> 7) + 1 : 0;
+    r.per = max(tl.min_tiles, (r.j1 - r.j0 + tl.n_splits - 1) / tl.n_splits);
+    r.n = max(1, (r.j1 - r.j0 + r.per - 1) / r.per);
+    return r;
+}
+
+template <int D, bool UF>
+__global__ void __launch_bounds__(PagedTileCfg<D>::NTHREADS, 1)
+fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                      const __grid_constant__ CUtensorMap tmQ, const PagedAttnArgs a, const PagedTile tl)
+{
+    using C = PagedTileCfg<D>;
+    extern __shared__ __align__(1024) char smem_raw[];
+    char *smem = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *q_full = reinterpret_cast<uint64_t *>(smem + C::BAR_OFF);
+    uint64_t *k_full = q_full + 1;
+    uint64_t *v_full = k_full + C::STAGES;
+    uint64_t *kv_empty = v_full + C::STAGES;
+    uint64_t *s_full = kv_empty + C::STAGES;       // [2]
+    uint64_t *p_full = s_full + 2;                 // [2]
+    uint64_t *o_tile = p_full + 2;                 // [2]
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(o_tile + 2);
+    int *found = reinterpret_cast<int *>(tmem_slot + 2);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int g = blockIdx.x % a.kv.Hkv;
+    const int split = (blockIdx.x / a.kv.Hkv) % tl.n_splits;
+
+    if (tid == 32) {
+        mbar_init(q_full, a.q_f16 ? 1 : 8);        // the TMA lane, or one arrival per softmax warp
+        for (int i = 0; i < C::STAGES; ++i) {
+            mbar_init(&k_full[i], 1);
+            mbar_init(&v_full[i], 1);
+            mbar_init(&kv_empty[i], 1);
+        }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&s_full[t], 1);
+            mbar_init(&p_full[t], 4);
+            mbar_init(&o_tile[t], 1);
+        }
+        fence_mbar_init();
+    }
+    if (warp == C::TMA_WARP && lane == 0) {
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
+        if (a.q_f16) tma_prefetch_desc(&tmQ);
+    }
+    grid_dep_wait();
+    grid_dep_launch();
+    if (warp == 0) {                               // the stream and group of this CTA
+        const int want = blockIdx.x / (a.kv.Hkv * tl.n_splits);
+        int base = 0, b = -1, grp = 0;
+        for (int i0 = 0; i0 < a.kv.n_seq && b < 0; i0 += 32) {
+            const int i = i0 + lane;
+            const int cnt = i < a.kv.n_seq ? paged_groups(min(paged_seq(a.kv, i).n_new, a.kv.max_new), a, tl) : 0;
+            int inc = cnt;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += x;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, want < base + inc);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                b = i0 + l;
+                // a stream's last group, whose key range is the longest, first
+                grp = base + __shfl_sync(0xffffffffu, inc, l) - 1 - want;
+            } else {
+                base += __shfl_sync(0xffffffffu, inc, 31);
+            }
+        }
+        if (lane == 0) {
+            found[0] = b;
+            found[1] = grp;
+        }
+    }
+    __syncthreads();
+    const int b = found[0];
+    if (b < 0) return;
+    PagedSeq s = paged_seq(a.kv, b);
+    if (s.n_new > a.kv.max_new) {                  // what exceeds the bound is not served
+        if (tid == 0) paged_report(a.kv, VTX_KERR_BOUND);
+    }
+    const int n_serve = min(s.n_new, a.kv.max_new);
+    const int tok0 = found[1] * 2 * tl.T;
+    const PagedRange rg = paged_range(s, tok0, a, tl);
+    if (split >= rg.n) return;
+    const int jb = rg.j0 + split * rg.per;
+    const int n_iter = max(0, min(jb + rg.per, rg.j1) - jb);
+    const bool two = tok0 + tl.T < n_serve;        // the second Q tile holds tokens
+
+    if (warp == C::MMA_WARP) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int off = s.len - s.n_new;
+
+    if (warp < 8) {
+        setmaxnreg_inc<C::REG_SOFTMAX>();
+        // =================== softmax warpgroups ===============================
+        const int t = warp >> 2, r = tid & 127;
+        const int tok = tok0 + t * tl.T + r / a.G, head = g * a.G + r % a.G;
+        const bool row_ok = r < tl.T * a.G && tok < n_serve;
+        const int iters = t == 0 || two ? n_iter : 0;
+        bool ok = true;
+        int lo = 1, hi = 0;
+        if (row_ok) {
+            hi = a.causal ? off + tok : s.len - 1;
+            lo = a.window > 0 ? max(0, off + tok - a.window + 1) : 0;
+        }
+        char *qtile = smem + C::Q_OFF + t * C::TILE;
+        if (!a.q_f16) {                            // F32 q: each thread rounds its row to half
+            const char *src = a.q + (long long)(s.q0 + tok) * a.q_nbt + (long long)head * a.q_nbh;
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+                uint4 pk = make_uint4(0u, 0u, 0u, 0u);
+                if (row_ok) {
+                    const float4 x = *reinterpret_cast<const float4 *>(src + c * 32);
+                    const float4 y = *reinterpret_cast<const float4 *>(src + c * 32 + 16);
+                    pk = make_uint4(pack_half2(x.x, x.y), pack_half2(x.z, x.w), pack_half2(y.x, y.y), pack_half2(y.z, y.w));
+                }
+                *reinterpret_cast<uint4 *>(qtile + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = pk;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t s_addr = tmem + lane_base + C::s_col(t);
+        const uint32_t o_addr = tmem + lane_base + C::o_col(t);
+        const float cx = UF ? 1.0f : a.scale * kLog2e;
+        float m_run = -INFINITY, l_run = 0.0f;
+
+        for (int it = 0; it < iters; ++it) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], it & 1, a.kv.err, VTX_KERR_S));
+            if (!ok) break;
+            tc_fence_after();
+            float x[128];
+            {
+                uint32_t raw[128];
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    tmem_ld32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&raw[c * 32]));
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 128; ++i) x[i] = __uint_as_float(raw[i]);
+            }
+            const int k0 = (jb + it) * C::BN;
+            if (UF) {
+#pragma unroll
+                for (int i = 0; i < 128; ++i) x[i] = paged_logit(x[i], a.scale, a.softcap);
+            }
+            const bool full = !row_ok || (k0 >= lo && k0 + C::BN - 1 <= hi);
+            if (__any_sync(0xffffffffu, !full)) {
+#pragma unroll
+                for (int i = 0; i < 128; ++i) x[i] = (k0 + i < lo || k0 + i > hi) ? -INFINITY : x[i];
+            }
+            // V rows outside the group's key range hold anything: clear them
+            if (k0 < rg.lo || k0 + C::BN - 1 > rg.hi) {
+                const int st = it % C::STAGES;
+                ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (it / C::STAGES) & 1, a.kv.err, VTX_KERR_KV));
+                if (!ok) break;
+                if (k0 + r < rg.lo || k0 + r > rg.hi) {
+                    char *v = smem + C::V_OFF + st * C::TILE + r * 128;
+#pragma unroll
+                    for (int i = 0; i < C::SUB * 8; ++i)
+                        *reinterpret_cast<uint4 *>(v + (i >> 3) * 16384 + (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_proxy_async_smem();
+            }
+            float mx8[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                mx8[k] = fmaxf(x[16 * k], x[16 * k + 1]);
+#pragma unroll
+                for (int i = 2; i < 16; i += 2) mx8[k] = fmax3(mx8[k], x[16 * k + i], x[16 * k + i + 1]);
+            }
+            const float mx = fmax3(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]),
+                                   fmaxf(mx8[6], mx8[7])) * cx;
+            bool rescale = false;
+            float alpha = 1.0f;
+            if (mx > m_run + 8.0f) {               // the reference moves only on a 2^8 jump
+                if (m_run != -INFINITY) {
+                    alpha = ex2(m_run - mx);
+                    rescale = it > 0;
+                }
+                m_run = mx;
+                l_run *= alpha;
+            }
+            const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
+            const uint64_t cx2 = pk2(cx, cx), nm2 = pk2(neg_m, neg_m);
+            uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
+            uint32_t pk[64];
+#pragma unroll
+            for (int i = 0; i < 64; ++i) {
+                float e0, e1;
+                upk2(ffma2(pk2(x[2 * i], x[2 * i + 1]), cx2, nm2), e0, e1);
+                if ((i & 3) == 3) {                // every fourth pair off the MUFU
+                    paged_exp2_pair(e0, e1);
+                } else {
+                    e0 = ex2(e0);
+                    e1 = ex2(e1);
+                }
+                sum2[i & 3] = fadd2(sum2[i & 3], pk2(e0, e1));
+                pk[i] = pack_half2(e0, e1);
+            }
+            {
+                float sa, sb;
+                upk2(fadd2(fadd2(sum2[0], sum2[1]), fadd2(sum2[2], sum2[3])), sa, sb);
+                l_run += sa + sb;
+            }
+            tmem_st32(s_addr, *reinterpret_cast<const uint32_t(*)[32]>(&pk[0]));
+            tmem_st32(s_addr + 32, *reinterpret_cast<const uint32_t(*)[32]>(&pk[32]));
+            // tcgen05.ld / st are warp-collective: the warp rescales when any row needs it
+            if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[32];
+                    tmem_ld32(o_addr + c * 32, o);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                    tmem_st32(o_addr + c * 32, o);
+                }
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[t]);
+        }
+        // ---- write-back: rows staged in this tile's own Q tile
+        if (iters > 0) {
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_tile[t], 0, a.kv.err, VTX_KERR_O));
+            tc_fence_after();
+        }
+        if (m_run == -INFINITY) l_run = 0.0f;      // saw nothing (the sum holds 2^-125s)
+        const bool part = rg.n > 1;
+        const float inv = part ? 1.0f : (l_run == 0.0f ? 0.0f : 1.0f / l_run);
+        const long long row = (long long)(s.q0 + tok) * a.Hq + head;
+        if (row_ok && ok) {
+            if (part)
+                reinterpret_cast<float2 *>(tl.part_ml)[(long long)split * a.kv.n_tokens * a.Hq + row] =
+                    make_float2(m_run, l_run);
+            else if (a.lse)
+                a.lse[row] = l_run == 0.0f ? -INFINITY : (m_run + log2f(l_run)) * kLn2;
+        }
+        if (t == 0 || two) {
+            // staged W bytes a row at a time (16-byte chunk c of row r at c ^ (r & 7))
+            constexpr int W = C::TILE / 128, CH = W / 16;
+            const bool f16 = !part && a.d_f16;
+            const int bytes = D * (f16 ? 2 : 4);
+            if (iters == 0) asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");   // after any Q rows written here
+            for (int c0 = 0; c0 < bytes; c0 += W) {
+                if (c0 > 0) asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");   // the staged rows were read
+                if (ok) {
+                    for (int c = 0; c < W / (f16 ? 64 : 128); ++c) {   // 32 columns
+                        uint32_t o[32];
+                        if (iters > 0) {
+                            tmem_ld32(o_addr + c0 / (f16 ? 2 : 4) + c * 32, o);
+                            tmem_ld_wait();
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = 0u;
+                        }
+                        float y[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(o[i]) * inv;
+                        if (f16) {
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+                                *reinterpret_cast<uint4 *>(qtile + r * W + (((c * 4 + q) ^ (r & 7)) << 4)) =
+                                    make_uint4(pack_half2(y[8 * q], y[8 * q + 1]), pack_half2(y[8 * q + 2], y[8 * q + 3]),
+                                               pack_half2(y[8 * q + 4], y[8 * q + 5]), pack_half2(y[8 * q + 6], y[8 * q + 7]));
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < 8; ++q)
+                                *reinterpret_cast<float4 *>(qtile + r * W + (((c * 8 + q) ^ (r & 7)) << 4)) =
+                                    make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+                        }
+                    }
+                }
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");               // staged
+                if (ok) {
+                    for (int i = r; i < 128 * CH; i += 128) {
+                        const int rr = i / CH, ch = i % CH;
+                        const int tk = tok0 + t * tl.T + rr / a.G, hd = g * a.G + rr % a.G;
+                        if (rr >= tl.T * a.G || tk >= n_serve) break;
+                        const uint4 v = *reinterpret_cast<const uint4 *>(qtile + rr * W + ((ch ^ (rr & 7)) << 4));
+                        char *p = part ? reinterpret_cast<char *>(tl.part_o + (((long long)split * a.kv.n_tokens + s.q0 + tk) * a.Hq + hd) * D)
+                                       : a.dst + (long long)(s.q0 + tk) * a.d_nbt + (long long)hd * a.d_nbh;
+                        *reinterpret_cast<uint4 *>(p + c0 + ch * 16) = v;
+                    }
+                }
+            }
+        }
+    } else {
+        setmaxnreg_dec<C::REG_PRODUCER>();
+        if (warp == C::TMA_WARP) {
+            // =================== TMA: Q, then K and V tile by tile ============
+            if (a.q_f16 && n_iter > 0) {
+                if (lane == 0) {
+                    const int nq = two ? 2 : 1;
+                    mbar_arrive_expect_tx(q_full, (uint32_t)(nq * C::SUB * 128 * tl.T * a.G));
+                    for (int t = 0; t < nq; ++t)
+                        for (int sub = 0; sub < C::SUB; ++sub)
+                            tma_load_4d(smem + C::Q_OFF + t * C::TILE + sub * 16384, &tmQ, q_full, sub * 64, g * a.G,
+                                        s.q0 + tok0 + t * tl.T, 0);
+                }
+                __syncwarp();
+            }
+            const int rows_box = min(128, 1 << a.kv.shift), per_tile = 128 / rows_box;   // boxes of a half-width tile
+            const int mask = (1 << a.kv.shift) - 1;
+            // lane = box of a tile; 64 boxes at most (16-row pages: 8 pages x SUB x {K, V} = 32 for D = 128)
+            const int kvsel = lane / (per_tile * C::SUB);                   // 0: K, 1: V, more: idle
+            const int sub = (lane / per_tile) % C::SUB, pg = lane % per_tile;
+            const bool mine = kvsel < 2;
+            auto page_at = [&](int it) -> int {    // this lane's page of tile it, -1: none needed
+                const int y = (jb + it) * C::BN + pg * rows_box;
+                if (!mine || it >= n_iter || y > rg.hi || y + rows_box <= rg.lo) return -1;
+                return max(paged_page(a.kv, b, y), 0);
+            };
+            int issued = 0, next = page_at(0);
+            for (int it = 0; it < n_iter; ++it) {
+                const int st = it % C::STAGES, cur = next;
+                next = page_at(it + 1);
+                if (it >= C::STAGES &&
+                    !__all_sync(0xffffffffu, mbar_wait(&kv_empty[st], ((it / C::STAGES) - 1) & 1, a.kv.err, VTX_KERR_KV)))
+                    break;
+                issued = it + 1;
+                const unsigned live = __ballot_sync(0xffffffffu, cur >= 0);
+                if (lane == 0) {
+                    const int n = __popc(live) / 2;                         // K's boxes; V has the same
+                    mbar_arrive_expect_tx(&k_full[st], (uint32_t)(n * rows_box * 128));
+                    mbar_arrive_expect_tx(&v_full[st], (uint32_t)(n * rows_box * 128));
+                }
+                __syncwarp();
+                if (cur >= 0) {
+                    const int y = (jb + it) * C::BN + pg * rows_box;
+                    char *dst = smem + (kvsel ? C::V_OFF : C::K_OFF) + st * C::TILE + sub * 16384 + pg * rows_box * 128;
+                    if (kvsel) tma_load_4d(dst, &tmV, &v_full[st], sub * 64, y & mask, g, cur);
+                    else tma_load_4d(dst, &tmK, &k_full[st], sub * 64, y & mask, g, cur);
+                }
+                __syncwarp();
+            }
+            // the last loads must have landed before shared memory is released
+            for (int it = max(0, issued - C::STAGES); it < issued; ++it) {
+                mbar_wait(&k_full[it % C::STAGES], (it / C::STAGES) & 1, a.kv.err, VTX_KERR_KV);
+                mbar_wait(&v_full[it % C::STAGES], (it / C::STAGES) & 1, a.kv.err, VTX_KERR_KV);
+            }
+            if (a.q_f16 && n_iter > 0) mbar_wait(q_full, 0, a.kv.err, VTX_KERR_Q);
+        } else if (warp == C::MMA_WARP && n_iter > 0) {
+            // =================== MMA issuer (warp converged, one elected lane) =
+            const uint32_t lead = elect_one();
+            constexpr uint32_t IDESC_QK = idesc_f16_f32(128, 128, 0, 0);
+            constexpr uint32_t IDESC_PV = idesc_f16_f32(128, D, 0, 1);
+            constexpr uint32_t HI = (1024u >> 4) | (1u << 14) | (2u << 29);   // SBO 1024, v1, 128-byte swizzle
+            const uint32_t sbase = smem_u32(smem);
+            const uint32_t lo_q = ((sbase + C::Q_OFF) >> 4) | (1u << 16);
+            const uint32_t lo_k = ((sbase + C::K_OFF) >> 4) | (1u << 16);
+            const uint32_t lo_v = ((sbase + C::V_OFF) >> 4) | ((16384u >> 4) << 16);   // LBO: next 64 columns
+            constexpr uint32_t T16 = C::TILE >> 4;
+            const int nt = two ? 2 : 1;
+            bool good = __all_sync(0xffffffffu, mbar_wait(q_full, 0, a.kv.err, VTX_KERR_Q));
+            tc_fence_after();
+            auto issue_qk = [&](int t, int st) {
+                const uint32_t d = tmem + C::s_col(t), q = lo_q + t * T16, k = lo_k + st * T16;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t ko = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+                    mma_f16_ss_w(lead, d, desc64(q + ko, HI), desc64(k + ko, HI), IDESC_QK, kk > 0);
+                }
+                mma_commit_w(lead, &s_full[t]);
+            };
+            auto issue_pv = [&](int t, int st, uint32_t acc) {
+                const uint32_t p = tmem + C::s_col(t), d = tmem + C::o_col(t), v = lo_v + st * T16;
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk)
+                    mma_f16_ts_w(lead, d, p + kk * 8, desc64(v + kk * (2048 >> 4), HI), IDESC_PV, kk > 0 ? 1u : acc);
+            };
+            for (int it = 0; it <= n_iter && good; ++it) {
+                const int st = it % C::STAGES, pst = (it + C::STAGES - 1) % C::STAGES;
+                for (int t = 0; t < nt && good; ++t) {
+                    if (it > 0) {
+                        if (t == 0) good = __all_sync(0xffffffffu, mbar_wait(&v_full[pst], ((it - 1) / C::STAGES) & 1, a.kv.err, VTX_KERR_KV));
+                        if (good) good = __all_sync(0xffffffffu, mbar_wait(&p_full[t], (it - 1) & 1, a.kv.err, VTX_KERR_P));
+                        if (!good) break;
+                        tc_fence_after();
+                        issue_pv(t, pst, it > 1 ? 1u : 0u);
+                        if (it == n_iter) mma_commit_w(lead, &o_tile[t]);
+                    }
+                    if (it < n_iter) {
+                        if (t == 0) good = __all_sync(0xffffffffu, mbar_wait(&k_full[st], (it / C::STAGES) & 1, a.kv.err, VTX_KERR_KV));
+                        if (!good) break;
+                        tc_fence_after();
+                        issue_qk(t, st);
+                    }
+                }
+                if (good && it > 0) mma_commit_w(lead, &kv_empty[pst]);
+            }
+            if (!good) {                           // release the write-back after a failed wait
+                for (int t = 0; t < nt; ++t) mma_commit_w(lead, &o_tile[t]);
+            }
+            // every MMA has retired before TMEM is released
+            for (int t = 0; t < nt; ++t) mbar_wait(&o_tile[t], 0, a.kv.err, VTX_KERR_O);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == C::MMA_WARP) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Merges the splits: grid (n_tokens), a warp per query head, a lane per 4 dims.
+template <int D>
+__global__ void __launch_bounds__(256)
+fa_paged_tile_combine_kernel(const PagedAttnArgs a, const PagedTile tl)
+{
+    grid_dep_wait();
+    grid_dep_launch();
+    const int t = blockIdx.x;
+    const int b = paged_find(a.kv, t);
+    if (b >= a.kv.n_seq) return;
+    const PagedSeq s = paged_seq(a.kv, b);
+    const int tok = t - s.q0;
+    if (tok < 0 || tok >= min(s.n_new, a.kv.max_new) || paged_groups(min(s.n_new, a.kv.max_new), a, tl) == 0) return;
+    const int n = paged_range(s, tok / (2 * tl.T) * 2 * tl.T, a, tl).n;
+    if (n == 1) return;
+    const int lane = threadIdx.x & 31, d = lane * 4;
+    const long long step = (long long)a.kv.n_tokens * a.Hq;
+    for (int h = threadIdx.x >> 5; h < a.Hq; h += 8) {
+        const long long row = (long long)t * a.Hq + h;
+        float top = -INFINITY;
+        for (int i = 0; i < n; ++i) top = fmaxf(top, tl.part_ml[(i * step + row) * 2]);
+        float l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (top != -INFINITY) {
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) {
+                const float2 y = reinterpret_cast<const float2 *>(tl.part_ml)[i * step + row];
+                const float f = ex2(y.x - top);
+                l = fmaf(f, y.y, l);
+                if (d < D) {
+                    const float4 v = *reinterpret_cast<const float4 *>(tl.part_o + (i * step + row) * D + d);
+                    acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y);
+                    acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
+                }
+            }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (d < D) {
+            paged_store2(a, t, h, d, acc.x * inv, acc.y * inv);
+            paged_store2(a, t, h, d + 2, acc.z * inv, acc.w * inv);
+        }
+        if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
+    }
+}
+
+}  // namespace vtx

@@ -17,6 +17,7 @@
 #include "paged_kv.cuh"
 #include "fa_paged.cuh"
 #include "fa_paged_decode.cuh"
+#include "fa_paged_sm100.cuh"
 #include "kv_score.cuh"
 #include "kv_evict.cuh"
 
@@ -84,6 +85,7 @@ int check_q(const vtx_paged_kv *p, const vtx_tensor *q) {
     if (p->n_tokens == 0) return VTX_OK;
     if (!q->data || !p->q_start) return VTX_ERR_NULL;
     if (reinterpret_cast<uintptr_t>(q->data) % 16 || q->nb[1] % 16 || q->nb[2] % 16) return VTX_ERR_STRIDE;
+    if (q->nb[1] >= (1ULL << 40) || q->nb[2] >= (1ULL << 40)) return VTX_ERR_STRIDE;
     return VTX_OK;
 }
 
@@ -175,6 +177,103 @@ int launch_attn(const PagedAttnArgs &a, cudaStream_t st) {
                       dim3(128), 0, st, a);
 }
 
+// The tensor-core kernel: F16 caches, when a stream may bring more rows than
+// the streaming kernel takes.
+struct TilePlan {
+    bool use;
+    PagedTile tile;
+    size_t o_bytes, bytes;
+};
+
+TilePlan plan_tile(const vtx_paged_kv *p, int G, int Hq, int min_rows, int sms) {
+    TilePlan t{};
+    t.use = p->k.type == VTX_TYPE_F16 && p->max_new * (long long)G > min_rows && p->n_seq > 0;
+    if (!t.use) return t;
+    const int Hkv = (int)p->k.ne[2], D = (int)p->k.ne[0];
+    t.tile.T = 128 / G;
+    const long long pair = 2 * t.tile.T;
+    // streams with more than min_rows rows, and what rounding each up to whole groups adds
+    const long long streams = std::min<long long>(p->n_seq, p->n_tokens / (min_rows / G + 1));
+    t.tile.groups = (int)((p->n_tokens + streams * (pair - 1)) / pair);
+    t.tile.min_tiles = 2;
+    // Splits of a group's key tiles: the number of least estimated time.  A key
+    // tile of a group takes about 2.2 us (D = 128); a merge writes and reads every
+    // row once per split at about 4 TB/s and costs a launch.  One stream: its
+    // groups are about equal, so whole waves count.  Several: lengths spread, so
+    // the average load plus half a CTA's time.
+    const int tiles = std::max(1, (p->max_kv_len + 127) / 128);
+    const double tile_us = D == 128 ? 2.2 : 1.6;
+    const double merge_us = (double)p->n_tokens * Hq * D * 8 / 4e6;
+    double best = 1e30;
+    t.tile.n_splits = 1;
+    for (int s = 1; s <= 32 && s <= (tiles + 1) / 2; ++s) {
+        const double each = (double)((tiles + s - 1) / s);
+        double us;
+        if (p->n_seq == 1) {
+            us = (double)(((long long)t.tile.groups * Hkv * s + sms - 1) / sms) * (each * tile_us + 4.0);
+        } else {
+            const double ctas = (double)p->n_tokens / pair * Hkv;
+            us = ctas * tiles * 0.5 / sms * tile_us + 0.5 * each * tile_us + 4.0;
+        }
+        if (s > 1) us += s * merge_us + 3.0;
+        if (us < best) {
+            best = us;
+            t.tile.n_splits = s;
+        }
+    }
+    if (t.tile.n_splits > 1) {
+        const size_t rows = (size_t)p->n_tokens * Hq * t.tile.n_splits;
+        t.o_bytes = align_up(rows * D * 4, 256);
+        t.bytes = t.o_bytes + align_up(rows * 8, 256);
+    }
+    return t;
+}
+
+// Map of a pool: (dim, row, head, page), boxes of 64 dims x min(page, 128) rows.
+int encode_pool_map(CUtensorMap *m, const vtx_tensor &t) {
+    PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+    if (!enc) return VTX_ERR_CUDA;
+    const size_t s2 = t.ne[2] > 1 ? t.nb[2] : t.nb[1] * (size_t)t.ne[1];
+    const size_t s3 = t.ne[3] > 1 ? t.nb[3] : s2 * (size_t)t.ne[2];
+    cuuint64_t dims[4] = {(cuuint64_t)t.ne[0], (cuuint64_t)t.ne[1], (cuuint64_t)t.ne[2], (cuuint64_t)t.ne[3]};
+    cuuint64_t strides[3] = {(cuuint64_t)t.nb[1], (cuuint64_t)s2, (cuuint64_t)s3};
+    cuuint32_t box[4] = {64, (cuuint32_t)std::min<int64_t>(t.ne[1], 128), 1, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, t.data, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? VTX_OK : VTX_ERR_STRIDE;
+}
+
+// Map of an F16 q: (dim, head, token), boxes of 64 dims x G heads x T tokens.
+int encode_paged_q_map(CUtensorMap *m, const vtx_tensor *q, int G, int T) {
+    PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+    if (!enc) return VTX_ERR_CUDA;
+    const size_t s1 = q->ne[2] > 1 ? q->nb[2] : (size_t)q->ne[0] * 2;
+    const size_t s2 = q->ne[1] > 1 ? q->nb[1] : s1 * (size_t)q->ne[2];
+    cuuint64_t dims[4] = {(cuuint64_t)q->ne[0], (cuuint64_t)q->ne[2], (cuuint64_t)q->ne[1], 1};
+    cuuint64_t strides[3] = {(cuuint64_t)s1, (cuuint64_t)s2, (cuuint64_t)(s2 * (size_t)q->ne[1])};
+    cuuint32_t box[4] = {64, (cuuint32_t)G, (cuuint32_t)T, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, q->data, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? VTX_OK : VTX_ERR_STRIDE;
+}
+
+template <int D, bool UF>
+int launch_tile(const CUtensorMap (&m)[3], const PagedAttnArgs &a, const PagedTile &tl, cudaStream_t st) {
+    using C = PagedTileCfg<D>;
+    static std::atomic<int> done[kMaxDevices];
+    int rc = allow_smem(fa_paged_sm100_kernel<D, UF>, C::SMEM, done);
+    if (rc != VTX_OK) return rc;
+    const long long ctas = (long long)tl.groups * a.kv.Hkv * tl.n_splits;
+    if (ctas > 0x7fffffffLL) return VTX_ERR_UNSUPPORTED;
+    if (ctas == 0) return VTX_OK;
+    rc = launch_pdl(fa_paged_sm100_kernel<D, UF>, dim3((unsigned)ctas), dim3(C::NTHREADS), C::SMEM, st, m[0], m[1],
+                    m[2], a, tl);
+    if (rc != VTX_OK || tl.n_splits == 1) return rc;
+    return launch_pdl(fa_paged_tile_combine_kernel<D>, dim3((unsigned)a.kv.n_tokens), dim3(256), 0, st, a, tl);
+}
+
 template <int D, int KVT>
 int launch_score(const PagedScoreArgs &a, cudaStream_t st) {
     return launch_pdl(kv_score_kernel<D, KVT>,
@@ -252,7 +351,9 @@ size_t vtx_flash_attn_paged_workspace(const vtx_paged_kv *kv, int32_t n_head_q) 
     if (check_paged(kv) != VTX_OK || n_head_q < 1 || n_head_q % kv->k.ne[2] ||
         n_head_q / kv->k.ne[2] > kMaxGroup)
         return (size_t)-1;
-    return plan_decode(kv, n_head_q / (int)kv->k.ne[2], current_sms()).bytes;
+    const int G = n_head_q / (int)kv->k.ne[2], sms = current_sms();
+    const DecodePlan d = plan_decode(kv, G, sms);
+    return d.bytes + plan_tile(kv, G, n_head_q, d.use ? d.rows : 0, sms).bytes;
 }
 
 int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, size_t workspace_bytes, void *stream) {
@@ -275,7 +376,9 @@ int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, si
     rc = ensure_device(&ds);
     if (rc != VTX_OK) return rc;
     DecodePlan dp = plan_decode(kv, Hq / (int)kv->k.ne[2], ds->sms);
-    if (workspace_bytes < dp.bytes || (dp.bytes && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256)))
+    TilePlan tp = plan_tile(kv, Hq / (int)kv->k.ne[2], Hq, dp.use ? dp.rows : 0, ds->sms);
+    const size_t need = dp.bytes + tp.bytes;
+    if (workspace_bytes < need || (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256)))
         return VTX_ERR_WORKSPACE;
     PagedAttnArgs a{};
     a.kv = view_of(kv, ds);
@@ -297,8 +400,22 @@ int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, si
         if (rc != VTX_OK || kv->max_new * (long long)a.G <= kFewRows) return rc;
         a.min_rows = dp.rows;
     }
-    if (d64) return f16 ? launch_attn<64, 1>(a, st) : launch_attn<64, 8>(a, st);
-    return f16 ? launch_attn<128, 1>(a, st) : launch_attn<128, 8>(a, st);
+    if (tp.use) {
+        char *ws = static_cast<char *>(workspace) + dp.bytes;
+        tp.tile.part_o = reinterpret_cast<float *>(ws);
+        tp.tile.part_ml = reinterpret_cast<float *>(ws + tp.o_bytes);
+        CUtensorMap m[3];
+        rc = encode_pool_map(&m[0], kv->k);
+        if (rc == VTX_OK) rc = encode_pool_map(&m[1], kv->v);
+        m[2] = m[0];                                          // an F32 q is read by the softmax warps
+        if (rc == VTX_OK && a.q_f16) rc = encode_paged_q_map(&m[2], q, a.G, tp.tile.T);
+        if (rc != VTX_OK) return rc;
+        // tanh, or a scale that the row maximum cannot carry: logits formed first
+        const bool uf = a.softcap != 0.0f || !(a.scale > 0.0f);
+        if (d64) return uf ? launch_tile<64, true>(m, a, tp.tile, st) : launch_tile<64, false>(m, a, tp.tile, st);
+        return uf ? launch_tile<128, true>(m, a, tp.tile, st) : launch_tile<128, false>(m, a, tp.tile, st);
+    }
+    return d64 ? launch_attn<64, 8>(a, st) : launch_attn<128, 8>(a, st);
 }
 
 int vtx_kv_score_paged(const vtx_kv_score_paged_args *p, void *stream) {
