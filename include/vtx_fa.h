@@ -463,8 +463,10 @@ VTX_API int vtx_kv_append_paged(const vtx_kv_append_paged_args *args, void *stre
  * Rows at or behind kv_len may hold anything, NaN included.  P and V (and a
  * F32 q) are rounded to half, everything else is F32.
  * workspace: 256-byte aligned, vtx_flash_attn_paged_workspace bytes (they
- * depend on kv's sizes and bounds and on n_head_q alone); calls that share
- * one must not overlap on the GPU. */
+ * depend on kv's sizes and bounds and on n_head_q alone).  Zero it once before
+ * its first call (cudaMemset): it holds arrival counters, which every call
+ * leaves at zero; a call with other sizes or bounds needs it zeroed again.
+ * Calls that share one must not overlap on the GPU. */
 typedef struct vtx_flash_attn_paged_args {
     const vtx_paged_kv *kv;
     const vtx_tensor *q;

@@ -37,6 +37,12 @@ __device__ __forceinline__ float paged_logit(float s, float scale, float softcap
     return softcap != 0.0f ? softcap * kLog2e * tanhf(s * (scale / softcap)) : s * (scale * kLog2e);
 }
 
+// The same with the choice made by the instantiation (UF: softcap).
+template <bool UF>
+__device__ __forceinline__ float paged_logit_t(float s, float cx, float scale, float softcap) {
+    return UF ? softcap * kLog2e * tanhf(s * (scale / softcap)) : s * cx;
+}
+
 // Two adjacent columns (d even) of a query row, rounded to half.
 __device__ __forceinline__ uint32_t paged_q2(const char *row, int f16, int d) {
     if (f16) return *reinterpret_cast<const uint32_t *>(row + d * 2);

@@ -19,7 +19,9 @@
 //         conflicts (keys 2n + tile, words c and c + 4 of a block).
 // Softmax in log2 units with a lazily moved reference m: O is rescaled only
 // when the running maximum passes it by 2^8 (2^6).  The warps' (m, l, O) are
-// merged in shared memory, the splits by fa_paged_combine_kernel.
+// merged in shared memory; with several splits every CTA leaves its result in the
+// workspace, and the one that arrives last at the (stream, KV head)'s counter
+// merges them in split order.
 #pragma once
 #include <cuda_fp16.h>
 #include <cstdint>
@@ -33,19 +35,20 @@ struct PagedSplit {
     int n_splits;             // splits of a stream's keys at most
     int tiles;                // 16-key tiles per split at least
     float *part_o, *part_ml;  // [n_seq][Hkv][n_splits][ROWS][D], ... [2] (m, l)
+    unsigned *arrived;        // [n_seq][Hkv], zero between calls
 };
 
 template <int D, int KVT> struct PagedDecodeCfg {
     static constexpr int KEYS = 16, WARPS = 4;
     static constexpr int ROW = KVT == 1 ? D * 2 : D / 32 * 34;
     static constexpr int PITCH = KVT == 1 ? ROW + 16 : ROW;
-    static constexpr int STAGES = KVT == 1 ? 3 : 5;
+    static constexpr int STAGES = KVT == 1 ? 2 : 4;
     static constexpr int STAGE_BYTES = 2 * KEYS * PITCH;
     // the ring, reused for the warp's 16 x D floats at the end
     static constexpr int WARP_BYTES = STAGES * STAGE_BYTES > 16 * D * 4 ? STAGES * STAGE_BYTES : 16 * D * 4;
     static constexpr int BAR_OFF = WARPS * WARP_BYTES;
     static constexpr int ML_OFF = BAR_OFF + WARPS * STAGES * 8;
-    static constexpr int SMEM = ML_OFF + WARPS * 16 * 8;
+    static constexpr int SMEM = ML_OFF + WARPS * 16 * 8 + 16;
 };
 
 // How a stream's keys are cut: `lo` its first needed tile's row, nt tiles of 16
@@ -192,8 +195,20 @@ __device__ __forceinline__ int paged_o_dim(int nb, int j, int c) {
     return KVT == 1 ? nb * 8 + 2 * c + j : (nb >> 2) * 32 + 8 * c + 4 * j + (nb & 3);
 }
 
-template <int D, int KVT, int ROWS>
-__global__ void __launch_bounds__(128, 2)
+// Normalises and writes 4 columns of query row r, and its lse with column 0.
+template <int D>
+__device__ __forceinline__ void paged_finish(const PagedAttnArgs &a, const PagedSeq &s, int g, int r, int d, float4 acc,
+                                             float m, float l)
+{
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int tok = s.q0 + r / a.G, head = g * a.G + r % a.G;
+    paged_store2(a, tok, head, d, acc.x * inv, acc.y * inv);
+    paged_store2(a, tok, head, d + 2, acc.z * inv, acc.w * inv);
+    if (a.lse && d == 0) a.lse[(long long)tok * a.Hq + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+template <int D, int KVT, int ROWS, bool UF>
+__global__ void __launch_bounds__(128, 3)
 fa_paged_decode_kernel(const PagedAttnArgs a, const PagedSplit sp)
 {
     grid_dep_wait();
@@ -283,6 +298,7 @@ fa_paged_decode_kernel(const PagedAttnArgs a, const PagedSplit sp)
 #pragma unroll
     for (int i = 0; i < NB; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    const float cx = a.scale * kLog2e;
     constexpr float kJump = KVT == 1 ? 8.0f : 6.0f, kBack = KVT == 1 ? 0.0f : 4.0f;
     bool ok = true;
     int done = 0;
@@ -302,9 +318,11 @@ fa_paged_decode_kernel(const PagedAttnArgs a, const PagedSplit sp)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     float &y = x[nt2][2 * u + j];
-                    y = paged_logit(y, a.scale, a.softcap);
-                    const int key = k0 + (KVT == 1 ? 8 * nt2 + 2 * c + j : 4 * c + 2 * j + nt2);
-                    if (!inner && (key < lo[u] || key > hi[u])) y = -INFINITY;
+                    y = paged_logit_t<UF>(y, cx, a.scale, a.softcap);
+                    if (!inner) {
+                        const int key = k0 + (KVT == 1 ? 8 * nt2 + 2 * c + j : 4 * c + 2 * j + nt2);
+                        y = key < lo[u] || key > hi[u] ? -INFINITY : y;
+                    }
                     mx = fmaxf(mx, y);
                 }
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -373,38 +391,33 @@ fa_paged_decode_kernel(const PagedAttnArgs a, const PagedSplit sp)
             *reinterpret_cast<float4 *>(sp.part_o + (work * ROWS + r) * D + d) = acc;
             if (d == 0) reinterpret_cast<float2 *>(sp.part_ml)[work * ROWS + r] = make_float2(top, tot);
         } else {
-            const float inv = tot == 0.f ? 0.f : 1.f / tot;
-            const int tok = s.q0 + r / a.G, head = g * a.G + r % a.G;
-            paged_store2(a, tok, head, d, acc.x * inv, acc.y * inv);
-            paged_store2(a, tok, head, d + 2, acc.z * inv, acc.w * inv);
-            if (a.lse && d == 0)
-                a.lse[(long long)tok * a.Hq + head] = tot == 0.f ? -INFINITY : (top + log2f(tot)) * kLn2;
+            paged_finish<D>(a, s, g, r, d, acc, top, tot);
         }
     }
-}
+    if (cut.n == 1) return;
 
-// Merges the splits' partials: grid (Hkv, n_seq), a warp per query row, a lane
-// per 4 dims (D = 64: two splits at a time), eight splits' loads in flight.
-template <int D, int ROWS>
-__global__ void __launch_bounds__(128)
-fa_paged_combine_kernel(const PagedAttnArgs a, const PagedSplit sp)
-{
-    grid_dep_wait();
-    grid_dep_launch();
+    // ---- merge the splits ---------------------------------------------------------
+    int *last = reinterpret_cast<int *>(smem + C::ML_OFF + C::WARPS * 16 * 8);
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        unsigned old;                                           // wraps to zero at the last arrival
+        asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;" : "=r"(old)
+                     : "l"(sp.arrived + (long long)b * a.kv.Hkv + g), "r"((unsigned)cut.n - 1) : "memory");
+        *last = old == (unsigned)cut.n - 1;
+    }
+    __syncthreads();
+    if (!*last) return;
+    __threadfence();
+    // a warp per query row, a lane per 4 dims (D = 64: two splits at a time),
+    // eight splits' loads in flight
     constexpr int LPR = D / 4, SPW = 32 / LPR, U = 8 / SPW;
-    const int g = blockIdx.x, b = blockIdx.y;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const PagedSeq s = paged_seq(a.kv, b);
-    const int rows = s.n_new * a.G;
-    if (rows == 0 || rows > ROWS) return;
-    const int n = paged_cut(s, a.causal, a.window, sp).n;
-    if (n == 1) return;
-    const long long w0 = ((long long)b * a.kv.Hkv + g) * sp.n_splits;
+    const long long w0 = work - split;
     const int d = (lane % LPR) * 4;
-    for (int r = warp; r < rows; r += 4) {
-        float m = -INFINITY, l = 0.f;
+    for (int r = warp; r < rows; r += C::WARPS) {
+        float top = -INFINITY, tot = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i0 = lane / LPR; i0 < n; i0 += SPW * U) {
+        for (int i0 = lane / LPR; i0 < cut.n; i0 += SPW * U) {
             float2 y[U];
             float4 v[U];
 #pragma unroll
@@ -412,46 +425,39 @@ fa_paged_combine_kernel(const PagedAttnArgs a, const PagedSplit sp)
                 const int i = i0 + u * SPW;
                 y[u] = make_float2(-INFINITY, 0.f);
                 v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (i < n) {
-                    y[u] = reinterpret_cast<const float2 *>(sp.part_ml)[(w0 + i) * ROWS + r];
-                    v[u] = *reinterpret_cast<const float4 *>(sp.part_o + ((w0 + i) * ROWS + r) * D + d);
+                if (i < cut.n) {
+                    y[u] = __ldcg(reinterpret_cast<const float2 *>(sp.part_ml) + (w0 + i) * ROWS + r);
+                    v[u] = __ldcg(reinterpret_cast<const float4 *>(sp.part_o + ((w0 + i) * ROWS + r) * D + d));
                 }
             }
-            float top = m;
+            float mx = top;
 #pragma unroll
-            for (int u = 0; u < U; ++u) top = fmaxf(top, y[u].x);
-            if (top == -INFINITY) continue;
-            const float f0 = ex2(m - top);
+            for (int u = 0; u < U; ++u) mx = fmaxf(mx, y[u].x);
+            if (mx == -INFINITY) continue;
+            const float f0 = ex2(top - mx);
             acc.x *= f0; acc.y *= f0; acc.z *= f0; acc.w *= f0;
-            l *= f0;
-            m = top;
+            tot *= f0;
+            top = mx;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float f = ex2(y[u].x - top);
-                l = fmaf(f, y[u].y, l);
+                const float f = ex2(y[u].x - mx);
+                tot = fmaf(f, y[u].y, tot);
                 acc.x = fmaf(f, v[u].x, acc.x); acc.y = fmaf(f, v[u].y, acc.y);
                 acc.z = fmaf(f, v[u].z, acc.z); acc.w = fmaf(f, v[u].w, acc.w);
             }
         }
         if (SPW == 2) {
-            const float m2 = __shfl_xor_sync(0xffffffffu, m, 16), l2 = __shfl_xor_sync(0xffffffffu, l, 16);
+            const float m2 = __shfl_xor_sync(0xffffffffu, top, 16), l2 = __shfl_xor_sync(0xffffffffu, tot, 16);
             const float4 o2 = make_float4(__shfl_xor_sync(0xffffffffu, acc.x, 16), __shfl_xor_sync(0xffffffffu, acc.y, 16),
                                           __shfl_xor_sync(0xffffffffu, acc.z, 16), __shfl_xor_sync(0xffffffffu, acc.w, 16));
-            const float top = fmaxf(m, m2);
-            const float f = m == -INFINITY ? 0.f : ex2(m - top), f2 = m2 == -INFINITY ? 0.f : ex2(m2 - top);
-            m = top;
-            l = l * f + l2 * f2;
+            const float mx = fmaxf(top, m2);
+            const float f = top == -INFINITY ? 0.f : ex2(top - mx), f2 = m2 == -INFINITY ? 0.f : ex2(m2 - mx);
+            top = mx;
+            tot = tot * f + l2 * f2;
             acc.x = acc.x * f + o2.x * f2; acc.y = acc.y * f + o2.y * f2;
             acc.z = acc.z * f + o2.z * f2; acc.w = acc.w * f + o2.w * f2;
         }
-        if (lane < LPR) {
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            const int tok = s.q0 + r / a.G, head = g * a.G + r % a.G;
-            paged_store2(a, tok, head, d, acc.x * inv, acc.y * inv);
-            paged_store2(a, tok, head, d + 2, acc.z * inv, acc.w * inv);
-            if (a.lse && lane == 0)
-                a.lse[(long long)tok * a.Hq + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
-        }
+        if (lane < LPR) paged_finish<D>(a, s, g, r, d, acc, top, tot);
     }
 }
 

@@ -8,14 +8,17 @@
 // for the whole call and walks the query rows 16 at a time, adding each tile's
 // weights to one register per key; a shuffle over the row lanes at the end
 // gives the sums in the same order on every run (no atomics).
-// Few rows (a decode step): bound by reading K once.  Many rows: bound by the
-// exponentials (one per query row and key) and mma.sync.
+// Three kernels.  Few query rows per KV head (a decode step): bound by reading K
+// once, kv_score_stream_kernel.  Many rows, F16: bound by the exponentials (one
+// per query row and key), kv_score_sm100_kernel.  Many rows over a Q8_0 cache
+// or with an F32 q: kv_score_kernel, the description above.
 #pragma once
 #include <cuda_fp16.h>
 #include <cstdint>
 #include "vtx_ptx.cuh"
 #include "paged_kv.cuh"
 #include "fa_paged.cuh"
+#include "fa_paged_decode.cuh"
 
 namespace vtx {
 
@@ -47,6 +50,10 @@ kv_score_kernel(const PagedScoreArgs a)
     const int k0 = blockIdx.x * 128 + warp * 32;
     if (k0 >= limit) return;
 
+    const int off = s.len - s.n_new;
+    int t0 = a.observe > 0 ? max(0, s.n_new - a.observe) : 0;
+    const int lo_any = t0 < s.n_new ? (a.window > 0 ? off + t0 - a.window + 1 : 0) : limit;   // nobody sees keys below
+
     // K rows of the warp's keys as B fragments.  The k index of the MMA is any
     // permutation of the head dim that Q shares: lane c of a quad takes dims
     // 32 i + 8 c ... + 7, one 16-byte load per row and 32 dims.  Q8_0: the
@@ -56,7 +63,7 @@ kv_score_kernel(const PagedScoreArgs a)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int key = k0 + nt * 8 + (lane >> 2);
-        const bool on = key < limit;
+        const bool on = key < limit && key >= lo_any;
         const char *kr = a.kv.k + (on ? paged_row(a.kv, b, key, g) : 0);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
@@ -74,8 +81,6 @@ kv_score_kernel(const PagedScoreArgs a)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) sum[nt][0] = sum[nt][1] = 0.f;
 
-    const int off = s.len - s.n_new;
-    int t0 = a.observe > 0 ? max(0, s.n_new - a.observe) : 0;
     if (a.causal) t0 = max(t0, k0 - off);                   // earlier tokens see none of these keys
     int t1 = s.n_new;
     if (a.window > 0) t1 = min(t1, k0 + 31 + a.window - off);   // nor do tokens past the window
@@ -144,6 +149,164 @@ kv_score_kernel(const PagedScoreArgs a)
                 a.score_out[e] = (a.decay != 0.f ? a.decay * a.score[e] : 0.f) + x;
             }
         }
+}
+
+// Streams with at most 16 query rows per KV head: the K half of the streaming
+// attention kernel.  A CTA per (stream, KV head, key split), its 4 warps take
+// tiles of 16 keys in turn through private rings of bulk copies; a tile's
+// weights are summed over the row lanes by shuffles and added to the old score,
+// which was loaded before the wait for the tile.
+template <int D, int KVT> struct ScoreStreamCfg {
+    using P = PagedDecodeCfg<D, KVT>;
+    static constexpr int STAGES = KVT == 1 ? 3 : 5;
+    static constexpr int STAGE_BYTES = 16 * P::PITCH;
+    static constexpr int WARP_BYTES = STAGES * STAGE_BYTES;
+    static constexpr int BAR_OFF = 4 * WARP_BYTES;
+    static constexpr int SMEM = BAR_OFF + 4 * STAGES * 8;
+};
+
+template <int D, int KVT, bool UF>
+__global__ void __launch_bounds__(128)
+kv_score_stream_kernel(const PagedScoreArgs a, const PagedSplit sp)
+{
+    grid_dep_wait();
+    grid_dep_launch();
+    using P = PagedDecodeCfg<D, KVT>;
+    using C = ScoreStreamCfg<D, KVT>;
+    constexpr int KC = D / 16;
+    extern __shared__ __align__(128) char smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3;
+    char *ring = smem + warp * C::WARP_BYTES;
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::BAR_OFF) + warp * C::STAGES;
+    const int g = blockIdx.x % a.kv.Hkv;
+    const int split = (blockIdx.x / a.kv.Hkv) % sp.n_splits;
+    const int b = blockIdx.x / (a.kv.Hkv * sp.n_splits);
+    PagedSeq s = paged_seq(a.kv, b);
+    if (threadIdx.x == 0 && split == 0 && (s.len > min(a.row_cap, a.kv.max_kv) || s.n_new > a.kv.max_new))
+        paged_report(a.kv, VTX_KERR_BOUND);
+    const int limit = min(s.len, a.row_cap);
+    const int off = s.len - s.n_new;
+    const int t0 = max(s.n_new - a.kv.max_new, a.observe > 0 ? max(0, s.n_new - a.observe) : 0);
+    const int rows = (s.n_new - t0) * a.G;
+    const int lo_any = rows == 0 ? limit : (a.window > 0 ? max(0, off + t0 - a.window + 1) : 0);
+    const PagedCut cut = paged_cut(PagedSeq{s.q0, s.n_new, limit}, 0, 0, sp);
+    if (split >= cut.n) return;
+    const int t_end = min(cut.per * (split + 1), cut.nt);
+    const int first = cut.per * split + warp;
+    const int nt = t_end > first ? (t_end - first + 3) / 4 : 0;
+
+    if (lane < C::STAGES) mbar_init(&full[lane], 1);
+    __syncwarp();
+    fence_mbar_init();
+    __syncwarp();
+    const char *kp = a.kv.k + (long long)g * a.kv.nb2;
+    int pages = 0;
+    auto issue = [&](int t) {
+        if ((t & 31) == 0) {
+            const int k = 16 * (first + (t + lane) * 4);
+            pages = t + lane < nt && k + 16 > lo_any ? max(paged_page(a.kv, b, k), 0) : 0;
+        }
+        const int pg = __shfl_sync(0xffffffffu, pages, t & 31);
+        const int k0 = 16 * (first + t * 4);
+        if (t >= nt || k0 + 16 <= lo_any) return;               // nobody sees this tile: not read
+        char *st = ring + (t % C::STAGES) * C::STAGE_BYTES;
+        uint64_t *bar = &full[t % C::STAGES];
+        const long long at = (long long)pg * a.kv.nb3 + (long long)(k0 & ((1 << a.kv.shift) - 1)) * a.kv.nb1;
+        fence_proxy_async_smem();
+        if (lane == 0) mbar_arrive_expect_tx(bar, 16 * P::ROW);
+        __syncwarp();
+        if constexpr (KVT == 1) {                               // rows behind kv_len are masked, whatever they hold
+            if (lane < 16) bulk_g2s(st + lane * P::PITCH, kp + at + (long long)lane * a.kv.nb1, P::ROW, bar);
+        } else {
+            if (lane == 0) bulk_g2s(st, kp + at, 16 * P::ROW, bar);
+        }
+    };
+#pragma unroll
+    for (int t = 0; t < C::STAGES; ++t) issue(t);
+
+    uint32_t qa[KC][4];
+    int lo[2], hi[2];
+    float ls[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int r = (lane >> 2) + 8 * u;
+        const bool on = r < rows;
+        const int tok = t0 + (on ? r / a.G : 0), head = g * a.G + (on ? r % a.G : 0);
+        hi[u] = on ? (a.causal ? min(off + tok, limit - 1) : limit - 1) : -1;
+        lo[u] = a.window > 0 ? off + tok - a.window + 1 : 0;
+        const char *qp = a.q + (long long)(s.q0 + tok) * a.q_nbt + (long long)head * a.q_nbh;
+        const float x = on ? a.lse[(long long)(s.q0 + tok) * a.Hq + head] : INFINITY;
+        ls[u] = x == -INFINITY ? INFINITY : x * kLog2e;
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) {
+            const int d = KVT == 1 ? kc * 16 + 2 * c : (kc >> 1) * 32 + (kc & 1) * 16 + 4 * c;
+            qa[kc][u] = on ? paged_q2(qp, a.q_f16, d) : 0u;
+            qa[kc][2 + u] = on ? paged_q2(qp, a.q_f16, d + (KVT == 1 ? 8 : 2)) : 0u;
+        }
+    }
+    // the value (key tile i, column j) that lanes 4v ... 4v + 3 write, v = 2i + j
+    const int v = lane >> 2, mine = KVT == 1 ? 8 * (v >> 1) + 2 * c + (v & 1) : 4 * c + 2 * (v & 1) + (v >> 1);
+    const long long base = ((long long)b * a.kv.Hkv + g) * a.row_cap;
+    // tiles nobody sees come first and use no stage
+    const int skip = min(nt, (lo_any >> 4) > first ? ((lo_any >> 4) - 1 - first) / 4 + 1 : 0);
+    const float cx = a.scale * kLog2e;
+    const int hi_all = a.causal ? off + t0 : limit - 1;        // every token sees [lo_all, hi_all]
+    const int lo_all = a.window > 0 ? off + s.n_new - a.window : 0;
+    // old scores of the next four tiles: their latency is a tile's whole time
+    auto old_of = [&](int t) {
+        const int key = 16 * (first + t * 4) + mine;
+        return t < nt && v < 4 && key < limit && a.decay != 0.f ? a.decay * a.score[base + key] : 0.f;
+    };
+    constexpr int U = 4;
+    float old[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) old[i] = old_of(i);
+    bool ok = true;
+    int done = 0;
+    for (int tb = 0; tb < nt && ok; tb += U) {
+#pragma unroll
+        for (int ui = 0; ui < U; ++ui) {
+            const int t = tb + ui;
+            if (t >= nt || !ok) break;
+            const int k0 = 16 * (first + t * 4), key = k0 + mine;
+            const bool inner = k0 >= lo_all && k0 + 15 <= hi_all;
+            float sum = 0.f;
+            if (t >= skip) {
+                ok = __all_sync(0xffffffffu,
+                                mbar_wait(&full[t % C::STAGES], ((t - skip) / C::STAGES) & 1, a.kv.err, VTX_KERR_KV));
+                if (!ok) break;
+                float x[2][4], w[4];
+                paged_tile_scores<D, KVT>(ring + (t % C::STAGES) * C::STAGE_BYTES, qa, x, lane);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int k = k0 + (KVT == 1 ? 8 * i + 2 * c + j : 4 * c + 2 * j + i);
+                        float y = 0.f;
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            if (u == 1 && rows <= 8) break;     // uniform
+                            const float p = ex2(paged_logit_t<UF>(x[i][2 * u + j], cx, a.scale, a.softcap) - ls[u]);
+                            y += inner || (k >= lo[u] && k <= hi[u]) ? p : 0.f;
+                        }
+                        w[2 * i + j] = y;
+                    }
+                // sum over the 8 row lanes, halving the values kept: lane v ends with value v & 3
+                const bool h1 = v & 2, h0 = v & 1;
+                const float a0 = (h1 ? w[2] : w[0]) + __shfl_xor_sync(0xffffffffu, h1 ? w[0] : w[2], 8);
+                const float a1 = (h1 ? w[3] : w[1]) + __shfl_xor_sync(0xffffffffu, h1 ? w[1] : w[3], 8);
+                sum = (h0 ? a1 : a0) + __shfl_xor_sync(0xffffffffu, h0 ? a0 : a1, 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                __syncwarp();
+            }
+            if (v < 4 && key < limit) a.score_out[base + key] = old[ui] + sum;
+            old[ui] = old_of(t + U);
+            issue(t + C::STAGES);
+            done = t + 1;
+        }
+    }
+    for (int t = max(done, skip); t < min(nt, done + C::STAGES); ++t)   // after a failed wait: copies must land
+        mbar_wait(&full[t % C::STAGES], ((t - skip) / C::STAGES) & 1, nullptr, 0);
 }
 
 }  // namespace vtx

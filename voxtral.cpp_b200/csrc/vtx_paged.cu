@@ -19,6 +19,7 @@
 #include "fa_paged_decode.cuh"
 #include "fa_paged_sm100.cuh"
 #include "kv_score.cuh"
+#include "kv_score_sm100.cuh"
 #include "kv_evict.cuh"
 
 using namespace vtx;
@@ -122,7 +123,7 @@ struct DecodePlan {
     bool use;                 // the streaming kernel is launched
     int rows;                 // its row count, 8 or 16
     PagedSplit split;
-    size_t o_bytes, bytes;
+    size_t c_bytes, o_bytes, bytes;   // counters, partial O, all
 };
 
 // Splits: about two waves of two CTAs per SM over (streams x KV heads), at
@@ -145,29 +146,31 @@ DecodePlan plan_decode(const vtx_paged_kv *p, int G, int sms) {
     d.split.tiles = (int)((tiles + want - 1) / want);
     if (want > 1) {
         const size_t rows = (size_t)base * want * d.rows;
+        d.c_bytes = align_up((size_t)base * 4, 256);
         d.o_bytes = align_up(rows * p->k.ne[0] * 4, 256);
-        d.bytes = d.o_bytes + align_up(rows * 8, 256);
+        d.bytes = d.c_bytes + d.o_bytes + align_up(rows * 8, 256);
     }
     return d;
 }
 
-template <int D, int KVT, int ROWS>
+template <int D, int KVT, int ROWS, bool UF>
 int launch_decode(const PagedAttnArgs &a, const PagedSplit &sp, cudaStream_t st) {
     using C = PagedDecodeCfg<D, KVT>;
     static std::atomic<int> done[kMaxDevices];
-    int rc = allow_smem(fa_paged_decode_kernel<D, KVT, ROWS>, C::SMEM, done);
+    int rc = allow_smem(fa_paged_decode_kernel<D, KVT, ROWS, UF>, C::SMEM, done);
     if (rc != VTX_OK) return rc;
     const long long ctas = (long long)a.kv.n_seq * a.kv.Hkv * sp.n_splits;
     if (ctas > 0x7fffffffLL) return VTX_ERR_UNSUPPORTED;
-    rc = launch_pdl(fa_paged_decode_kernel<D, KVT, ROWS>, dim3((unsigned)ctas), dim3(128), C::SMEM, st, a, sp);
-    if (rc != VTX_OK || sp.n_splits == 1) return rc;
-    return launch_pdl(fa_paged_combine_kernel<D, ROWS>, dim3((unsigned)a.kv.Hkv, (unsigned)a.kv.n_seq), dim3(128), 0,
-                      st, a, sp);
+    return launch_pdl(fa_paged_decode_kernel<D, KVT, ROWS, UF>, dim3((unsigned)ctas), dim3(128), C::SMEM, st, a, sp);
 }
 
 template <int D, int KVT>
 int launch_decode_rows(const PagedAttnArgs &a, const DecodePlan &d, cudaStream_t st) {
-    return d.rows == 8 ? launch_decode<D, KVT, 8>(a, d.split, st) : launch_decode<D, KVT, 16>(a, d.split, st);
+    if (a.softcap != 0.0f)
+        return d.rows == 8 ? launch_decode<D, KVT, 8, true>(a, d.split, st)
+                           : launch_decode<D, KVT, 16, true>(a, d.split, st);
+    return d.rows == 8 ? launch_decode<D, KVT, 8, false>(a, d.split, st)
+                       : launch_decode<D, KVT, 16, false>(a, d.split, st);
 }
 
 template <int D, int KVT>
@@ -279,6 +282,52 @@ int launch_score(const PagedScoreArgs &a, cudaStream_t st) {
     return launch_pdl(kv_score_kernel<D, KVT>,
                       dim3((unsigned)((a.kv.max_kv + 127) / 128), (unsigned)a.kv.Hkv, (unsigned)a.kv.n_seq), dim3(128),
                       0, st, a);
+}
+
+// Few query rows: the splits of the streaming attention kernel (whose K half
+// this is), without partials.
+template <int D, int KVT, bool UF>
+int launch_score_stream_t(const PagedScoreArgs &a, const PagedSplit &sp, cudaStream_t st) {
+    using C = ScoreStreamCfg<D, KVT>;
+    static std::atomic<int> done[kMaxDevices];
+    int rc = allow_smem(kv_score_stream_kernel<D, KVT, UF>, C::SMEM, done);
+    if (rc != VTX_OK) return rc;
+    const long long ctas = (long long)a.kv.n_seq * a.kv.Hkv * sp.n_splits;
+    if (ctas > 0x7fffffffLL) return VTX_ERR_UNSUPPORTED;
+    return launch_pdl(kv_score_stream_kernel<D, KVT, UF>, dim3((unsigned)ctas), dim3(128), C::SMEM, st, a, sp);
+}
+
+template <int D, int KVT>
+int launch_score_stream(const PagedScoreArgs &a, int sms, cudaStream_t st) {
+    const long long base = (long long)a.kv.n_seq * a.kv.Hkv;
+    const int tiles = std::max(1, (a.kv.max_kv + 15) / 16);
+    PagedSplit sp{};
+    const long long want = std::max<long long>((4LL * sms + base - 1) / base, (tiles + 63) / 64);
+    sp.n_splits = (int)std::min<long long>(want, (tiles + 3) / 4);
+    sp.tiles = (tiles + sp.n_splits - 1) / sp.n_splits;
+    return a.softcap != 0.0f ? launch_score_stream_t<D, KVT, true>(a, sp, st)
+                             : launch_score_stream_t<D, KVT, false>(a, sp, st);
+}
+
+template <int D, int NT, bool UF>
+int launch_score_tile_n(const CUtensorMap (&m)[2], const PagedScoreArgs &a, int T, cudaStream_t st) {
+    using C = ScoreTileCfg<D, NT>;
+    static std::atomic<int> done[kMaxDevices];
+    int rc = allow_smem(kv_score_sm100_kernel<D, NT, UF>, C::SMEM, done);
+    if (rc != VTX_OK) return rc;
+    return launch_pdl(kv_score_sm100_kernel<D, NT, UF>,
+                      dim3((unsigned)((a.kv.max_kv + 128 * NT - 1) / (128 * NT)), (unsigned)a.kv.Hkv,
+                           (unsigned)a.kv.n_seq),
+                      dim3(C::NTHREADS), C::SMEM, st, m[0], m[1], a, T);
+}
+
+// Four key tiles per CTA halve the reads of Q from L2, two spread over more
+// SMs: four once they fill the GPU (500 tokens: 16000 keys 102 us with four, 116
+// with two; 4000 keys 51 and 31 us).
+template <int D, bool UF>
+int launch_score_tile(const CUtensorMap (&m)[2], const PagedScoreArgs &a, int T, int sms, cudaStream_t st) {
+    const long long ctas4 = ((long long)a.kv.max_kv + 511) / 512 * a.kv.Hkv * a.kv.n_seq;
+    return ctas4 >= sms ? launch_score_tile_n<D, 4, UF>(m, a, T, st) : launch_score_tile_n<D, 2, UF>(m, a, T, st);
 }
 
 struct EvictPlan {
@@ -393,8 +442,10 @@ int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, si
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool f16 = kv->k.type == VTX_TYPE_F16, d64 = kv->k.ne[0] == 64;
     if (dp.use) {
-        dp.split.part_o = static_cast<float *>(workspace);
-        dp.split.part_ml = reinterpret_cast<float *>(static_cast<char *>(workspace) + dp.o_bytes);
+        char *ws = static_cast<char *>(workspace);
+        dp.split.arrived = reinterpret_cast<unsigned *>(ws);
+        dp.split.part_o = reinterpret_cast<float *>(ws + dp.c_bytes);
+        dp.split.part_ml = reinterpret_cast<float *>(ws + dp.c_bytes + dp.o_bytes);
         rc = d64 ? (f16 ? launch_decode_rows<64, 1>(a, dp, st) : launch_decode_rows<64, 8>(a, dp, st))
                  : (f16 ? launch_decode_rows<128, 1>(a, dp, st) : launch_decode_rows<128, 8>(a, dp, st));
         if (rc != VTX_OK || kv->max_new * (long long)a.G <= kFewRows) return rc;
@@ -443,8 +494,23 @@ int vtx_kv_score_paged(const vtx_kv_score_paged_args *p, void *stream) {
     a.scale = p->params->scale; a.softcap = p->params->logit_softcap;
     a.causal = p->params->causal != 0; a.window = p->params->window;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool f16 = kv->k.type == VTX_TYPE_F16;
-    if (kv->k.ne[0] == 64) return f16 ? launch_score<64, 1>(a, st) : launch_score<64, 8>(a, st);
+    const bool f16 = kv->k.type == VTX_TYPE_F16, d64 = kv->k.ne[0] == 64;
+    const long long rows = (long long)(p->observe > 0 ? std::min(p->observe, kv->max_new) : kv->max_new) * a.G;
+    if (rows <= kFewRows) {
+        if (d64) return f16 ? launch_score_stream<64, 1>(a, ds->sms, st) : launch_score_stream<64, 8>(a, ds->sms, st);
+        return f16 ? launch_score_stream<128, 1>(a, ds->sms, st) : launch_score_stream<128, 8>(a, ds->sms, st);
+    }
+    if (f16 && a.q_f16) {
+        CUtensorMap m[2];
+        const int T = 128 / a.G;
+        rc = encode_pool_map(&m[0], kv->k);
+        if (rc == VTX_OK) rc = encode_paged_q_map(&m[1], p->q, a.G, T);
+        if (rc != VTX_OK) return rc;
+        if (a.softcap != 0.0f)
+            return d64 ? launch_score_tile<64, true>(m, a, T, ds->sms, st) : launch_score_tile<128, true>(m, a, T, ds->sms, st);
+        return d64 ? launch_score_tile<64, false>(m, a, T, ds->sms, st) : launch_score_tile<128, false>(m, a, T, ds->sms, st);
+    }
+    if (d64) return f16 ? launch_score<64, 1>(a, st) : launch_score<64, 8>(a, st);
     return f16 ? launch_score<128, 1>(a, st) : launch_score<128, 8>(a, st);
 }
 

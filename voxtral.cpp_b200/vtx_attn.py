@@ -435,6 +435,9 @@ class DecodeLayerPlan:
 
 # ---- paged decoder cache ------------------------------------------------------
 
+_ROW_TYPES = {torch.float32: (F32, 4), torch.float16: (F16, 2)}      # dtype -> (type id, bytes)
+
+
 class PagedKv:
     """A decoder cache in pages with one step's ragged batch of new tokens
     (vtx_paged_kv), and the calls over it: append, attend, score, evict.
@@ -477,15 +480,19 @@ class PagedKv:
                 self._lib.vtx_kv_evict_paged_workspace(ctypes.byref(c))]
         if ctypes.c_size_t(-1).value in need:
             raise VtxError(-3, "paged cache rejected")
-        # one buffer for every call: they follow one another
-        self.workspace = torch.empty(max(max(need), 256), dtype=torch.uint8, device=self.dev)
-        self._ws = (ctypes.c_void_p(self.workspace.data_ptr()), ctypes.c_size_t(self.workspace.numel()))
+        # attention's holds arrival counters: zero once, left zeroed by every call
+        self.workspace = torch.zeros(max(need[0], 256), dtype=torch.uint8, device=self.dev)
+        self.evict_workspace = torch.empty(max(need[1], 256), dtype=torch.uint8, device=self.dev)
+        self._ws, self._evict_ws = ((w.data_ptr(), w.numel()) for w in (self.workspace, self.evict_workspace))
         # argument blocks, made once: a call only sets its tensors
+        self._q_shape = (n_tokens, n_head_q, self.head_dim)
+        self._kv_shape = (n_tokens, self.n_head_kv, self.head_dim)
         self._q, self._dst, self._params = VtxTensor(), VtxTensor(), FaParams()
         for d in (self._q, self._dst):
             d.ne[0], d.ne[3] = self.head_dim, 1
         self._q.ne[1], self._q.ne[2] = n_tokens, n_head_q
         self._dst.ne[1], self._dst.ne[2] = n_head_q, n_tokens
+        self._q_nb, self._dst_nb = self._q.nb, self._dst.nb
         at, adr = ctypes.addressof, ctypes.addressof(c)
         self._append, self._attend = KvAppendPagedArgs(), FlashAttnPagedArgs()
         self._score, self._evict = KvScorePagedArgs(), KvEvictPagedArgs()
@@ -512,22 +519,25 @@ class PagedKv:
         d.data = t.data_ptr()
         return d
 
-    def _rows(self, t: torch.Tensor, heads: int, what: str, d: VtxTensor, token: int, head: int) -> None:
-        """Puts a (n_tokens, heads, D) float32 / float16 view into descriptor d."""
-        if tuple(t.shape) != (self.n_tokens, heads, self.head_dim) or t.stride(2) != 1 or t.device != self.dev:
-            raise VtxError(-3, f"{what} must be ({self.n_tokens}, {heads}, {self.head_dim}), last axis contiguous")
-        es = t.element_size()
-        d.type = _ggml_type(t, None)
-        d.nb[0], d.nb[token], d.nb[head], d.data = es, t.stride(0) * es, t.stride(1) * es, t.data_ptr()
+    def _rows(self, t: torch.Tensor, what: str, d: VtxTensor, nb, token: int, head: int) -> None:
+        """Puts a (n_tokens, n_head_q, D) float32 / float16 view into descriptor d."""
+        st, kind = t.stride(), _ROW_TYPES.get(t.dtype)
+        if t.shape != self._q_shape or st[2] != 1 or t.device != self.dev:
+            raise VtxError(-3, f"{what} must be {self._q_shape} on {self.dev}, last axis contiguous")
+        if kind is None:
+            raise VtxError(-2, f"{what}: dtype {t.dtype}")
+        d.type, es = kind
+        nb[0], nb[token], nb[head], d.data = es, st[0] * es, st[1] * es, t.data_ptr()
 
     def _array(self, t: Optional[torch.Tensor], dtype: torch.dtype, what: str, cap: Optional[int]) -> Optional[int]:
         """Checks a (n_seq, n_head_kv, cap) row array; returns its cap."""
         if t is None:
             return cap
-        if t.dtype != dtype or t.dim() != 3 or t.shape[0] != self.n_seq or t.shape[1] != self.n_head_kv or \
-                not t.is_contiguous() or t.device != self.dev or (cap is not None and t.shape[2] != cap):
+        shape = t.shape
+        if len(shape) != 3 or shape[0] != self.n_seq or shape[1] != self.n_head_kv or t.dtype != dtype or \
+                not t.is_contiguous() or t.device != self.dev or (cap is not None and shape[2] != cap):
             raise VtxError(-3, f"{what} must be a contiguous ({self.n_seq}, {self.n_head_kv}, rows) {dtype} tensor")
-        return t.shape[2]
+        return shape[2]
 
     def _set_params(self, scale, causal, window, softcap) -> None:
         p = self._params
@@ -535,14 +545,15 @@ class PagedKv:
         p.logit_softcap, p.causal, p.window = softcap, 1 if causal else 0, window
 
     def _call(self, fn, args, stream: Optional[torch.cuda.Stream], *ws) -> None:
-        if self.dev.type != "cuda":
+        dev = self.dev
+        if dev.type != "cuda":
             raise VtxError(-8, "the pools are not on a GPU")
-        s = stream.cuda_stream if stream is not None else torch.cuda.current_stream(self.dev).cuda_stream
-        if torch.cuda.current_device() != self.dev.index:
-            with torch.cuda.device(self.dev):
-                rc = fn(ctypes.byref(args), *ws, ctypes.c_void_p(s))
+        s = stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(dev.index)
+        if torch.cuda.current_device() == dev.index:
+            rc = fn(ctypes.byref(args), *ws, s)
         else:
-            rc = fn(ctypes.byref(args), *ws, ctypes.c_void_p(s))
+            with torch.cuda.device(dev):
+                rc = fn(ctypes.byref(args), *ws, s)
         if rc != 0:
             raise VtxError(rc, fn.__name__)
 
@@ -555,30 +566,30 @@ class PagedKv:
         n_head_q, D) float32 rotated into q_out (float32 or float16; made as
         float16 when not given).  row_pos (int32) and score (float32),
         (n_seq, n_head_kv, rows): the new rows' entries are set."""
-        T, Hq, Hkv, D = self.n_tokens, self.n_head_q, self.n_head_kv, self.head_dim
-        for t, h in ((k, Hkv), (v, Hkv)) + (((q, Hq),) if q is not None else ()):
-            if t.dtype != torch.float32 or tuple(t.shape) != (T, h, D) or t.stride(2) != 1 or t.stride(1) != D:
-                raise VtxError(-4, f"q/k/v must be ({T}, heads, {D}) float32 with heads contiguous")
-        if positions.dtype != torch.int32 or positions.shape != (T,) or not positions.is_contiguous():
+        D, a = self.head_dim, self._append
+        ks, vs = k.stride(), v.stride()
+        if k.shape != self._kv_shape or v.shape != self._kv_shape or ks[2] != 1 or ks[1] != D or vs[2] != 1 or \
+                vs[1] != D or k.dtype != torch.float32 or v.dtype != torch.float32:
+            raise VtxError(-4, f"k and v must be {self._kv_shape} float32 with heads contiguous")
+        if positions.dtype != torch.int32 or positions.shape != (self.n_tokens,) or not positions.is_contiguous():
             raise VtxError(-3, "positions must be contiguous int32, one per token")
-        if q is not None and q_out is None:
-            q_out = torch.empty(q.shape, dtype=torch.float16, device=q.device)
-        a = self._append
-        if q_out is not None:
-            if q is None:
-                raise VtxError(-1, "q_out without q")
-            if tuple(q_out.shape) != (T, Hq, D) or q_out.stride(2) != 1 or q_out.stride(1) != D:
-                raise VtxError(-4, f"q_out must be ({T}, {Hq}, {D}) with heads contiguous")
-            a.n_head_q, a.q_out_type = Hq, _ggml_type(q_out, None)
-            a.q, a.q_nb1 = q.data_ptr(), q.stride(0) * 4
-            a.q_out, a.q_out_nb1 = q_out.data_ptr(), q_out.stride(0) * q_out.element_size()
+        if q is not None:
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=torch.float16, device=q.device)
+            qs, os_, kind = q.stride(), q_out.stride(), _ROW_TYPES.get(q_out.dtype)
+            if q.shape != self._q_shape or q_out.shape != self._q_shape or qs[2] != 1 or qs[1] != D or os_[2] != 1 or \
+                    os_[1] != D or q.dtype != torch.float32 or kind is None:
+                raise VtxError(-4, f"q (float32) and q_out must be {self._q_shape} with heads contiguous")
+            a.n_head_q, (a.q_out_type, es) = self.n_head_q, kind
+            a.q, a.q_nb1, a.q_out, a.q_out_nb1 = q.data_ptr(), qs[0] * 4, q_out.data_ptr(), os_[0] * es
+        elif q_out is not None:
+            raise VtxError(-1, "q_out without q")
         else:
             a.q = a.q_out = None
         a.freq_base = freq_base
-        a.k, a.k_nb1, a.v, a.v_nb1 = k.data_ptr(), k.stride(0) * 4, v.data_ptr(), v.stride(0) * 4
+        a.k, a.k_nb1, a.v, a.v_nb1 = k.data_ptr(), ks[0] * 4, v.data_ptr(), vs[0] * 4
         a.positions = positions.data_ptr()
-        cap = self._array(score, torch.float32, "score", self._array(row_pos, torch.int32, "row_pos", None))
-        a.row_cap = cap or 0
+        a.row_cap = self._array(score, torch.float32, "score", self._array(row_pos, torch.int32, "row_pos", None)) or 0
         a.row_pos = row_pos.data_ptr() if row_pos is not None else None
         a.score = score.data_ptr() if score is not None else None
         self._call(self._lib.vtx_kv_append_paged, a, stream)
@@ -592,16 +603,16 @@ class PagedKv:
         optional float32 (n_tokens, n_head_q) that receives ln sum exp.  scale
         defaults to D ** -0.5."""
         if out is None:
-            out = torch.empty((self.n_tokens, self.n_head_q, self.head_dim), dtype=torch.float32, device=self.dev)
-        self._rows(q, self.n_head_q, "q", self._q, 1, 2)
-        self._rows(out, self.n_head_q, "out", self._dst, 2, 1)
+            out = torch.empty(self._q_shape, dtype=torch.float32, device=self.dev)
+        self._rows(q, "q", self._q, self._q_nb, 1, 2)
+        self._rows(out, "out", self._dst, self._dst_nb, 2, 1)
         self._set_params(scale, causal, window, logit_softcap)
         self._attend.lse = self._check_lse(lse) if lse is not None else None
         self._call(self._lib.vtx_flash_attn_paged, self._attend, stream, *self._ws)
         return out
 
     def _check_lse(self, lse: torch.Tensor) -> int:
-        if lse.dtype != torch.float32 or tuple(lse.shape) != (self.n_tokens, self.n_head_q) or not lse.is_contiguous():
+        if lse.shape != self._q_shape[:2] or lse.dtype != torch.float32 or not lse.is_contiguous():
             raise VtxError(-3, "lse must be a contiguous float32 (n_tokens, n_head_q) tensor")
         return lse.data_ptr()
 
@@ -614,7 +625,7 @@ class PagedKv:
         score_out.  q and lse as attend read and wrote them."""
         out = score if score_out is None else score_out
         cap = self._array(out, torch.float32, "score_out", self._array(score, torch.float32, "score", None))
-        self._rows(q, self.n_head_q, "q", self._q, 1, 2)
+        self._rows(q, "q", self._q, self._q_nb, 1, 2)
         self._set_params(scale, causal, window, logit_softcap)
         a = self._score
         a.lse, a.score, a.score_out = self._check_lse(lse), score.data_ptr(), out.data_ptr()
@@ -644,7 +655,7 @@ class PagedKv:
         a.score, a.row_pos, a.next_pos, a.kv_len_out = score.data_ptr(), ptr(row_pos), ptr(next_pos), kv_len_out.data_ptr()
         a.score_out, a.pos_out, a.src_out = ptr(score_out), ptr(pos_out), ptr(src_out)
         a.keep, a.n_sink, a.n_recent = keep, n_sink, n_recent
-        self._call(self._lib.vtx_kv_evict_paged, a, stream, *self._ws)
+        self._call(self._lib.vtx_kv_evict_paged, a, stream, *self._evict_ws)
         return kv_len_out
 
 
