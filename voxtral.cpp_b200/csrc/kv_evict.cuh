@@ -22,12 +22,14 @@ struct PagedEvictArgs {
     int2 *moves;              // [n_seq * Hkv][max_moves] (source row, destination row)
     int2 *counts;             // [n_seq * Hkv] (moves, rows left)
     int max_moves;
-    int row_bytes, vec;       // bytes of one head's row; copy width
+    int row_bytes;            // bytes of one head's row
     int slices;               // CTAs per (stream, head) of the move kernel
 };
 
-constexpr int kEvictThreads = 1024;
+constexpr int kEvictThreads = 512, kEvictWarps = kEvictThreads / 32;
+constexpr int kEvictBins = 2048;                  // 11-bit digits: 11 + 11 + 10 bits of a key
 constexpr int kEvictKeysInSmem = 48 * 1024;       // rows whose keys fit in shared memory
+constexpr int kEvictBatch = 8;                    // moves a warp has in flight
 
 // Order-preserving key: protected rows above everything, NaN as -inf, -0 as +0.
 __device__ __forceinline__ uint32_t evict_key(float x, bool safe) {
@@ -37,34 +39,12 @@ __device__ __forceinline__ uint32_t evict_key(float x, bool safe) {
     return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
-// Exclusive sums over the CTA of two counts per thread; `total` gets both sums.
-__device__ __forceinline__ int2 evict_scan(int2 x, int2 *warp_sum, int2 &total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int2 inc = x;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int a = __shfl_up_sync(0xffffffffu, inc.x, o), b = __shfl_up_sync(0xffffffffu, inc.y, o);
-        if (lane >= o) { inc.x += a; inc.y += b; }
-    }
-    __syncthreads();
-    if (lane == 31) warp_sum[warp] = inc;
-    __syncthreads();
-    int2 base = make_int2(0, 0);
-    total = make_int2(0, 0);
-#pragma unroll
-    for (int w = 0; w < kEvictThreads / 32; ++w) {
-        if (w == warp) base = total;
-        total.x += warp_sum[w].x;
-        total.y += warp_sum[w].y;
-    }
-    return make_int2(base.x + inc.x - x.x, base.y + inc.y - x.y);
-}
-
-// The m-th largest key by a radix select, 8 bits at a time from the top: a
-// histogram of the keys that match the prefix so far, then the bin that holds
-// the m-th.  Rows with a larger key are kept, of those with an equal one the
-// first ones.  Each thread owns a run of E consecutive rows, so two block
-// scans number the gaps and the moved rows in row order.
+// The m-th largest key by a radix select from the top digit down: a histogram of
+// the keys that match the prefix so far, then the bin that holds the m-th.  Rows
+// with a larger key are kept, of those with an equal one the first ones.  A warp
+// owns a run of rows and walks it 32 at a time, so ballots number the equal keys,
+// the gaps and the moved rows in row order.  Bound by latency: about a dozen
+// barriers and four dependent trips to memory per (stream, head).
 template <bool SMEM>
 __global__ void __launch_bounds__(kEvictThreads)
 kv_evict_select_kernel(const PagedEvictArgs a)
@@ -72,13 +52,14 @@ kv_evict_select_kernel(const PagedEvictArgs a)
     grid_dep_wait();
     grid_dep_launch();
     extern __shared__ uint32_t keys[];
-    __shared__ int hist[256];
-    __shared__ int2 warp_sum[kEvictThreads / 32];
+    __shared__ int hist[kEvictBins];
+    __shared__ int2 warp_sum[kEvictWarps];
     __shared__ int pick[2];
     const int b = blockIdx.x / a.kv.Hkv;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const unsigned below = (1u << lane) - 1;
     const long long item = blockIdx.x;
-    int n = a.kv.kv_len[b];
+    const int n = a.kv.kv_len[b];
     const int most = (int)min((long long)min(a.kv.max_kv, a.row_cap), (long long)a.kv.max_pages << a.kv.shift);
     if (n < 0 || n > most) {                       // nothing of this stream is touched
         if (tid == 0) {
@@ -95,78 +76,109 @@ kv_evict_select_kernel(const PagedEvictArgs a)
         const int p = row_pos ? row_pos[j] : j;
         return evict_key(score[j], p < a.n_sink || p >= recent);
     };
-    if (SMEM) {
+    const bool some = m > 0 && m < n;              // there is a choice to make
+    if (SMEM && some)
         for (int j = tid; j < n; j += kEvictThreads) keys[j] = key_of(j);
-    }
     uint32_t prefix = 0;
     int need = m;                                  // rank of the threshold among the keys that match the prefix
-    if (m < n && m > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
+    if (some) {
+#pragma unroll
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+            for (int i = tid; i < kEvictBins; i += kEvictThreads) hist[i] = 0;
             __syncthreads();
             for (int j = tid; j < n; j += kEvictThreads) {
                 const uint32_t k = SMEM ? keys[j] : key_of(j);
-                if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
+                if (pass == 0 || (k >> (shift + bits)) == (prefix >> (shift + bits)))
+                    atomicAdd(&hist[(k >> shift) & ((1 << bits) - 1)], 1);
             }
             __syncthreads();
-            if (tid < 32) {                        // lane l: bins 255 - 8l ... 248 - 8l, from the top
-                int c[8], t = 0;
+            // thread i: the four bins from 2047 - 4i down; the sum of all above it by a scan
+            int c[4], t = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) { c[i] = hist[255 - 8 * tid - i]; t += c[i]; }
-                int inc = t;
+            for (int i = 0; i < 4; ++i) { c[i] = hist[kEvictBins - 1 - 4 * tid - i]; t += c[i]; }
+            int inc = t;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int x = __shfl_up_sync(0xffffffffu, inc, o);
-                    if (tid >= o) inc += x;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += x;
+            }
+            if (lane == 31) warp_sum[warp].x = inc;
+            __syncthreads();
+            int above = inc - t;
+#pragma unroll
+            for (int w = 0; w < kEvictWarps; ++w) above += w < warp ? warp_sum[w].x : 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (above < need && above + c[i] >= need) {
+                    pick[0] = kEvictBins - 1 - 4 * tid - i;
+                    pick[1] = need - above;
                 }
-                int above = inc - t;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (above < need && above + c[i] >= need) { pick[0] = 255 - 8 * tid - i; pick[1] = need - above; }
-                    above += c[i];
-                }
+                above += c[i];
             }
             __syncthreads();
             prefix |= (uint32_t)pick[0] << shift;
             need = pick[1];
         }
     }
-    __syncthreads();
     // keys > prefix stay, and the first `need` of those equal to it
-    const bool all = m == n;
-    const int E = (n + kEvictThreads - 1) / kEvictThreads;
-    const int j0 = min(tid * E, n), j1 = min(j0 + E, n);
+    const int run = (n + kEvictThreads - 1) / kEvictThreads * 32;
+    const int r0 = min(warp * run, n), r1 = min(r0 + run, n);
+    // exclusive sums over the warps of two counts, and their totals
+    auto sums = [&](int x, int y, int2 &total) {
+        __syncthreads();
+        if (lane == 0) warp_sum[warp] = make_int2(x, y);
+        __syncthreads();
+        int2 before = make_int2(0, 0);
+        total = before;
+#pragma unroll
+        for (int w = 0; w < kEvictWarps; ++w) {
+            if (w == warp) before = total;
+            total.x += warp_sum[w].x;
+            total.y += warp_sum[w].y;
+        }
+        return before;
+    };
     int2 tot;
-    int eq = 0;
-    if (!all && m > 0)
-        for (int j = j0; j < j1; ++j) eq += (SMEM ? keys[j] : key_of(j)) == prefix;
-    const int eq0 = evict_scan(make_int2(eq, 0), warp_sum, tot).x;
-    auto each = [&](auto f) {                      // f(row, kept) over this thread's rows
+    int eq0 = 0;
+    if (some) {
+        for (int j = r0 + lane; j - lane < r1; j += 32)
+            eq0 += __popc(__ballot_sync(0xffffffffu, j < r1 && (SMEM ? keys[j] : key_of(j)) == prefix));
+        eq0 = sums(eq0, 0, tot).x;
+    }
+    auto each = [&](auto f) {                      // f(row, live, kept), a warp's rows in order
         int e = eq0;
-        for (int j = j0; j < j1; ++j) {
-            bool kept = all;
-            if (!all && m > 0) {
-                const uint32_t k = SMEM ? keys[j] : key_of(j);
-                kept = k > prefix || (k == prefix && e < need);
-                e += k == prefix;
+        for (int j = r0 + lane; j - lane < r1; j += 32) {
+            const bool live = j < r1;
+            bool kept = live && m == n;
+            if (some) {
+                const uint32_t k = live ? (SMEM ? keys[j] : key_of(j)) : 0u;
+                const unsigned same = __ballot_sync(0xffffffffu, live && k == prefix);
+                kept = live && (k > prefix || (k == prefix && e + __popc(same & below) < need));
+                e += __popc(same);
             }
-            f(j, kept);
+            f(j, live, kept);
         }
     };
-    int2 cnt = make_int2(0, 0);                    // gaps below m, kept rows behind it
-    each([&](int j, bool kept) {
-        cnt.x += j < m && !kept;
-        cnt.y += j >= m && kept;
-    });
-    int2 at = evict_scan(cnt, warp_sum, tot);
+    int gaps = 0, late = 0;                        // gaps below m, kept rows behind it
+    if (some)
+        each([&](int j, bool live, bool kept) {
+            gaps += __popc(__ballot_sync(0xffffffffu, live && j < m && !kept));
+            late += __popc(__ballot_sync(0xffffffffu, j >= m && kept));
+        });
+    int2 at = sums(gaps, late, tot);
     int2 *mv = a.moves + item * a.max_moves;
     float *so = a.score_out ? a.score_out + item * a.out_cap : nullptr;
     int *po = a.pos_out ? a.pos_out + item * a.out_cap : nullptr;
     int *ro = a.src_out ? a.src_out + item * a.out_cap : nullptr;
-    each([&](int j, bool kept) {
-        if (j < m && !kept) mv[at.x++].y = j;
-        if (j >= m && kept) mv[at.y++].x = j;
-        if (j < m && kept) {                       // in place these write what is there
+    each([&](int j, bool live, bool kept) {
+        const unsigned gap = __ballot_sync(0xffffffffu, live && j < m && !kept);
+        const unsigned far = __ballot_sync(0xffffffffu, j >= m && kept);
+        if ((gap >> lane) & 1u) mv[at.x + __popc(gap & below)].y = j;
+        if ((far >> lane) & 1u) mv[at.y + __popc(far & below)].x = j;
+        at.x += __popc(gap);
+        at.y += __popc(far);
+        if (j < m && kept) {                       // in place these stand already
             if (so && so != score) so[j] = score[j];
             if (po && po != row_pos) po[j] = row_pos ? row_pos[j] : j;
             if (ro) ro[j] = j;
@@ -182,12 +194,11 @@ kv_evict_select_kernel(const PagedEvictArgs a)
     if (tid == 0) a.counts[item] = make_int2(tot.x, m);
 }
 
-template <typename V>
-__device__ __forceinline__ void evict_copy_row(char *dst, const char *src, int n, int lane) {
-    for (int i = lane; i < n; i += 32) reinterpret_cast<V *>(dst)[i] = reinterpret_cast<const V *>(src)[i];
-}
-
-// Grid (n_seq * Hkv * slices), a warp per move.
+// Grid (n_seq * Hkv * slices).  A warp copies eight moves at a time: lanes 0-7
+// read the moves and their pages, then half of the warp takes the K row and half
+// the V row of each move, all loads before the first store.  V: the copy's unit
+// (16, 8 or 4 bytes), N units per lane and row.
+template <typename V, int N>
 __global__ void __launch_bounds__(256)
 kv_evict_move_kernel(const PagedEvictArgs a)
 {
@@ -200,19 +211,34 @@ kv_evict_move_kernel(const PagedEvictArgs a)
     const int2 c = a.counts[item];
     if (slice == 0 && g == 0 && threadIdx.x == 0) a.kv_len_out[b] = c.y;
     const int2 *mv = a.moves + (long long)item * a.max_moves;
-    for (int i = slice * 8 + warp; i < c.x; i += a.slices * 8) {
-        const int2 x = mv[i];
-        const int ps = paged_page(a.kv, b, x.x), pd = paged_page(a.kv, b, x.y);
-        if (ps < 0 || pd < 0) continue;
-        const int mask = (1 << a.kv.shift) - 1;
-        const long long src = (long long)ps * a.kv.nb3 + (long long)(x.x & mask) * a.kv.nb1 + (long long)g * a.kv.nb2;
-        const long long dst = (long long)pd * a.kv.nb3 + (long long)(x.y & mask) * a.kv.nb1 + (long long)g * a.kv.nb2;
-        if (a.vec == 16) {
-            evict_copy_row<uint4>(a.kv.k + dst, a.kv.k + src, a.row_bytes / 16, lane);
-            evict_copy_row<uint4>(a.kv.v + dst, a.kv.v + src, a.row_bytes / 16, lane);
-        } else {
-            evict_copy_row<uint32_t>(a.kv.k + dst, a.kv.k + src, a.row_bytes / 4, lane);
-            evict_copy_row<uint32_t>(a.kv.v + dst, a.kv.v + src, a.row_bytes / 4, lane);
+    char *pool = lane < 16 ? a.kv.k : a.kv.v;
+    const int units = a.row_bytes / (int)sizeof(V), u0 = lane & 15;
+    const long long head = (long long)g * a.kv.nb2;
+    const int mask = (1 << a.kv.shift) - 1;
+    for (int i0 = (slice * 8 + warp) * kEvictBatch; i0 < c.x; i0 += a.slices * 8 * kEvictBatch) {
+        long long src = -1, dst = -1;
+        if (lane < kEvictBatch && i0 + lane < c.x) {
+            const int2 x = mv[i0 + lane];
+            const int ps = paged_page(a.kv, b, x.x), pd = paged_page(a.kv, b, x.y);
+            if (ps >= 0 && pd >= 0) {
+                src = head + (long long)ps * a.kv.nb3 + (long long)(x.x & mask) * a.kv.nb1;
+                dst = head + (long long)pd * a.kv.nb3 + (long long)(x.y & mask) * a.kv.nb1;
+            }
+        }
+        V v[kEvictBatch][N];
+#pragma unroll
+        for (int i = 0; i < kEvictBatch; ++i) {
+            const long long at = __shfl_sync(0xffffffffu, src, i);
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (at >= 0 && u0 + 16 * k < units) v[i][k] = reinterpret_cast<const V *>(pool + at)[u0 + 16 * k];
+        }
+#pragma unroll
+        for (int i = 0; i < kEvictBatch; ++i) {
+            const long long at = __shfl_sync(0xffffffffu, dst, i);
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (at >= 0 && u0 + 16 * k < units) reinterpret_cast<V *>(pool + at)[u0 + 16 * k] = v[i][k];
         }
     }
 }

@@ -549,8 +549,7 @@ int vtx_kv_evict_paged(const vtx_kv_evict_paged_args *p, void *workspace, size_t
     a.moves = static_cast<int2 *>(workspace);
     a.counts = reinterpret_cast<int2 *>(static_cast<char *>(workspace) + e.moves_bytes);
     a.row_bytes = row_bytes(kv->k.type, kv->k.ne[0]);
-    a.vec = kv->k.type == VTX_TYPE_F16 ? 16 : 4;
-    // about eight CTAs per SM over all items, at most one per 64 possible moves
+    // a CTA per 64 moves at most (8 warps of 8), about eight CTAs per SM over all
     a.slices = (int)std::max<long long>(1, std::min<long long>((8LL * ds->sms + e.items - 1) / e.items,
                                                                (e.max_moves + 63) / 64));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -564,7 +563,11 @@ int vtx_kv_evict_paged(const vtx_kv_evict_paged_args *p, void *workspace, size_t
         rc = launch_pdl(kv_evict_select_kernel<false>, dim3((unsigned)e.items), dim3(kEvictThreads), 0, st, a);
     }
     if (rc != VTX_OK) return rc;
-    return launch_pdl(kv_evict_move_kernel, dim3((unsigned)(e.items * a.slices)), dim3(256), 0, st, a);
+    const dim3 grid((unsigned)(e.items * a.slices));
+    // rows of 256 or 128 (F16), 136 or 68 bytes (Q8_0: 8- and 4-byte aligned)
+    if (kv->k.type == VTX_TYPE_F16) return launch_pdl(kv_evict_move_kernel<uint4, 1>, grid, dim3(256), 0, st, a);
+    if (a.row_bytes % 8 == 0) return launch_pdl(kv_evict_move_kernel<uint2, 2>, grid, dim3(256), 0, st, a);
+    return launch_pdl(kv_evict_move_kernel<uint32_t, 2>, grid, dim3(256), 0, st, a);
 }
 
 }  // extern "C"
