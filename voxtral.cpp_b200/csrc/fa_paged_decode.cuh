@@ -36,6 +36,7 @@ struct PagedSplit {
     int tiles;                // 16-key tiles per split at least
     float *part_o, *part_ml;  // [n_seq][Hkv][n_splits][ROWS][D], ... [2] (m, l)
     unsigned *arrived;        // [n_seq][Hkv], zero between calls
+    int beside;               // runs beside the kernel launched just before (see the kernel)
 };
 
 template <int D, int KVT> struct PagedDecodeCfg {
@@ -208,11 +209,8 @@ __device__ __forceinline__ void paged_finish(const PagedAttnArgs &a, const Paged
 }
 
 template <int D, int KVT, int ROWS, bool UF>
-__global__ void __launch_bounds__(128, 3)
-fa_paged_decode_kernel(const PagedAttnArgs a, const PagedSplit sp)
+__device__ __forceinline__ void paged_decode_cta(const PagedAttnArgs &a, const PagedSplit &sp)
 {
-    grid_dep_wait();
-    grid_dep_launch();
     using C = PagedDecodeCfg<D, KVT>;
     constexpr int KC = D / 16, NB = D / 8;
     extern __shared__ __align__(128) char smem[];
@@ -459,6 +457,21 @@ fa_paged_decode_kernel(const PagedAttnArgs a, const PagedSplit sp)
         }
         if (lane < LPR) paged_finish<D>(a, s, g, r, d, acc, top, tot);
     }
+}
+
+// sp.beside: the kernel just before is the chunks' (fa_paged_sm100_kernel), which
+// touches other streams' rows only.  It started once everything before it was
+// complete, and this kernel starts once all of its CTAs have, so nothing needs to
+// be waited for: the few-token streams fill the SMs that its last CTAs leave
+// idle.  The wait comes last instead, so that this kernel's end is both ends.
+template <int D, int KVT, int ROWS, bool UF>
+__global__ void __launch_bounds__(128, 3)
+fa_paged_decode_kernel(const PagedAttnArgs a, const PagedSplit sp)
+{
+    if (!sp.beside) grid_dep_wait();
+    grid_dep_launch();
+    paged_decode_cta<D, KVT, ROWS, UF>(a, sp);
+    if (sp.beside) grid_dep_wait();
 }
 
 }  // namespace vtx

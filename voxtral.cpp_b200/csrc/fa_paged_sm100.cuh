@@ -512,7 +512,8 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     }
 }
 
-// Merges the splits: grid (n_tokens), a warp per query head, a lane per 4 dims.
+// Merges the splits: grid (n_tokens, ceil(Hq / 8)), a warp per query head, a lane
+// per 4 dims; at most 32 splits, whose (m, l) the lanes read at once.
 template <int D>
 __global__ void __launch_bounds__(256)
 fa_paged_tile_combine_kernel(const PagedAttnArgs a, const PagedTile tl)
@@ -523,38 +524,41 @@ fa_paged_tile_combine_kernel(const PagedAttnArgs a, const PagedTile tl)
     const int b = paged_find(a.kv, t);
     if (b >= a.kv.n_seq) return;
     const PagedSeq s = paged_seq(a.kv, b);
-    const int tok = t - s.q0;
-    if (tok < 0 || tok >= min(s.n_new, a.kv.max_new) || paged_groups(min(s.n_new, a.kv.max_new), a, tl) == 0) return;
+    const int tok = t - s.q0, served = min(s.n_new, a.kv.max_new);
+    if (tok < 0 || tok >= served || paged_groups(served, a, tl) == 0) return;
     const int n = paged_range(s, tok / (2 * tl.T) * 2 * tl.T, a, tl).n;
-    if (n == 1) return;
-    const int lane = threadIdx.x & 31, d = lane * 4;
-    const long long step = (long long)a.kv.n_tokens * a.Hq;
-    for (int h = threadIdx.x >> 5; h < a.Hq; h += 8) {
-        const long long row = (long long)t * a.Hq + h;
-        float top = -INFINITY;
-        for (int i = 0; i < n; ++i) top = fmaxf(top, tl.part_ml[(i * step + row) * 2]);
-        float l = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (top != -INFINITY) {
-#pragma unroll 4
-            for (int i = 0; i < n; ++i) {
-                const float2 y = reinterpret_cast<const float2 *>(tl.part_ml)[i * step + row];
-                const float f = ex2(y.x - top);
-                l = fmaf(f, y.y, l);
-                if (d < D) {
-                    const float4 v = *reinterpret_cast<const float4 *>(tl.part_o + (i * step + row) * D + d);
-                    acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y);
-                    acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
-                }
-            }
+    const int lane = threadIdx.x & 31, d = lane * 4, h = blockIdx.y * 8 + (threadIdx.x >> 5);
+    if (n == 1 || h >= a.Hq) return;
+    const long long step = (long long)a.kv.n_tokens * a.Hq, row = (long long)t * a.Hq + h;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < n) ml = reinterpret_cast<const float2 *>(tl.part_ml)[lane * step + row];
+    float top = ml.x;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+    float l = f * ml.y;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < n; i0 += 4) {
+        float4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            v[u] = i0 + u < n && d < D ? *reinterpret_cast<const float4 *>(tl.part_o + ((i0 + u) * step + row) * D + d)
+                                       : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float w = __shfl_sync(0xffffffffu, f, (i0 + u) & 31);
+            acc.x = fmaf(w, v[u].x, acc.x); acc.y = fmaf(w, v[u].y, acc.y);
+            acc.z = fmaf(w, v[u].z, acc.z); acc.w = fmaf(w, v[u].w, acc.w);
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        if (d < D) {
-            paged_store2(a, t, h, d, acc.x * inv, acc.y * inv);
-            paged_store2(a, t, h, d + 2, acc.z * inv, acc.w * inv);
-        }
-        if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
     }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (d < D) {
+        paged_store2(a, t, h, d, acc.x * inv, acc.y * inv);
+        paged_store2(a, t, h, d + 2, acc.z * inv, acc.w * inv);
+    }
+    if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
 }
 
 }  // namespace vtx

@@ -1,10 +1,10 @@
 // kv_evict.cuh — eviction of a paged cache's rows by score, in place.
 //
-// Per (stream, KV head), of n rows the m = min(n, keep) best stay.  Two
-// kernels: kv_evict_select_kernel finds them (one CTA per (stream, head)),
-// writes the new score / position / source arrays and the list of moves;
-// kv_evict_move_kernel copies the K and V rows of the moves and writes the new
-// lengths.  A move takes a kept row at or behind m to a gap below m, so no row
+// Per (stream, KV head), of n rows the m = min(n, keep) best stay.
+// kv_evict_select_kernel finds them (one CTA per (stream, head)), writes the new
+// score / position / source arrays and the list of moves; kv_evict_move_kernel
+// copies the K and V rows of the moves and writes the new lengths.  With few
+// moves the first kernel does that too (UNIT > 0).  A move takes a kept row at or behind m to a gap below m, so no row
 // is both read and written and the moves run in any order.
 #pragma once
 #include <cuda_fp16.h>
@@ -39,13 +39,59 @@ __device__ __forceinline__ uint32_t evict_key(float x, bool safe) {
     return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
+// Copies moves i0, i0 + step, ... (batches of eight) of a (stream, head): lanes
+// 0-7 read the moves and their pages, then half of the warp takes the K row and
+// half the V row of each move, all loads before the first store.  UNIT: bytes a
+// lane copies at once (16, 8 or 4).
+template <int UNIT> struct EvictUnit;
+template <> struct EvictUnit<16> { using V = uint4; };
+template <> struct EvictUnit<8> { using V = uint2; };
+template <> struct EvictUnit<4> { using V = uint32_t; };
+template <int UNIT>
+__device__ __forceinline__ void evict_move(const PagedEvictArgs &a, const int2 *mv, int count, int i0, int step, int b,
+                                           int g, int lane)
+{
+    using V = typename EvictUnit<UNIT>::V;
+    constexpr int N = UNIT == 16 ? 1 : 2;          // rows of 128 / 256, 136 and 68 bytes over 16 lanes
+    char *pool = lane < 16 ? a.kv.k : a.kv.v;
+    const int units = a.row_bytes / UNIT, u0 = lane & 15;
+    const long long head = (long long)g * a.kv.nb2;
+    const int mask = (1 << a.kv.shift) - 1;
+    for (; i0 < count; i0 += step) {
+        long long src = -1, dst = -1;
+        if (lane < kEvictBatch && i0 + lane < count) {
+            const int2 x = mv[i0 + lane];
+            const int ps = paged_page(a.kv, b, x.x), pd = paged_page(a.kv, b, x.y);
+            if (ps >= 0 && pd >= 0) {
+                src = head + (long long)ps * a.kv.nb3 + (long long)(x.x & mask) * a.kv.nb1;
+                dst = head + (long long)pd * a.kv.nb3 + (long long)(x.y & mask) * a.kv.nb1;
+            }
+        }
+        V v[kEvictBatch][N];
+#pragma unroll
+        for (int i = 0; i < kEvictBatch; ++i) {
+            const long long at = __shfl_sync(0xffffffffu, src, i);
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (at >= 0 && u0 + 16 * k < units) v[i][k] = reinterpret_cast<const V *>(pool + at)[u0 + 16 * k];
+        }
+#pragma unroll
+        for (int i = 0; i < kEvictBatch; ++i) {
+            const long long at = __shfl_sync(0xffffffffu, dst, i);
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (at >= 0 && u0 + 16 * k < units) reinterpret_cast<V *>(pool + at)[u0 + 16 * k] = v[i][k];
+        }
+    }
+}
+
 // The m-th largest key by a radix select from the top digit down: a histogram of
 // the keys that match the prefix so far, then the bin that holds the m-th.  Rows
 // with a larger key are kept, of those with an equal one the first ones.  A warp
 // owns a run of rows and walks it 32 at a time, so ballots number the equal keys,
 // the gaps and the moved rows in row order.  Bound by latency: about a dozen
 // barriers and four dependent trips to memory per (stream, head).
-template <bool SMEM>
+template <bool SMEM, int UNIT>
 __global__ void __launch_bounds__(kEvictThreads)
 kv_evict_select_kernel(const PagedEvictArgs a)
 {
@@ -64,7 +110,8 @@ kv_evict_select_kernel(const PagedEvictArgs a)
     if (n < 0 || n > most) {                       // nothing of this stream is touched
         if (tid == 0) {
             paged_report(a.kv, VTX_KERR_BOUND);
-            a.counts[item] = make_int2(0, n);
+            if (UNIT == 0) a.counts[item] = make_int2(0, n);
+            else if (item % a.kv.Hkv == 0) a.kv_len_out[b] = n;
         }
         return;
     }
@@ -191,56 +238,27 @@ kv_evict_select_kernel(const PagedEvictArgs a)
         if (po) po[x.y] = row_pos ? row_pos[x.x] : x.x;
         if (ro) ro[x.y] = x.x;
     }
-    if (tid == 0) a.counts[item] = make_int2(tot.x, m);
+    if constexpr (UNIT == 0) {
+        if (tid == 0) a.counts[item] = make_int2(tot.x, m);
+    } else {
+        evict_move<UNIT>(a, mv, tot.x, warp * kEvictBatch, kEvictWarps * kEvictBatch, b, (int)(item % a.kv.Hkv), lane);
+        if (tid == 0 && item % a.kv.Hkv == 0) a.kv_len_out[b] = m;
+    }
 }
 
-// Grid (n_seq * Hkv * slices).  A warp copies eight moves at a time: lanes 0-7
-// read the moves and their pages, then half of the warp takes the K row and half
-// the V row of each move, all loads before the first store.  V: the copy's unit
-// (16, 8 or 4 bytes), N units per lane and row.
-template <typename V, int N>
+// Grid (n_seq * Hkv * slices).
+template <int UNIT>
 __global__ void __launch_bounds__(256)
 kv_evict_move_kernel(const PagedEvictArgs a)
 {
     grid_dep_wait();
     grid_dep_launch();
-    const int slice = blockIdx.x % a.slices;
-    const int item = blockIdx.x / a.slices;
+    const int slice = blockIdx.x % a.slices, item = blockIdx.x / a.slices;
     const int g = item % a.kv.Hkv, b = item / a.kv.Hkv;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int2 c = a.counts[item];
     if (slice == 0 && g == 0 && threadIdx.x == 0) a.kv_len_out[b] = c.y;
-    const int2 *mv = a.moves + (long long)item * a.max_moves;
-    char *pool = lane < 16 ? a.kv.k : a.kv.v;
-    const int units = a.row_bytes / (int)sizeof(V), u0 = lane & 15;
-    const long long head = (long long)g * a.kv.nb2;
-    const int mask = (1 << a.kv.shift) - 1;
-    for (int i0 = (slice * 8 + warp) * kEvictBatch; i0 < c.x; i0 += a.slices * 8 * kEvictBatch) {
-        long long src = -1, dst = -1;
-        if (lane < kEvictBatch && i0 + lane < c.x) {
-            const int2 x = mv[i0 + lane];
-            const int ps = paged_page(a.kv, b, x.x), pd = paged_page(a.kv, b, x.y);
-            if (ps >= 0 && pd >= 0) {
-                src = head + (long long)ps * a.kv.nb3 + (long long)(x.x & mask) * a.kv.nb1;
-                dst = head + (long long)pd * a.kv.nb3 + (long long)(x.y & mask) * a.kv.nb1;
-            }
-        }
-        V v[kEvictBatch][N];
-#pragma unroll
-        for (int i = 0; i < kEvictBatch; ++i) {
-            const long long at = __shfl_sync(0xffffffffu, src, i);
-#pragma unroll
-            for (int k = 0; k < N; ++k)
-                if (at >= 0 && u0 + 16 * k < units) v[i][k] = reinterpret_cast<const V *>(pool + at)[u0 + 16 * k];
-        }
-#pragma unroll
-        for (int i = 0; i < kEvictBatch; ++i) {
-            const long long at = __shfl_sync(0xffffffffu, dst, i);
-#pragma unroll
-            for (int k = 0; k < N; ++k)
-                if (at >= 0 && u0 + 16 * k < units) reinterpret_cast<V *>(pool + at)[u0 + 16 * k] = v[i][k];
-        }
-    }
+    evict_move<UNIT>(a, a.moves + (long long)item * a.max_moves, c.x, (slice * 8 + (threadIdx.x >> 5)) * kEvictBatch,
+                     a.slices * 8 * kEvictBatch, b, g, threadIdx.x & 31);
 }
 
 }  // namespace vtx

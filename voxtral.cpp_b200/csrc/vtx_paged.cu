@@ -224,7 +224,12 @@ TilePlan plan_tile(const vtx_paged_kv *p, int G, int Hq, int min_rows, int sms) 
             t.tile.n_splits = s;
         }
     }
+#ifdef NSPLIT
+    t.tile.n_splits = NSPLIT;
+#endif
     if (t.tile.n_splits > 1) {
+        // every split that long, so that shorter streams have fewer
+        t.tile.min_tiles = std::max(2, (tiles + t.tile.n_splits - 1) / t.tile.n_splits);
         const size_t rows = (size_t)p->n_tokens * Hq * t.tile.n_splits;
         t.o_bytes = align_up(rows * D * 4, 256);
         t.bytes = t.o_bytes + align_up(rows * 8, 256);
@@ -271,10 +276,14 @@ int launch_tile(const CUtensorMap (&m)[3], const PagedAttnArgs &a, const PagedTi
     const long long ctas = (long long)tl.groups * a.kv.Hkv * tl.n_splits;
     if (ctas > 0x7fffffffLL) return VTX_ERR_UNSUPPORTED;
     if (ctas == 0) return VTX_OK;
-    rc = launch_pdl(fa_paged_sm100_kernel<D, UF>, dim3((unsigned)ctas), dim3(C::NTHREADS), C::SMEM, st, m[0], m[1],
-                    m[2], a, tl);
-    if (rc != VTX_OK || tl.n_splits == 1) return rc;
-    return launch_pdl(fa_paged_tile_combine_kernel<D>, dim3((unsigned)a.kv.n_tokens), dim3(256), 0, st, a, tl);
+    return launch_pdl(fa_paged_sm100_kernel<D, UF>, dim3((unsigned)ctas), dim3(C::NTHREADS), C::SMEM, st, m[0], m[1],
+                      m[2], a, tl);
+}
+
+template <int D>
+int launch_tile_combine(const PagedAttnArgs &a, const PagedTile &tl, cudaStream_t st) {
+    return launch_pdl(fa_paged_tile_combine_kernel<D>, dim3((unsigned)a.kv.n_tokens, (unsigned)((a.Hq + 7) / 8)),
+                      dim3(256), 0, st, a, tl);
 }
 
 template <int D, int KVT>
@@ -343,6 +352,17 @@ EvictPlan plan_evict(const vtx_paged_kv *p) {
     e.moves_bytes = align_up((size_t)e.items * e.max_moves * sizeof(int2), 256);
     e.bytes = e.moves_bytes + align_up((size_t)e.items * sizeof(int2), 256);
     return e;
+}
+
+template <bool SMEM, int UNIT>
+int launch_evict_select(const PagedEvictArgs &a, long long items, cudaStream_t st) {
+    const size_t keys = SMEM ? (size_t)a.kv.max_kv * 4 : 0;
+    if (SMEM) {
+        static std::atomic<int> done[kMaxDevices];
+        const int rc = allow_smem(kv_evict_select_kernel<SMEM, UNIT>, kEvictKeysInSmem * 4, done);
+        if (rc != VTX_OK) return rc;
+    }
+    return launch_pdl(kv_evict_select_kernel<SMEM, UNIT>, dim3((unsigned)items), dim3(kEvictThreads), keys, st, a);
 }
 
 }  // namespace
@@ -441,16 +461,8 @@ int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, si
     a.causal = p->params->causal != 0; a.window = p->params->window;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool f16 = kv->k.type == VTX_TYPE_F16, d64 = kv->k.ne[0] == 64;
-    if (dp.use) {
-        char *ws = static_cast<char *>(workspace);
-        dp.split.arrived = reinterpret_cast<unsigned *>(ws);
-        dp.split.part_o = reinterpret_cast<float *>(ws + dp.c_bytes);
-        dp.split.part_ml = reinterpret_cast<float *>(ws + dp.c_bytes + dp.o_bytes);
-        rc = d64 ? (f16 ? launch_decode_rows<64, 1>(a, dp, st) : launch_decode_rows<64, 8>(a, dp, st))
-                 : (f16 ? launch_decode_rows<128, 1>(a, dp, st) : launch_decode_rows<128, 8>(a, dp, st));
-        if (rc != VTX_OK || kv->max_new * (long long)a.G <= kFewRows) return rc;
-        a.min_rows = dp.rows;
-    }
+    // chunks first (their CTAs are long), few-token streams beside them
+    a.min_rows = dp.use ? dp.rows : 0;
     if (tp.use) {
         char *ws = static_cast<char *>(workspace) + dp.bytes;
         tp.tile.part_o = reinterpret_cast<float *>(ws);
@@ -463,10 +475,24 @@ int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, si
         if (rc != VTX_OK) return rc;
         // tanh, or a scale that the row maximum cannot carry: logits formed first
         const bool uf = a.softcap != 0.0f || !(a.scale > 0.0f);
-        if (d64) return uf ? launch_tile<64, true>(m, a, tp.tile, st) : launch_tile<64, false>(m, a, tp.tile, st);
-        return uf ? launch_tile<128, true>(m, a, tp.tile, st) : launch_tile<128, false>(m, a, tp.tile, st);
+        if (d64) rc = uf ? launch_tile<64, true>(m, a, tp.tile, st) : launch_tile<64, false>(m, a, tp.tile, st);
+        else rc = uf ? launch_tile<128, true>(m, a, tp.tile, st) : launch_tile<128, false>(m, a, tp.tile, st);
+    } else if (kv->max_new * (long long)a.G > a.min_rows) {
+        rc = d64 ? launch_attn<64, 8>(a, st) : launch_attn<128, 8>(a, st);
     }
-    return d64 ? launch_attn<64, 8>(a, st) : launch_attn<128, 8>(a, st);
+    if (rc != VTX_OK) return rc;
+    if (dp.use) {
+        char *ws = static_cast<char *>(workspace);
+        dp.split.arrived = reinterpret_cast<unsigned *>(ws);
+        dp.split.part_o = reinterpret_cast<float *>(ws + dp.c_bytes);
+        dp.split.part_ml = reinterpret_cast<float *>(ws + dp.c_bytes + dp.o_bytes);
+        dp.split.beside = kv->max_new * (long long)a.G > a.min_rows;
+        rc = d64 ? (f16 ? launch_decode_rows<64, 1>(a, dp, st) : launch_decode_rows<64, 8>(a, dp, st))
+                 : (f16 ? launch_decode_rows<128, 1>(a, dp, st) : launch_decode_rows<128, 8>(a, dp, st));
+        if (rc != VTX_OK) return rc;
+    }
+    if (!tp.use || tp.tile.n_splits == 1) return VTX_OK;
+    return d64 ? launch_tile_combine<64>(a, tp.tile, st) : launch_tile_combine<128>(a, tp.tile, st);
 }
 
 int vtx_kv_score_paged(const vtx_kv_score_paged_args *p, void *stream) {
@@ -552,22 +578,23 @@ int vtx_kv_evict_paged(const vtx_kv_evict_paged_args *p, void *workspace, size_t
     // a CTA per 64 moves at most (8 warps of 8), about eight CTAs per SM over all
     a.slices = (int)std::max<long long>(1, std::min<long long>((8LL * ds->sms + e.items - 1) / e.items,
                                                                (e.max_moves + 63) / 64));
+    // rows of 256 or 128 (F16), 136 or 68 bytes (Q8_0: 8- and 4-byte aligned)
+    const int unit = kv->k.type == VTX_TYPE_F16 ? 16 : a.row_bytes % 8 == 0 ? 8 : 4;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int keys = std::min(kv->max_kv_len, kEvictKeysInSmem) * 4;
-    if (kv->max_kv_len <= kEvictKeysInSmem) {
-        static std::atomic<int> done[kMaxDevices];
-        rc = allow_smem(kv_evict_select_kernel<true>, kEvictKeysInSmem * 4, done);
-        if (rc != VTX_OK) return rc;
-        rc = launch_pdl(kv_evict_select_kernel<true>, dim3((unsigned)e.items), dim3(kEvictThreads), (size_t)keys, st, a);
-    } else {
-        rc = launch_pdl(kv_evict_select_kernel<false>, dim3((unsigned)e.items), dim3(kEvictThreads), 0, st, a);
+    // Few moves: one kernel (1024 rows: 10.2 -> 8 us and one launch less); a
+    // (stream, head) is one CTA there, too little for many.  Not in place on
+    // kv_len, which the other heads' CTAs may not have read yet.
+    if (e.max_moves <= 512 && p->kv_len_out != kv->kv_len) {
+        if (unit == 16) return launch_evict_select<true, 16>(a, e.items, st);
+        return unit == 8 ? launch_evict_select<true, 8>(a, e.items, st) : launch_evict_select<true, 4>(a, e.items, st);
     }
+    rc = kv->max_kv_len <= kEvictKeysInSmem ? launch_evict_select<true, 0>(a, e.items, st)
+                                            : launch_evict_select<false, 0>(a, e.items, st);
     if (rc != VTX_OK) return rc;
     const dim3 grid((unsigned)(e.items * a.slices));
-    // rows of 256 or 128 (F16), 136 or 68 bytes (Q8_0: 8- and 4-byte aligned)
-    if (kv->k.type == VTX_TYPE_F16) return launch_pdl(kv_evict_move_kernel<uint4, 1>, grid, dim3(256), 0, st, a);
-    if (a.row_bytes % 8 == 0) return launch_pdl(kv_evict_move_kernel<uint2, 2>, grid, dim3(256), 0, st, a);
-    return launch_pdl(kv_evict_move_kernel<uint32_t, 2>, grid, dim3(256), 0, st, a);
+    if (unit == 16) return launch_pdl(kv_evict_move_kernel<16>, grid, dim3(256), 0, st, a);
+    return unit == 8 ? launch_pdl(kv_evict_move_kernel<8>, grid, dim3(256), 0, st, a)
+                     : launch_pdl(kv_evict_move_kernel<4>, grid, dim3(256), 0, st, a);
 }
 
 }  // extern "C"
