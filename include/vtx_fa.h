@@ -405,8 +405,8 @@ VTX_API int vtx_attn_out_proj(const vtx_out_proj_args *args, void *stream);
  * - n_tokens: tokens of the packed arrays (q_start's entries are cut there).
  *   max_new and max_kv_len bound every stream's new tokens and kv_len: they
  *   size grids and workspaces.  A stream above a bound is reported and what
- *   exceeds it is not served (vtx_flash_attn_paged serves a longer kv_len
- *   exactly).
+ *   exceeds it is not served (but see vtx_flash_attn_paged, which serves a
+ *   longer kv_len exactly in most cases).
  * page_table, kv_len and q_start are device memory, read by the kernels only:
  * a captured call may be replayed after they changed within the bounds. */
 typedef struct vtx_paged_kv {
@@ -460,8 +460,12 @@ VTX_API int vtx_kv_append_paged(const vtx_kv_append_paged_args *args, void *stre
  * additionally j > kv_len - n + i - W; rows of an evicted cache are not
  * positions, so a window does not fit there).  max_bias must be 0.
  * Hq / Hkv <= 16; base and strides of q and dst multiples of 16 bytes.
- * Rows at or behind kv_len may hold anything, NaN included.  P and V (and a
- * F32 q) are rounded to half, everything else is F32.
+ * Rows at or behind kv_len may hold anything, NaN included.
+ * Rounded to half: P, a F32 q, V of a Q8_0 cache where a stream brings more
+ * than 16 query rows (tokens * Hq / Hkv) per KV head, and K there too when
+ * max_kv_len >= 1024 (such caches are unpacked into the workspace, and a
+ * kv_len above max_kv_len is reported).  Everything else is F32.  A Q8_0
+ * scale of V above 1023 overflows.
  * workspace: 256-byte aligned, vtx_flash_attn_paged_workspace bytes (they
  * depend on kv's sizes and bounds and on n_head_q alone).  Zero it once before
  * its first call (cudaMemset): it holds arrival counters, which every call

@@ -75,11 +75,14 @@ def attend(c, scale=None, causal=True, window=0, softcap=0.0):
     return out, lse, a, err, tiny
 
 
-def attend_tolerance(ref, n_half):
+def attend_tolerance(ref, n_half, k_half_dim=0):
     """Elementwise bounds (out in f32, lse).  n_half operands of P V are rounded
     to half (2^-11 each: P, and V where it was Q8_0); an exponential's error is
-    below 2^-18, half P below 2^-14 loses at most 2^-25 of the row's largest."""
+    below 2^-18, half P below 2^-14 loses at most 2^-25 of the row's largest.
+    k_half_dim = D: K was rounded to half too, each product off by 2^-11."""
     out, lse, a, err, tiny = ref
+    if k_half_dim:
+        err = err + err / ((k_half_dim + 8) * 2.0 ** -24) * 2.0 ** -11
     fin = np.where(np.isfinite(lse), np.abs(lse), 0.0)
     return (a * (n_half * 2.0 ** -11 + 2 * err[..., None] + 2.0 ** -17) + tiny * 2.0 ** -25 + 1e-30,
             err + 2.0 ** -18 + fin * 2.0 ** -22)

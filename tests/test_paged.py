@@ -252,7 +252,9 @@ def device_kv(c, nhd=False, **kw):
 
 def check_attend(c, got, lse, ref, what=""):
     n_half = 2 if c["kv"] == "q8_0" else 1
-    tol, ltol = R.attend_tolerance(ref, n_half)
+    # a Q8_0 cache of 1024 rows or more is unpacked where a stream brings a chunk
+    long = c["kv"] == "q8_0" and max(c["len"]) >= 1024 and np.diff(c["start"]).max() * c["Hq"] // c["Hkv"] > 16
+    tol, ltol = R.attend_tolerance(ref, n_half, c["D"] if long else 0)
     f16 = got.dtype == torch.float16
     got = got.double().cpu().numpy()
     if f16:
@@ -294,6 +296,9 @@ ATTEND = [
     ("f16", [(300, 1300), (129, 129), (1, 2000)], 8, 2, 128, 64, {}),
     ("q8_0", [(200, 900), (129, 129)], 8, 2, 128, 32, {}),
     ("f16", [(64, 1999)], 4, 4, 64, 16, {}),
+    ("q8_0", [(90, 1500), (1, 700), (0, 30), (40, 40), (1, 3)], 8, 2, 128, 16, {}),
+    ("q8_0", [(90, 1500), (33, 1025)], 5, 5, 64, 32, dict(window=300)),
+    ("q8_0", [(300, 1200)], 15, 5, 128, 128, dict(softcap=10.0)),
     ("f16", [(33, 3000)], 8, 1, 64, 128, {}),
 ]
 
@@ -470,7 +475,8 @@ SCORE = [("f16", [(1, 1)], 8, 2, 128, 16, {}), ("f16", RAGGED, 8, 2, 128, 16, {}
          ("f16", RAGGED, 15, 5, 64, 32, dict(window=20)), ("q8_0", RAGGED, 16, 1, 64, 16, dict(softcap=5.0)),
          ("f16", RAGGED, 8, 2, 128, 16, dict(causal=False)), ("f16", [(100, 600), (1, 40)], 8, 2, 128, 16, dict(observe=32)),
          ("f16", [(1, 2000), (1, 300)], 32, 8, 128, 16, dict(decay=0.5)), ("q8_0", [(1, 700)], 32, 8, 128, 16, {}),
-         ("f16", [(300, 1500)], 8, 2, 128, 64, dict(decay=0.0)), ("f16", [(70, 300)], 4, 4, 64, 16, dict(window=100, observe=9))]
+         ("f16", [(300, 1500)], 8, 2, 128, 64, dict(decay=0.0)), ("q8_0", [(300, 1500), (2, 90)], 8, 2, 128, 64, {}),
+         ("q8_0", [(200, 400)], 15, 5, 64, 16, dict(window=50)), ("f16", [(60, 5000)], 32, 16, 64, 128, {}), ("f16", [(70, 300)], 4, 4, 64, 16, dict(window=100, observe=9))]
 
 
 @pytest.mark.gpu

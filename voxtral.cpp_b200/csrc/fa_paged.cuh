@@ -10,7 +10,8 @@
 // 16 rows, tiles of 32 keys in shared memory.  F16 rows as they are.  Q8_0: K
 // as its integers (exact halves) with each block's scale applied to that
 // block's f32 sum, so scores and lse carry no rounding of K; V as d * q rounded
-// to half, like P.
+// to half, like P.  It serves chunks over Q8_0 caches that are short; longer ones
+// are unpacked to F16 pages for the tensor-core kernel (paged_unpack_kernel).
 #pragma once
 #include <cuda_fp16.h>
 #include <cstdint>
@@ -69,6 +70,16 @@ __device__ __forceinline__ uint4 paged_load8(const char *row, int d, float s) {
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
+// Four int8 of a word as two pairs of halves, exactly.
+__device__ __forceinline__ void q8_halves(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));   // 1152
+    w ^= 0x80808080u;
+    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), off);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2 *>(&b), off);
+    lo = *reinterpret_cast<const uint32_t *>(&x);
+    hi = *reinterpret_cast<const uint32_t *>(&y);
+}
 // Writes two adjacent columns of an output row.
 __device__ __forceinline__ void paged_store2(const PagedAttnArgs &a, int tok, int head, int d, float x, float y) {
     char *p = a.dst + (long long)tok * a.d_nbt + (long long)head * a.d_nbh;
@@ -218,6 +229,60 @@ fa_paged_kernel(const PagedAttnArgs a)
             paged_store2(a, t, head, nb * 8 + 2 * (lane & 3), o[nb][2 * u] * inv, o[nb][2 * u + 1] * inv);
         if (a.lse && (lane & 3) == 0)
             a.lse[(long long)t * a.Hq + head] = l[u] == 0.f ? -INFINITY : (m[u] + log2f(l[u])) * kLn2;
+    }
+}
+
+// 8 values at 2-byte aligned shared memory as exact halves.
+__device__ __forceinline__ void q8_lds8(const char *p, uint32_t (&h)[4]) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(3));
+    const uint32_t sh = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 2) * 8;
+    const uint32_t x = w[0], y = w[1], z = sh ? w[2] : 0u;
+    q8_halves(__funnelshift_r(x, y, sh), h[0], h[1]);
+    q8_halves(__funnelshift_r(y, z, sh), h[2], h[3]);
+}
+
+// Copies the Q8_0 pages of the streams that bring more than a.min_rows query rows
+// into F16 pages of 256 rows in `out` (stream s, page p: page s * out.max_pages +
+// p), values d * q rounded to half: 272 bytes read and 512 written per row and
+// KV head, next to 4 * 128 flops per query row for each of those rows.
+// Grid (32-row ranges, Hkv, n_seq), 128 threads.
+template <int D>
+__global__ void __launch_bounds__(128)
+paged_unpack_kernel(const PagedAttnArgs a, const PagedView out)
+{
+    grid_dep_wait();
+    grid_dep_launch();
+    constexpr int ROW = D / 32 * 34;
+    __shared__ __align__(16) char raw[2 * 32 * ROW];
+    const int b = blockIdx.z, g = blockIdx.y, r0 = blockIdx.x * 32;
+    const PagedSeq s = paged_seq(a.kv, b);
+    const int end = min(s.len, out.max_pages << out.shift);
+    const int lo = a.window > 0 ? s.len - s.n_new - a.window + 1 : 0;
+    if (s.n_new * a.G <= a.min_rows || r0 >= end || r0 + 32 <= lo) return;
+    // groups of 16 rows are contiguous in a page
+    constexpr int CH = 16 * ROW / 16;
+    for (int i = threadIdx.x; i < 4 * CH; i += 128) {
+        const int grp = i / CH, r = r0 + (grp & 1) * 16;
+        if (r >= end || r + 16 <= lo) continue;
+        const char *src = (grp < 2 ? a.kv.k : a.kv.v) + paged_row(a.kv, b, r, g);
+        reinterpret_cast<uint4 *>(raw)[i] = reinterpret_cast<const uint4 *>(src)[i % CH];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * 32 * (D / 8); i += 128) {
+        const int sel = i / (32 * (D / 8)), r = i / (D / 8) % 32, c = i % (D / 8);
+        const int grp = r0 + (r & 16);
+        if (grp >= end || grp + 16 <= lo) continue;
+        const char *blk = raw + (sel * 32 + r) * ROW + (c >> 2) * 34;
+        const __half d = *reinterpret_cast<const __half *>(blk);
+        uint32_t h[4];
+        q8_lds8(blk + 2 + (c & 3) * 8, h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const __half2 x = __hmul2(*reinterpret_cast<const __half2 *>(&h[j]), __half2half2(d));
+            h[j] = *reinterpret_cast<const uint32_t *>(&x);
+        }
+        char *dst = (sel ? out.v : out.k) + paged_row(out, b, r0 + r, g) + c * 16;
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
     }
 }
 

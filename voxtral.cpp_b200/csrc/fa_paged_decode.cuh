@@ -66,16 +66,6 @@ __device__ __forceinline__ PagedCut paged_cut(const PagedSeq &s, int causal, int
     return c;
 }
 
-// Four int8 of a word as two pairs of halves, exactly.
-__device__ __forceinline__ void q8_halves(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));   // 1152
-    w ^= 0x80808080u;
-    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
-    const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), off);
-    const __half2 y = __hsub2(*reinterpret_cast<const __half2 *>(&b), off);
-    lo = *reinterpret_cast<const uint32_t *>(&x);
-    hi = *reinterpret_cast<const uint32_t *>(&y);
-}
 // The word at a byte offset of 2 mod 4 (HALF) or 0 mod 4 in shared memory.
 template <bool HALF>
 __device__ __forceinline__ uint32_t lds_word(const char *p) {

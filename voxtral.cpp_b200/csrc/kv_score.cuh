@@ -9,9 +9,9 @@
 // weights to one register per key; a shuffle over the row lanes at the end
 // gives the sums in the same order on every run (no atomics).
 // Three kernels.  Few query rows per KV head (a decode step): bound by reading K
-// once, kv_score_stream_kernel.  Many rows, F16: bound by the exponentials (one
-// per query row and key), kv_score_sm100_kernel.  Many rows over a Q8_0 cache
-// or with an F32 q: kv_score_kernel, the description above.
+// once, kv_score_stream_kernel.  Many rows: bound by the exponentials (one per
+// query row and key), kv_score_sm100_kernel.  Many rows with an F32 q, which TMA
+// cannot round: kv_score_kernel, the description above.
 #pragma once
 #include <cuda_fp16.h>
 #include <cstdint>

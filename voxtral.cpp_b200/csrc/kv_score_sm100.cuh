@@ -1,5 +1,5 @@
 // kv_score_sm100.cuh — accumulated attention weight of many query rows on the
-// tensor core (F16 cache and q): kv_score.cuh's sum with the product turned
+// tensor core (F16 q): kv_score.cuh's sum with the product turned
 // round, S^T = K Q^T, so that a key is a TMEM lane and its thread adds up its
 // own row of weights; nothing crosses threads.
 //
@@ -16,6 +16,10 @@
 // not kept.
 // A column's -lse and last visible row are staged; (-inf, -1) makes a column
 // count nothing (rows past the tokens, or T * G < 128).
+// Q8_0: a K tile is made once by the threads, as two halves per value, d * q
+// rounded and what that lost; two products per tile then carry about 22 bits of K
+// (one rounded half would move a weight by 2^-12), and the tensor core has the
+// time, since the exponentials bound the kernel.
 // Key rows that do not exist or that nobody sees only affect their own lane.
 #pragma once
 #include <cuda.h>
@@ -28,10 +32,11 @@
 
 namespace vtx {
 
-template <int D, int NT> struct ScoreTileCfg {
+template <int D, int KVT, int NT> struct ScoreTileCfg {
     static constexpr int SUB = D / 64, TILE = 128 * D * 2, STAGES = 2;
     static constexpr int PER = 4 / NT;             // warpgroups and TMEM buffers per key tile
-    static constexpr int K_OFF = 0, Q_OFF = NT * TILE;
+    static constexpr int K_TILES = KVT == 1 ? NT : 2 * NT;             // Q8_0: high and low parts
+    static constexpr int K_OFF = 0, Q_OFF = K_TILES * TILE;
     static constexpr int LSE_OFF = Q_OFF + STAGES * TILE;              // per stage: -lse, last visible row
     static constexpr int LSTAGES = 4;
     static constexpr int SUM_OFF = LSE_OFF + LSTAGES * 1024, BAR_OFF = SUM_OFF + 1024;
@@ -41,12 +46,12 @@ template <int D, int NT> struct ScoreTileCfg {
 };
 
 // Grid (key ranges of 128 NT, Hkv, n_seq).
-template <int D, int NT, bool UF>
-__global__ void __launch_bounds__(ScoreTileCfg<D, NT>::NTHREADS, 1)
+template <int D, int KVT, int NT, bool UF>
+__global__ void __launch_bounds__(ScoreTileCfg<D, KVT, NT>::NTHREADS, 1)
 kv_score_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmQ,
                       const PagedScoreArgs a, int T)
 {
-    using C = ScoreTileCfg<D, NT>;
+    using C = ScoreTileCfg<D, KVT, NT>;
     extern __shared__ __align__(1024) char smem_raw[];
     char *smem = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *k_full = reinterpret_cast<uint64_t *>(smem + C::BAR_OFF);
@@ -62,7 +67,7 @@ kv_score_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int b = blockIdx.z, g = blockIdx.y;
     if (tid == 0) {
-        mbar_init(k_full, 1);
+        mbar_init(k_full, KVT == 1 ? 1 : 16);      // the TMA lane, or the warps that make K
         mbar_init(mma_done, 1);
         for (int i = 0; i < C::STAGES; ++i) {
             mbar_init(&q_full[i], 1);
@@ -119,6 +124,32 @@ kv_score_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const long long e = ((long long)b * a.kv.Hkv + g) * a.row_cap + key;
         const float old = half == 0 && key < limit && a.decay != 0.f ? a.decay * a.score[e] : 0.f;
+        if constexpr (KVT == 8) {
+            if (n_iter > 0) {
+                for (int i = tid; i < NT * 128 * (D / 8); i += 512) {
+                    const int r = i / (D / 8), c = i % (D / 8), ky = k0 + r;
+                    if (ky >= limit || ky < lo_any) continue;           // affects its own lane only
+                    const char *row = a.kv.k + paged_row(a.kv, b, ky, g);
+                    const float d = q8_scale(row, c * 8);
+                    const unsigned short *w = reinterpret_cast<const unsigned short *>(row + (c >> 2) * 34 + 2 + (c & 3) * 8);
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float x = d * (float)(int8_t)(w[j] & 0xff), y = d * (float)(int8_t)(w[j] >> 8);
+                        hi[j] = pack_half2(x, y);
+                        const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi[j]));
+                        lo[j] = pack_half2(x - h.x, y - h.y);
+                    }
+                    char *dst = smem + C::K_OFF + (r >> 7) * C::TILE + (c >> 3) * 16384 + (r & 127) * 128 +
+                                (((c & 7) ^ (r & 7)) << 4);
+                    *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4 *>(dst + NT * C::TILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(k_full);
+            }
+        }
         const float cx = a.scale * kLog2e;
         const unsigned reach = a.window > 0 ? (unsigned)a.window : 0x80000000u;
         float sum = 0.f;
@@ -186,28 +217,30 @@ kv_score_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     } else if (warp == C::TMA_WARP) {
         // =================== TMA: the K tiles, then Q tile by tile =========
         if (n_iter > 0) {
-            // boxes of a half-width tile row range: 16 a tile at most, two tiles a round
-            const int rows_box = min(128, 1 << a.kv.shift), per = 128 / rows_box * C::SUB;
-            unsigned need = 0;                     // bit u: this lane's box of round u is loaded
-            int n = 0;
+            if constexpr (KVT == 1) {
+                // boxes of a half-width tile row range: 16 a tile at most, two tiles a round
+                const int rows_box = min(128, 1 << a.kv.shift), per = 128 / rows_box * C::SUB;
+                unsigned need = 0;                     // bit u: this lane's box of round u is loaded
+                int n = 0;
 #pragma unroll
-            for (int u = 0; u < NT / 2; ++u) {
-                const int j = lane / per, y = k0 + (2 * u + j) * 128 + (lane % per) / C::SUB * rows_box;
-                const bool on = j < 2 && y < limit && y + rows_box > lo_any;
-                n += __popc(__ballot_sync(0xffffffffu, on));
-                need |= (unsigned)on << u;
-            }
-            if (lane == 0) mbar_arrive_expect_tx(k_full, (uint32_t)(n * rows_box * 128));
-            __syncwarp();
+                for (int u = 0; u < NT / 2; ++u) {
+                    const int j = lane / per, y = k0 + (2 * u + j) * 128 + (lane % per) / C::SUB * rows_box;
+                    const bool on = j < 2 && y < limit && y + rows_box > lo_any;
+                    n += __popc(__ballot_sync(0xffffffffu, on));
+                    need |= (unsigned)on << u;
+                }
+                if (lane == 0) mbar_arrive_expect_tx(k_full, (uint32_t)(n * rows_box * 128));
+                __syncwarp();
 #pragma unroll
-            for (int u = 0; u < NT / 2; ++u) {
-                const int j = 2 * u + lane / per, r = (lane % per) / C::SUB * rows_box, sub = lane % C::SUB;
-                if ((need >> u) & 1u)
-                    tma_load_4d(smem + C::K_OFF + j * C::TILE + sub * 16384 + r * 128, &tmK, k_full, sub * 64,
-                                (k0 + j * 128 + r) & ((1 << a.kv.shift) - 1), g,
-                                max(paged_page(a.kv, b, k0 + j * 128 + r), 0));
+                for (int u = 0; u < NT / 2; ++u) {
+                    const int j = 2 * u + lane / per, r = (lane % per) / C::SUB * rows_box, sub = lane % C::SUB;
+                    if ((need >> u) & 1u)
+                        tma_load_4d(smem + C::K_OFF + j * C::TILE + sub * 16384 + r * 128, &tmK, k_full, sub * 64,
+                                    (k0 + j * 128 + r) & ((1 << a.kv.shift) - 1), g,
+                                    max(paged_page(a.kv, b, k0 + j * 128 + r), 0));
+                }
+                __syncwarp();
             }
-            __syncwarp();
             int issued = 0;
             if (lane == 0) {
                 for (int it = 0; it < n_iter; ++it) {
@@ -284,6 +317,9 @@ kv_score_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
                     const uint32_t ko = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
                     mma_f16_ss_w(lead, tmem + buf * 128, desc64(lo_k + t * T16 + ko, HI), desc64(lo_q + st * T16 + ko, HI),
                                  IDESC, kk > 0);
+                    if constexpr (KVT == 8)
+                        mma_f16_ss_w(lead, tmem + buf * 128, desc64(lo_k + (NT + t) * T16 + ko, HI),
+                                     desc64(lo_q + st * T16 + ko, HI), IDESC, 1);
                 }
                 mma_commit_w(lead, &s_full[buf]);
             }

@@ -17,7 +17,7 @@ enum { VTX_KERR_PAGE = 40, VTX_KERR_BOUND = 41 };
 struct PagedView {
     char *k, *v;
     long long nb1, nb2, nb3;               // row, head and page strides (bytes), the same for k and v
-    const int *table, *kv_len, *q_start;
+    const int *table, *kv_len, *q_start;   // table NULL: stream s owns pages s * max_pages ...
     int n_seq, n_tokens, max_new, max_kv;
     int max_pages, n_pages, shift;         // page_size = 1 << shift
     int Hkv;
@@ -48,7 +48,8 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedView &kv, int b) {
 // The page of row `row` of stream b (row < its len); a table entry outside the
 // pool is reported and answered with -1.
 __device__ __forceinline__ int paged_page(const PagedView &kv, int b, int row) {
-    const int p = kv.table[(long long)b * kv.max_pages + (row >> kv.shift)];
+    const long long i = (long long)b * kv.max_pages + (row >> kv.shift);
+    const int p = kv.table ? kv.table[i] : (int)i;
     if ((unsigned)p < (unsigned)kv.n_pages) return p;
     paged_report(kv, VTX_KERR_PAGE);
     return -1;

@@ -180,19 +180,32 @@ int launch_attn(const PagedAttnArgs &a, cudaStream_t st) {
                       dim3(128), 0, st, a);
 }
 
-// The tensor-core kernel: F16 caches, when a stream may bring more rows than
-// the streaming kernel takes.
+// The tensor-core kernel, when a stream may bring more rows than the streaming
+// kernel takes: F16 caches, and Q8_0 caches of kUnpackFrom rows or more, whose
+// pages it reads as an F16 copy in the workspace.  K is rounded to half there,
+// which moves a row's lse by about 2^-12 / sqrt(visible keys), hence the bound; and
+// below it mma.sync on the pages is as fast.  Copies above kUnpackBytes: no.
+constexpr int kUnpackFrom = 1024, kUnpackPage = 256;
+constexpr size_t kUnpackBytes = size_t(2) << 30;
+
 struct TilePlan {
     bool use;
     PagedTile tile;
-    size_t o_bytes, bytes;
+    int unpack;               // pages of kUnpackPage rows per stream, 0: none
+    size_t o_bytes, u_bytes, bytes;   // partial O, one unpacked pool, all
 };
 
 TilePlan plan_tile(const vtx_paged_kv *p, int G, int Hq, int min_rows, int sms) {
     TilePlan t{};
-    t.use = p->k.type == VTX_TYPE_F16 && p->max_new * (long long)G > min_rows && p->n_seq > 0;
-    if (!t.use) return t;
     const int Hkv = (int)p->k.ne[2], D = (int)p->k.ne[0];
+    if (p->k.type == VTX_TYPE_Q8_0 && p->max_kv_len >= kUnpackFrom) {
+        t.unpack = (p->max_kv_len + kUnpackPage - 1) / kUnpackPage;
+        t.u_bytes = (size_t)p->n_seq * t.unpack * kUnpackPage * Hkv * D * 2;
+        if (2 * t.u_bytes > kUnpackBytes) t.unpack = 0;
+    }
+    t.use = (p->k.type == VTX_TYPE_F16 || t.unpack) && p->max_new * (long long)G > min_rows && p->n_seq > 0;
+    if (!t.use || !t.unpack) t.u_bytes = 0;
+    if (!t.use) return t;
     t.tile.T = 128 / G;
     const long long pair = 2 * t.tile.T;
     // streams with more than min_rows rows, and what rounding each up to whole groups adds
@@ -234,20 +247,39 @@ TilePlan plan_tile(const vtx_paged_kv *p, int G, int Hq, int min_rows, int sms) 
         t.o_bytes = align_up(rows * D * 4, 256);
         t.bytes = t.o_bytes + align_up(rows * 8, 256);
     }
+    t.bytes += 2 * t.u_bytes;                                // pages are multiples of 256 bytes
     return t;
 }
 
-// Map of a pool: (dim, row, head, page), boxes of 64 dims x min(page, 128) rows.
-int encode_pool_map(CUtensorMap *m, const vtx_tensor &t) {
+// The F16 copy of a Q8_0 cache, at the end of the tile plan's workspace.
+PagedView unpacked_view(const PagedView &kv, const TilePlan &t, int D, char *ws) {
+    PagedView u = kv;
+    u.k = ws + t.bytes - 2 * t.u_bytes;
+    u.v = u.k + t.u_bytes;
+    u.nb1 = D * 2; u.nb2 = (long long)kUnpackPage * D * 2; u.nb3 = u.nb2 * kv.Hkv;
+    u.table = nullptr;
+    u.max_pages = t.unpack; u.n_pages = kv.n_seq * t.unpack;
+    u.shift = 8;
+    return u;
+}
+
+template <int D>
+int launch_unpack(const PagedAttnArgs &a, const PagedView &out, cudaStream_t st) {
+    return launch_pdl(paged_unpack_kernel<D>, dim3((unsigned)((a.kv.max_kv + 31) / 32), (unsigned)a.kv.Hkv,
+                                                   (unsigned)a.kv.n_seq), dim3(128), 0, st, a, out);
+}
+
+// Map of an F16 pool: (dim, row, head, page), boxes of 64 dims x min(page, 128) rows.
+int encode_pool_map(CUtensorMap *m, const PagedView &kv, void *pool, int D) {
     PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
     if (!enc) return VTX_ERR_CUDA;
-    const size_t s2 = t.ne[2] > 1 ? t.nb[2] : t.nb[1] * (size_t)t.ne[1];
-    const size_t s3 = t.ne[3] > 1 ? t.nb[3] : s2 * (size_t)t.ne[2];
-    cuuint64_t dims[4] = {(cuuint64_t)t.ne[0], (cuuint64_t)t.ne[1], (cuuint64_t)t.ne[2], (cuuint64_t)t.ne[3]};
-    cuuint64_t strides[3] = {(cuuint64_t)t.nb[1], (cuuint64_t)s2, (cuuint64_t)s3};
-    cuuint32_t box[4] = {64, (cuuint32_t)std::min<int64_t>(t.ne[1], 128), 1, 1};
+    const long long page = 1LL << kv.shift;                   // extent-1 axes: any legal stride
+    const long long s2 = kv.Hkv > 1 ? kv.nb2 : kv.nb1 * page, s3 = kv.n_pages > 1 ? kv.nb3 : s2 * kv.Hkv;
+    cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)page, (cuuint64_t)kv.Hkv, (cuuint64_t)kv.n_pages};
+    cuuint64_t strides[3] = {(cuuint64_t)kv.nb1, (cuuint64_t)s2, (cuuint64_t)s3};
+    cuuint32_t box[4] = {64, (cuuint32_t)std::min<long long>(page, 128), 1, 1};
     cuuint32_t estr[4] = {1, 1, 1, 1};
-    return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, t.data, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, pool, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? VTX_OK : VTX_ERR_STRIDE;
 }
@@ -318,25 +350,26 @@ int launch_score_stream(const PagedScoreArgs &a, int sms, cudaStream_t st) {
                              : launch_score_stream_t<D, KVT, false>(a, sp, st);
 }
 
-template <int D, int NT, bool UF>
+template <int D, int KVT, int NT, bool UF>
 int launch_score_tile_n(const CUtensorMap (&m)[2], const PagedScoreArgs &a, int T, cudaStream_t st) {
-    using C = ScoreTileCfg<D, NT>;
+    using C = ScoreTileCfg<D, KVT, NT>;
     static std::atomic<int> done[kMaxDevices];
-    int rc = allow_smem(kv_score_sm100_kernel<D, NT, UF>, C::SMEM, done);
+    int rc = allow_smem(kv_score_sm100_kernel<D, KVT, NT, UF>, C::SMEM, done);
     if (rc != VTX_OK) return rc;
-    return launch_pdl(kv_score_sm100_kernel<D, NT, UF>,
+    return launch_pdl(kv_score_sm100_kernel<D, KVT, NT, UF>,
                       dim3((unsigned)((a.kv.max_kv + 128 * NT - 1) / (128 * NT)), (unsigned)a.kv.Hkv,
                            (unsigned)a.kv.n_seq),
                       dim3(C::NTHREADS), C::SMEM, st, m[0], m[1], a, T);
 }
 
-// Four key tiles per CTA halve the reads of Q from L2, two spread over more
+// F16: four key tiles per CTA halve the reads of Q from L2, two spread over more
 // SMs: four once they fill the GPU (500 tokens: 16000 keys 102 us with four, 116
-// with two; 4000 keys 51 and 31 us).
+// with two; 4000 keys 51 and 31 us).  Q8_0: two (shared memory).
 template <int D, bool UF>
-int launch_score_tile(const CUtensorMap (&m)[2], const PagedScoreArgs &a, int T, int sms, cudaStream_t st) {
+int launch_score_tile(const CUtensorMap (&m)[2], const PagedScoreArgs &a, bool f16, int T, int sms, cudaStream_t st) {
     const long long ctas4 = ((long long)a.kv.max_kv + 511) / 512 * a.kv.Hkv * a.kv.n_seq;
-    return ctas4 >= sms ? launch_score_tile_n<D, 4, UF>(m, a, T, st) : launch_score_tile_n<D, 2, UF>(m, a, T, st);
+    if (!f16) return launch_score_tile_n<D, 8, 2, UF>(m, a, T, st);
+    return ctas4 >= sms ? launch_score_tile_n<D, 1, 4, UF>(m, a, T, st) : launch_score_tile_n<D, 1, 2, UF>(m, a, T, st);
 }
 
 struct EvictPlan {
@@ -463,20 +496,27 @@ int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, si
     const bool f16 = kv->k.type == VTX_TYPE_F16, d64 = kv->k.ne[0] == 64;
     // chunks first (their CTAs are long), few-token streams beside them
     a.min_rows = dp.use ? dp.rows : 0;
+    PagedAttnArgs ta = a;                                     // what the tensor-core kernel reads
     if (tp.use) {
         char *ws = static_cast<char *>(workspace) + dp.bytes;
         tp.tile.part_o = reinterpret_cast<float *>(ws);
         tp.tile.part_ml = reinterpret_cast<float *>(ws + tp.o_bytes);
+        const int D = (int)kv->k.ne[0];
+        if (tp.unpack) {
+            ta.kv = unpacked_view(a.kv, tp, D, ws);
+            rc = d64 ? launch_unpack<64>(a, ta.kv, st) : launch_unpack<128>(a, ta.kv, st);
+            if (rc != VTX_OK) return rc;
+        }
         CUtensorMap m[3];
-        rc = encode_pool_map(&m[0], kv->k);
-        if (rc == VTX_OK) rc = encode_pool_map(&m[1], kv->v);
+        rc = encode_pool_map(&m[0], ta.kv, ta.kv.k, D);
+        if (rc == VTX_OK) rc = encode_pool_map(&m[1], ta.kv, ta.kv.v, D);
         m[2] = m[0];                                          // an F32 q is read by the softmax warps
         if (rc == VTX_OK && a.q_f16) rc = encode_paged_q_map(&m[2], q, a.G, tp.tile.T);
         if (rc != VTX_OK) return rc;
         // tanh, or a scale that the row maximum cannot carry: logits formed first
         const bool uf = a.softcap != 0.0f || !(a.scale > 0.0f);
-        if (d64) rc = uf ? launch_tile<64, true>(m, a, tp.tile, st) : launch_tile<64, false>(m, a, tp.tile, st);
-        else rc = uf ? launch_tile<128, true>(m, a, tp.tile, st) : launch_tile<128, false>(m, a, tp.tile, st);
+        if (d64) rc = uf ? launch_tile<64, true>(m, ta, tp.tile, st) : launch_tile<64, false>(m, ta, tp.tile, st);
+        else rc = uf ? launch_tile<128, true>(m, ta, tp.tile, st) : launch_tile<128, false>(m, ta, tp.tile, st);
     } else if (kv->max_new * (long long)a.G > a.min_rows) {
         rc = d64 ? launch_attn<64, 8>(a, st) : launch_attn<128, 8>(a, st);
     }
@@ -492,7 +532,7 @@ int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, si
         if (rc != VTX_OK) return rc;
     }
     if (!tp.use || tp.tile.n_splits == 1) return VTX_OK;
-    return d64 ? launch_tile_combine<64>(a, tp.tile, st) : launch_tile_combine<128>(a, tp.tile, st);
+    return d64 ? launch_tile_combine<64>(ta, tp.tile, st) : launch_tile_combine<128>(ta, tp.tile, st);
 }
 
 int vtx_kv_score_paged(const vtx_kv_score_paged_args *p, void *stream) {
@@ -526,15 +566,18 @@ int vtx_kv_score_paged(const vtx_kv_score_paged_args *p, void *stream) {
         if (d64) return f16 ? launch_score_stream<64, 1>(a, ds->sms, st) : launch_score_stream<64, 8>(a, ds->sms, st);
         return f16 ? launch_score_stream<128, 1>(a, ds->sms, st) : launch_score_stream<128, 8>(a, ds->sms, st);
     }
-    if (f16 && a.q_f16) {
+    if (a.q_f16) {
         CUtensorMap m[2];
         const int T = 128 / a.G;
-        rc = encode_pool_map(&m[0], kv->k);
-        if (rc == VTX_OK) rc = encode_paged_q_map(&m[1], p->q, a.G, T);
+        rc = encode_paged_q_map(&m[1], p->q, a.G, T);
+        m[0] = m[1];                                          // Q8_0 pages are read by the threads
+        if (rc == VTX_OK && f16) rc = encode_pool_map(&m[0], a.kv, a.kv.k, (int)kv->k.ne[0]);
         if (rc != VTX_OK) return rc;
         if (a.softcap != 0.0f)
-            return d64 ? launch_score_tile<64, true>(m, a, T, ds->sms, st) : launch_score_tile<128, true>(m, a, T, ds->sms, st);
-        return d64 ? launch_score_tile<64, false>(m, a, T, ds->sms, st) : launch_score_tile<128, false>(m, a, T, ds->sms, st);
+            return d64 ? launch_score_tile<64, true>(m, a, f16, T, ds->sms, st)
+                       : launch_score_tile<128, true>(m, a, f16, T, ds->sms, st);
+        return d64 ? launch_score_tile<64, false>(m, a, f16, T, ds->sms, st)
+                   : launch_score_tile<128, false>(m, a, f16, T, ds->sms, st);
     }
     if (d64) return f16 ? launch_score<64, 1>(a, st) : launch_score<64, 8>(a, st);
     return f16 ? launch_score<128, 1>(a, st) : launch_score<128, 8>(a, st);
