@@ -3,9 +3,9 @@
 // src/voxtral.cpp:1802 for ragged batches, bound by the tensor core and the
 // exponentials (4 D flops and one exp per query row and visible key).
 //
-// A CTA owns a group of two 128-row Q tiles of one stream and KV head (row =
-// token * G + head of the group, T = 128 / G tokens a tile) and one split of
-// its key tiles of 128.  Two softmax warpgroups, one per Q tile (a thread per
+// A CTA owns a group of two 128-row Q tiles (one, when pairs would leave SMs idle)
+// of one stream and KV head (row = token * G + head of the group, T = 128 / G
+// tokens a tile) and one split of its key tiles of 128.  Two softmax warpgroups, one per Q tile (a thread per
 // row = TMEM lane), take turns on the tensor core; a third warpgroup holds the
 // TMA and the MMA warp and gives its registers away (setmaxnreg).  Per key tile
 // and Q tile: S = Q K^T into TMEM, P = 2^(x - m) over S's first half columns,
@@ -25,7 +25,9 @@
 // P, so lse carries neither P's rounding to half nor more than that error.
 //
 // Splits: with few groups the key tiles of a group are cut into up to n_splits
-// ranges; their (m, l, O) are merged by fa_paged_tile_combine_kernel.
+// ranges; their (m, l, O) are merged by fa_paged_tile_combine_kernel.  With one
+// stream the first `whole` (group, head) items, full waves of CTAs, are not cut:
+// only the rest is, so that the last wave is full too.
 #pragma once
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -39,8 +41,10 @@ namespace vtx {
 
 struct PagedTile {
     int T;                    // tokens per Q tile: 128 / G
+    int tokens;               // tokens per group: 2 T, or T when pairs would leave SMs idle
     int groups;               // bound on the groups of all streams
     int n_splits, min_tiles;  // splits of a group's key tiles at most, key tiles per split at least
+    int whole;                // (group, head) items that are not split, the first ones
     float *part_o, *part_ml;  // [n_splits][n_tokens][Hq][D], ... [2] (m, l)
 };
 
@@ -77,9 +81,9 @@ __device__ __forceinline__ void paged_exp2_pair(float &a, float &b) {
     b = __int_as_float(__float_as_int(pb) + (__float_as_int(tb) << 23));
 }
 
-// Groups (pairs of Q tiles) of a stream with n_new tokens.
+// Groups (pairs of Q tiles, or single ones) of a stream with n_new tokens.
 __device__ __forceinline__ int paged_groups(int n_new, const PagedAttnArgs &a, const PagedTile &tl) {
-    return n_new * a.G > a.min_rows ? (n_new + 2 * tl.T - 1) / (2 * tl.T) : 0;
+    return n_new * a.G > a.min_rows ? (n_new + tl.tokens - 1) / tl.tokens : 0;
 }
 
 // Key tiles [j0, j1) of a group whose first token is tok0, and their splits.
@@ -88,14 +92,15 @@ struct PagedRange {
     int j0, j1, per, n;
 };
 __device__ __forceinline__ PagedRange paged_range(const PagedSeq &s, int tok0, const PagedAttnArgs &a,
-                                                  const PagedTile &tl) {
+                                                  const PagedTile &tl, bool cut) {
     PagedRange r;
-    const int off = s.len - s.n_new, last = min(s.n_new, tok0 + 2 * tl.T) - 1;
+    const int off = s.len - s.n_new, last = min(s.n_new, tok0 + tl.tokens) - 1;
     r.hi = a.causal ? off + last : s.len - 1;
     r.lo = a.window > 0 ? max(0, off + tok0 - a.window + 1) : 0;
     r.j0 = r.hi >= r.lo ? r.lo >> 7 : 0;
     r.j1 = r.hi >= r.lo ? (r.hi >> 7) + 1 : 0;
-    r.per = max(tl.min_tiles, (r.j1 - r.j0 + tl.n_splits - 1) / tl.n_splits);
+    const int most = cut ? tl.n_splits : 1;
+    r.per = max(tl.min_tiles, (r.j1 - r.j0 + most - 1) / most);
     r.n = max(1, (r.j1 - r.j0 + r.per - 1) / r.per);
     return r;
 }
@@ -119,8 +124,11 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     int *found = reinterpret_cast<int *>(tmem_slot + 2);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int g = blockIdx.x % a.kv.Hkv;
-    const int split = (blockIdx.x / a.kv.Hkv) % tl.n_splits;
+    // item = group * Hkv + head; behind the whole ones n_splits CTAs each
+    const int behind = (int)blockIdx.x - tl.whole;
+    const int item = behind < 0 ? (int)blockIdx.x : tl.whole + behind / tl.n_splits;
+    const int split = behind < 0 ? 0 : behind % tl.n_splits;
+    const int g = item % a.kv.Hkv;
 
     if (tid == 32) {
         mbar_init(q_full, a.q_f16 ? 1 : 8);        // the TMA lane, or one arrival per softmax warp
@@ -144,7 +152,7 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     grid_dep_wait();
     grid_dep_launch();
     if (warp == 0) {                               // the stream and group of this CTA
-        const int want = blockIdx.x / (a.kv.Hkv * tl.n_splits);
+        const int want = item / a.kv.Hkv;
         int base = 0, b = -1, grp = 0;
         for (int i0 = 0; i0 < a.kv.n_seq && b < 0; i0 += 32) {
             const int i = i0 + lane;
@@ -178,12 +186,12 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
         if (tid == 0) paged_report(a.kv, VTX_KERR_BOUND);
     }
     const int n_serve = min(s.n_new, a.kv.max_new);
-    const int tok0 = found[1] * 2 * tl.T;
-    const PagedRange rg = paged_range(s, tok0, a, tl);
+    const int tok0 = found[1] * tl.tokens;
+    const PagedRange rg = paged_range(s, tok0, a, tl, behind >= 0);
     if (split >= rg.n) return;
     const int jb = rg.j0 + split * rg.per;
     const int n_iter = max(0, min(jb + rg.per, rg.j1) - jb);
-    const bool two = tok0 + tl.T < n_serve;        // the second Q tile holds tokens
+    const bool two = tl.tokens > tl.T && tok0 + tl.T < n_serve;        // the second Q tile holds tokens
 
     if (warp == C::MMA_WARP) {
         tmem_alloc(tmem_slot, 512);
@@ -512,53 +520,71 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     }
 }
 
-// Merges the splits: grid (n_tokens, ceil(Hq / 8)), a warp per query head, a lane
-// per 4 dims; at most 32 splits, whose (m, l) the lanes read at once.
+// Merges the splits: grid (n_tokens, ceil(Hq / 32)), a warp per four query heads, a
+// lane per 4 dims; at most 32 splits, whose (m, l) the lanes read at once.
 template <int D>
 __global__ void __launch_bounds__(256)
 fa_paged_tile_combine_kernel(const PagedAttnArgs a, const PagedTile tl)
 {
     grid_dep_wait();
     grid_dep_launch();
+    constexpr int H = 4;
     const int t = blockIdx.x;
     const int b = paged_find(a.kv, t);
     if (b >= a.kv.n_seq) return;
     const PagedSeq s = paged_seq(a.kv, b);
     const int tok = t - s.q0, served = min(s.n_new, a.kv.max_new);
     if (tok < 0 || tok >= served || paged_groups(served, a, tl) == 0) return;
-    const int n = paged_range(s, tok / (2 * tl.T) * 2 * tl.T, a, tl).n;
-    const int lane = threadIdx.x & 31, d = lane * 4, h = blockIdx.y * 8 + (threadIdx.x >> 5);
-    if (n == 1 || h >= a.Hq) return;
-    const long long step = (long long)a.kv.n_tokens * a.Hq, row = (long long)t * a.Hq + h;
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (lane < n) ml = reinterpret_cast<const float2 *>(tl.part_ml)[lane * step + row];
-    float top = ml.x;
+    const int lane = threadIdx.x & 31, d = lane * 4, h0 = blockIdx.y * 32 + (threadIdx.x >> 5) * H;
+    const int grp = tok / tl.tokens, n = paged_range(s, grp * tl.tokens, a, tl, true).n;
+    if (n == 1 || h0 >= a.Hq) return;
+    const long long step = (long long)a.kv.n_tokens * a.Hq, row = (long long)t * a.Hq + h0;
+    float2 ml[H];
+    bool on[H];                                    // heads whose item was cut
 #pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
-    float l = f * ml.y;
+    for (int j = 0; j < H; ++j) {
+        // whole items exist with one stream only, whose last group comes first
+        on[j] = h0 + j < a.Hq && (paged_groups(served, a, tl) - 1 - grp) * a.kv.Hkv + (h0 + j) / a.G >= tl.whole;
+        ml[j] = make_float2(-INFINITY, 0.f);
+        if (on[j] && lane < n) ml[j] = reinterpret_cast<const float2 *>(tl.part_ml)[lane * step + row + j];
+    }
+    float top[H], f[H], l[H];
+    float4 acc[H];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 < n; i0 += 4) {
-        float4 v[4];
+    for (int j = 0; j < H; ++j) {
+        top[j] = ml[j].x;
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            v[u] = i0 + u < n && d < D ? *reinterpret_cast<const float4 *>(tl.part_o + ((i0 + u) * step + row) * D + d)
-                                       : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int o = 16; o; o >>= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
+        f[j] = ml[j].x == -INFINITY ? 0.f : ex2(ml[j].x - top[j]);
+        l[j] = f[j] * ml[j].y;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const float w = __shfl_sync(0xffffffffu, f, (i0 + u) & 31);
-            acc.x = fmaf(w, v[u].x, acc.x); acc.y = fmaf(w, v[u].y, acc.y);
-            acc.z = fmaf(w, v[u].z, acc.z); acc.w = fmaf(w, v[u].w, acc.w);
+        for (int o = 16; o; o >>= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], o);
+        acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll 2
+    for (int i = 0; i < n; ++i) {
+        float4 v[H];
+#pragma unroll
+        for (int j = 0; j < H; ++j)
+            v[j] = on[j] && d < D ? *reinterpret_cast<const float4 *>(tl.part_o + (i * step + row + j) * D + d)
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+            const float w = __shfl_sync(0xffffffffu, f[j], i);
+            acc[j].x = fmaf(w, v[j].x, acc[j].x); acc[j].y = fmaf(w, v[j].y, acc[j].y);
+            acc[j].z = fmaf(w, v[j].z, acc[j].z); acc[j].w = fmaf(w, v[j].w, acc[j].w);
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (d < D) {
-        paged_store2(a, t, h, d, acc.x * inv, acc.y * inv);
-        paged_store2(a, t, h, d + 2, acc.z * inv, acc.w * inv);
+#pragma unroll
+    for (int j = 0; j < H; ++j) {
+        if (!on[j]) continue;
+        const float inv = l[j] == 0.f ? 0.f : 1.f / l[j];
+        if (d < D) {
+            paged_store2(a, t, h0 + j, d, acc[j].x * inv, acc[j].y * inv);
+            paged_store2(a, t, h0 + j, d + 2, acc[j].z * inv, acc[j].w * inv);
+        }
+        if (a.lse && lane == 0) a.lse[row + j] = l[j] == 0.f ? -INFINITY : (top[j] + log2f(l[j])) * kLn2;
     }
-    if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
 }
 
 }  // namespace vtx

@@ -126,9 +126,9 @@ struct DecodePlan {
     size_t c_bytes, o_bytes, bytes;   // counters, partial O, all
 };
 
-// Splits: about two waves of two CTAs per SM over (streams x KV heads), at
-// most 128 tiles (2048 keys) each so that ragged lengths spread evenly, and at
-// least one tile per warp.
+// Splits over (streams x KV heads): one wave of three CTAs per SM for one
+// stream, two for several (ragged lengths spread more evenly), at most 128 tiles
+// (2048 keys) each, and at least one tile per warp.
 DecodePlan plan_decode(const vtx_paged_kv *p, int G, int sms) {
     DecodePlan d{};
     // the only stream may bring more tokens than fit: then all go one way
@@ -140,7 +140,8 @@ DecodePlan plan_decode(const vtx_paged_kv *p, int G, int sms) {
     d.rows = p->max_new * (long long)G <= 8 ? 8 : 16;
     const long long base = (long long)p->n_seq * p->k.ne[2];
     const int tiles = std::max(1, (p->max_kv_len + 15) / 16);
-    long long want = std::max<long long>((4LL * sms + base - 1) / base, (tiles + 127) / 128);
+    long long want = p->n_seq == 1 ? 3LL * sms / base : (6LL * sms + base - 1) / base;
+    want = std::max<long long>(std::max<long long>(want, 1), (tiles + 127) / 128);
     want = std::min<long long>(want, (tiles + 3) / 4);
     d.split.n_splits = (int)want;
     d.split.tiles = (int)((tiles + want - 1) / want);
@@ -207,39 +208,53 @@ TilePlan plan_tile(const vtx_paged_kv *p, int G, int Hq, int min_rows, int sms) 
     if (!t.use || !t.unpack) t.u_bytes = 0;
     if (!t.use) return t;
     t.tile.T = 128 / G;
-    const long long pair = 2 * t.tile.T;
     // streams with more than min_rows rows, and what rounding each up to whole groups adds
     const long long streams = std::min<long long>(p->n_seq, p->n_tokens / (min_rows / G + 1));
-    t.tile.groups = (int)((p->n_tokens + streams * (pair - 1)) / pair);
+    auto groups_of = [&](long long tokens) { return (p->n_tokens + streams * (tokens - 1)) / tokens; };
+    // single Q tiles over short caches while they fit on the SMs at once (a prompt of
+    // 391 tokens, 8 KV heads: 104 CTAs instead of 56, 14.8 us instead of 15.9; over
+    // 14k keys pairs win, which share K and V and the tensor core: 512 tokens 154
+    // against 211 us)
+    const long long pair = groups_of(t.tile.T) * Hkv <= sms && p->max_kv_len <= 1024 ? t.tile.T : 2 * t.tile.T;
+    t.tile.tokens = (int)pair;
+    t.tile.groups = (int)groups_of(pair);
     t.tile.min_tiles = 2;
     // Splits of a group's key tiles: the number of least estimated time.  A key
-    // tile of a group takes about 2.2 us (D = 128); a merge writes and reads every
-    // row once per split at about 4 TB/s and costs a launch.  One stream: its
-    // groups are about equal, so whole waves count.  Several: lengths spread, so
-    // the average load plus half a CTA's time.
+    // tile of a group takes about 2.1 us (D = 128), a CTA's start and end 6; a
+    // merge writes and reads a split's rows at about 5 TB/s and costs a launch.
+    // One stream: its groups are about equal, so whole waves count, and full waves
+    // are left whole.  Several: lengths spread, so the average load plus half a
+    // CTA's time.
     const int tiles = std::max(1, (p->max_kv_len + 127) / 128);
-    const double tile_us = D == 128 ? 2.2 : 1.6;
-    const double merge_us = (double)p->n_tokens * Hq * D * 8 / 4e6;
-    double best = 1e30;
+    const double tile_us = D == 128 ? 2.1 : 1.6, cta_us = 6.0;
+    const double row_us = (double)D * 8 / 5e6;               // one row, one split
+    const long long items = (long long)t.tile.groups * Hkv;
+    double best = 1e30, one = 1e30;
     t.tile.n_splits = 1;
     for (int s = 1; s <= 32 && s <= (tiles + 1) / 2; ++s) {
-        const double each = (double)((tiles + s - 1) / s);
-        double us;
+        const double each = (double)((tiles + s - 1) / s) * tile_us + cta_us;
         if (p->n_seq == 1) {
-            us = (double)(((long long)t.tile.groups * Hkv * s + sms - 1) / sms) * (each * tile_us + 4.0);
+            for (long long whole = 0; whole <= (s > 1 ? items : 0); whole += sms) {
+                const double us = (double)(whole / sms) * (tiles * tile_us + cta_us) +
+                                  (double)(((items - whole) * s + sms - 1) / sms) * each +
+                                  (s > 1 ? (items - whole) * 256.0 * s * row_us + 3.0 : 0.0);
+                if (s == 1) one = us;
+                // launches of full waves are short of power, not of SMs: a small gain
+                // is none there (2048 tokens at 14k: 519 us whole, 530 with the last
+                // wave split; 1184 tokens: 394 and 290)
+                if (us < best && (s == 1 || items < sms || us < 0.85 * one)) {
+                    best = us;
+                    t.tile.n_splits = s;
+                    t.tile.whole = (int)whole;
+                }
+            }
         } else {
             const double ctas = (double)p->n_tokens / pair * Hkv;
-            us = ctas * tiles * 0.5 / sms * tile_us + 0.5 * each * tile_us + 4.0;
-        }
-        if (s > 1) us += s * merge_us + 3.0;
-        if (us < best) {
-            best = us;
-            t.tile.n_splits = s;
+            const double us = ctas * tiles * 0.5 / sms * tile_us + 0.5 * each +
+                              (s > 1 ? (double)p->n_tokens * Hq * s * row_us + 3.0 : 0.0);
+            if (us < best) { best = us; t.tile.n_splits = s; }
         }
     }
-#ifdef NSPLIT
-    t.tile.n_splits = NSPLIT;
-#endif
     if (t.tile.n_splits > 1) {
         // every split that long, so that shorter streams have fewer
         t.tile.min_tiles = std::max(2, (tiles + t.tile.n_splits - 1) / t.tile.n_splits);
@@ -305,7 +320,8 @@ int launch_tile(const CUtensorMap (&m)[3], const PagedAttnArgs &a, const PagedTi
     static std::atomic<int> done[kMaxDevices];
     int rc = allow_smem(fa_paged_sm100_kernel<D, UF>, C::SMEM, done);
     if (rc != VTX_OK) return rc;
-    const long long ctas = (long long)tl.groups * a.kv.Hkv * tl.n_splits;
+    const long long items = (long long)tl.groups * a.kv.Hkv;
+    const long long ctas = tl.whole + (items - tl.whole) * tl.n_splits;
     if (ctas > 0x7fffffffLL) return VTX_ERR_UNSUPPORTED;
     if (ctas == 0) return VTX_OK;
     return launch_pdl(fa_paged_sm100_kernel<D, UF>, dim3((unsigned)ctas), dim3(C::NTHREADS), C::SMEM, st, m[0], m[1],
@@ -314,7 +330,7 @@ int launch_tile(const CUtensorMap (&m)[3], const PagedAttnArgs &a, const PagedTi
 
 template <int D>
 int launch_tile_combine(const PagedAttnArgs &a, const PagedTile &tl, cudaStream_t st) {
-    return launch_pdl(fa_paged_tile_combine_kernel<D>, dim3((unsigned)a.kv.n_tokens, (unsigned)((a.Hq + 7) / 8)),
+    return launch_pdl(fa_paged_tile_combine_kernel<D>, dim3((unsigned)a.kv.n_tokens, (unsigned)((a.Hq + 31) / 32)),
                       dim3(256), 0, st, a, tl);
 }
 
