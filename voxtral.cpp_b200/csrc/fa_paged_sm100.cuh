@@ -530,7 +530,7 @@ fa_paged_tile_combine_kernel(const PagedAttnArgs a, const PagedTile tl)
     grid_dep_launch();
     constexpr int H = 4;
     const int t = blockIdx.x;
-    const int b = paged_find(a.kv, t);
+    const int b = paged_find(a.kv, t, threadIdx.x & 31);
     if (b >= a.kv.n_seq) return;
     const PagedSeq s = paged_seq(a.kv, b);
     const int tok = t - s.q0, served = min(s.n_new, a.kv.max_new);

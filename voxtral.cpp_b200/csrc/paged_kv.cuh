@@ -62,16 +62,18 @@ __device__ __forceinline__ long long paged_row(const PagedView &kv, int b, int r
            (long long)g * kv.nb2;
 }
 
-// Stream of packed token t (the last one whose q_start is <= t and that has
-// tokens): every thread of the CTA counts a share of the streams.  The CTA's
-// threads all call it; `t` is uniform.
-__device__ __forceinline__ int paged_find(const PagedView &kv, int t) {
-    int n = 0;
-    for (int i0 = 0; i0 < kv.n_seq; i0 += blockDim.x) {
-        const int i = i0 + (int)threadIdx.x;
-        n += __syncthreads_count(i < kv.n_seq && kv.q_start[i + 1] <= t);
+// Stream of packed token t: the first whose tokens end behind t (n_seq: none).  A
+// warp searches q_start 32 entries at a time; all lanes call it, `t` is uniform.
+__device__ __forceinline__ int paged_find(const PagedView &kv, int t, int lane) {
+    int lo = 0, hi = kv.n_seq;                              // the answer lies in [lo, hi]
+    while (hi - lo > 32) {
+        const int step = (hi - lo + 31) / 32, i = lo + lane * step;
+        const int c = __popc(__ballot_sync(0xffffffffu, i < hi && kv.q_start[i + 1] <= t));
+        hi = min(hi, lo + c * step);
+        if (c > 0) lo += (c - 1) * step + 1;
     }
-    return n;                               // n_seq when no stream holds t
+    const int i = lo + lane;
+    return lo + __popc(__ballot_sync(0xffffffffu, i < hi && kv.q_start[i + 1] <= t));
 }
 
 // ---- append ---------------------------------------------------------------------
@@ -89,32 +91,114 @@ struct KvAppendPagedArgs {
     double turns[64];                       // base^(-2i/D) / (2 pi): turns per position of pair i
 };
 
-// Grid (tokens, ceil((Hq + 2 Hkv) / rows_per_cta)), 8 warps, a warp per row,
-// as kv_append_kernel.  HBM-bound: (Hq + 2 Hkv) * D * 4 bytes read and
-// Hq * D * (2 or 4) + 2 Hkv * row bytes written per token.
+// A head row, 8 values per lane, as Q8_0 into 4-byte aligned `row`: the bytes of
+// store_q8_lane in whole words.  A block is four lanes, two blocks are 17 words: the
+// even block's values start 2 bytes in, so its words join two neighbours (the first
+// takes the scale, the odd block's first lane closes it with its own scale); the odd
+// block's values are aligned.  u: the lane's place in its row.
+__device__ __forceinline__ void store_q8_words(const float (&x)[8], char *row, int u, bool put) {
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const float id = amax != 0.f ? 127.f / amax : 0.f;
+    const uint32_t d = __half_as_ushort(__float2half_rn(amax / 127.f));
+    uint32_t q[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        q[i] = (uint32_t)(__float2int_rn(x[4 * i] * id) & 0xff) | (uint32_t)(__float2int_rn(x[4 * i + 1] * id) & 0xff) << 8 |
+               (uint32_t)(__float2int_rn(x[4 * i + 2] * id) & 0xff) << 16 |
+               (uint32_t)(__float2int_rn(x[4 * i + 3] * id) & 0xff) << 24;
+    const uint32_t before = __shfl_up_sync(0xffffffffu, q[1], 1);
+    if (!put) return;                                       // the shuffles want the whole warp
+    const int j = u & 3;
+    uint32_t *w = reinterpret_cast<uint32_t *>(row) + (u >> 3) * 17 + 2 * j;
+    if (u & 4) {
+        w[9] = q[0];
+        w[10] = q[1];
+        if (j == 0) w[8] = before >> 16 | d << 16;
+    } else {
+        w[0] = (j == 0 ? d : before >> 16) | q[0] << 16;
+        w[1] = __funnelshift_r(q[0], q[1], 16);
+    }
+}
+
+// 8 floats from 16-byte (W16) or 8-byte aligned memory.
+template <bool W16>
+__device__ __forceinline__ void load_f8(float (&x)[8], const float *p) {
+    if constexpr (W16) {
+        *reinterpret_cast<float4 *>(&x[0]) = *reinterpret_cast<const float4 *>(p);
+        *reinterpret_cast<float4 *>(&x[4]) = *reinterpret_cast<const float4 *>(p + 4);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) *reinterpret_cast<float2 *>(&x[i]) = *reinterpret_cast<const float2 *>(p + i);
+    }
+}
+template <bool W16>
+__device__ __forceinline__ void store_8(void *dst, bool f16, const float (&x)[8]) {
+    if (f16) {
+        const uint4 h = make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]),
+                                   pack_half2(x[6], x[7]));
+        if constexpr (W16) {
+            *static_cast<uint4 *>(dst) = h;
+        } else {
+            static_cast<uint2 *>(dst)[0] = make_uint2(h.x, h.y);
+            static_cast<uint2 *>(dst)[1] = make_uint2(h.z, h.w);
+        }
+    } else if constexpr (W16) {
+        static_cast<float4 *>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        static_cast<float4 *>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) static_cast<float2 *>(dst)[i] = make_float2(x[2 * i], x[2 * i + 1]);
+    }
+}
+
+// Grid (tokens, ceil((Hq + 2 Hkv) / rows_per_cta)), 8 warps; D / 8 lanes per row, 8
+// values each, so a warp takes 2 (D = 128) or 4 rows at once.
+// HBM-bound by its bytes: (Hq + 2 Hkv) * D * 4 read and Hq * D * (2 or 4) + 2 Hkv *
+// row bytes written per token.  The way to a row's page (stream of the token, its
+// lengths, the table) is three dependent trips to memory, so a warp loads its first
+// rows before it takes them.  A whole warp per row issued 5900 instructions per
+// token and was bound by them (7639 tokens, Q8_0: 64 us against APPEND_US).
 // Angle of pair i: pos * turns[i] turns, reduced to (-1/2, 1/2] in double (three
 // operations), then sincospi in float: an error of about 1e-7 at any position.
-template <int D>
+template <int D, bool W16>
 __global__ void __launch_bounds__(256)
 kv_append_paged_kernel(const __grid_constant__ KvAppendPagedArgs a)
 {
     grid_dep_wait();
     grid_dep_launch();
-    constexpr int E = D / 32;                               // elements per lane
+    constexpr int LPR = D / 8, RPW = 32 / LPR, NR = 3;      // lanes per row, rows per warp, row sets in flight
     __shared__ float2 cs[D / 2];                            // (cos, sin) of pair i
     const int t = blockIdx.x;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int nwarps = blockDim.x >> 5, r0 = blockIdx.y * a.rows_per_cta;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, u = lane % LPR;
+    const int r0 = blockIdx.y * a.rows_per_cta, r1 = min(r0 + a.rows_per_cta, a.Hq + 2 * a.kv.Hkv);
+    const int first = r0 + warp * RPW + lane / LPR;         // this lane's rows: first, first + 8 RPW, ...
+    float x[NR][8];
+    // rows of a token: Q heads, then K heads, then V heads
+    auto load = [&](int rb) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            const int r = rb + 8 * RPW * i;
+            const float *src = r < a.Hq ? a.q + (long long)t * a.q_nb1 + (long long)r * D
+                               : r < a.Hq + a.kv.Hkv ? a.k + (long long)t * a.k_nb1 + (long long)(r - a.Hq) * D
+                               : a.v + (long long)t * a.v_nb1 + (long long)(r - a.Hq - a.kv.Hkv) * D;
+            if (r < r1) load_f8<W16>(x[i], src + u * 8);
+        }
+    };
+    load(first);
     const int pos = a.positions[t];
     if (r0 < a.Hq + a.kv.Hkv && threadIdx.x < D / 2) {      // some Q or K row here
-        double x = (double)pos * a.turns[threadIdx.x];
-        x -= rint(x);
+        double y = (double)pos * a.turns[threadIdx.x];
+        y -= rint(y);
         float s, c;
-        sincospif(2.0f * (float)x, &s, &c);
+        sincospif(2.0f * (float)y, &s, &c);
         cs[threadIdx.x] = make_float2(c, s);
     }
-    const int b = paged_find(a.kv, t);                      // also orders the table
     __syncthreads();
+    const int b = paged_find(a.kv, t, lane);
     int row = -1;
     if (b < a.kv.n_seq) {
         const PagedSeq s = paged_seq(a.kv, b);
@@ -126,50 +210,32 @@ kv_append_paged_kernel(const __grid_constant__ KvAppendPagedArgs a)
     }
     const int page = row >= 0 ? paged_page(a.kv, b, row) : -1;
     const long long at = (long long)page * a.kv.nb3 + (long long)(row & ((1 << a.kv.shift) - 1)) * a.kv.nb1;
-    const int per_tok = a.Hq + 2 * a.kv.Hkv;
-    for (int r = r0 + warp; r < min(r0 + a.rows_per_cta, per_tok); r += nwarps) {
-        const int kind = r < a.Hq ? 0 : (r < a.Hq + a.kv.Hkv ? 1 : 2);   // Q, K, V
-        const int h = kind == 0 ? r : (kind == 1 ? r - a.Hq : r - a.Hq - a.kv.Hkv);
-        const float *src = kind == 0 ? a.q + (long long)t * a.q_nb1
-                                     : (kind == 1 ? a.k + (long long)t * a.k_nb1 : a.v + (long long)t * a.v_nb1);
-        src += (long long)h * D + lane * E;
-        float x[E];
+    for (int rb = first; rb - lane / LPR < r1; rb += 8 * RPW * NR) {     // uniform within the warp
+        if (rb != first) load(rb);
 #pragma unroll
-        for (int i = 0; i < E; i += 2) {
-            const float2 p = *reinterpret_cast<const float2 *>(src + i);
-            x[i] = p.x;
-            x[i + 1] = p.y;
-        }
-        if (kind != 2) {
+        for (int i = 0; i < NR; ++i) {
+            const int r = rb + 8 * RPW * i;
+            if (r < a.Hq + a.kv.Hkv) {
 #pragma unroll
-            for (int j = 0; j < E / 2; ++j) rope_pair(x[2 * j], x[2 * j + 1], cs[lane * E / 2 + j]);
-        }
-        if (kind == 0) {
-            const long long o = (long long)t * a.qo_nb1 + (long long)h * D + lane * E;
-#pragma unroll
-            for (int i = 0; i < E; i += 2) {
-                if (a.qo_f16)
-                    *reinterpret_cast<__half2 *>(static_cast<__half *>(a.q_out) + o + i) =
-                        __floats2half2_rn(x[i], x[i + 1]);
-                else
-                    *reinterpret_cast<float2 *>(static_cast<float *>(a.q_out) + o + i) = make_float2(x[i], x[i + 1]);
+                for (int j = 0; j < 4; ++j) rope_pair(x[i][2 * j], x[i][2 * j + 1], cs[u * 4 + j]);
             }
-            continue;
-        }
-        if (page < 0) continue;
-        if (kind == 1 && lane == 0) {                       // the row starts without weight
-            const long long e = ((long long)b * a.kv.Hkv + h) * a.row_cap + row;
-            if (a.row_pos) a.row_pos[e] = pos;
-            if (a.score) a.score[e] = 0.0f;
-        }
-        char *dst = (kind == 1 ? a.kv.k : a.kv.v) + at + (long long)h * a.kv.nb2;
-        if (a.q8) {
-            store_q8_lane<E>(x, dst, lane);
-        } else {
-#pragma unroll
-            for (int i = 0; i < E; i += 2)
-                *reinterpret_cast<__half2 *>(reinterpret_cast<__half *>(dst) + lane * E + i) =
-                    __floats2half2_rn(x[i], x[i + 1]);
+            const bool is_k = r < a.Hq + a.kv.Hkv;
+            const int h = r - a.Hq - (is_k ? 0 : a.kv.Hkv);
+            char *dst = (is_k ? a.kv.k : a.kv.v) + at + (long long)h * a.kv.nb2;
+            const bool put = r >= a.Hq && r < r1 && page >= 0;
+            if (r < a.Hq && r < r1)
+                store_8<W16>(static_cast<char *>(a.q_out) + ((long long)t * a.qo_nb1 + (long long)r * D + u * 8) *
+                                                                (a.qo_f16 ? 2 : 4), a.qo_f16, x[i]);
+            if (put && is_k && u == 0) {                    // the row starts without weight
+                const long long e = ((long long)b * a.kv.Hkv + h) * a.row_cap + row;
+                if (a.row_pos) a.row_pos[e] = pos;
+                if (a.score) a.score[e] = 0.0f;
+            }
+            if (a.q8) {
+                if (__any_sync(0xffffffffu, put)) store_q8_words(x[i], dst, u, put);
+            } else if (put) {
+                store_8<true>(dst + u * 16, true, x[i]);    // pool rows are 16-byte aligned
+            }
         }
     }
 }

@@ -454,15 +454,18 @@ int vtx_kv_append_paged(const vtx_kv_append_paged_args *p, void *stream) {
     a.row_pos = p->row_pos; a.score = p->score; a.row_cap = p->row_cap;
     for (int i = 0; i < D / 2; ++i)
         a.turns[i] = std::pow((double)p->freq_base, -2.0 * i / D) / (2.0 * 3.14159265358979323846);
-    // few tokens: 8 rows (one per warp) per CTA, so that all rows are in flight
-    // together; many tokens: one CTA and one cos/sin table per token
+    // few tokens: a warp's rows (two or four) at once per CTA and warp, so that all
+    // rows are in flight together; many: one CTA and one cos/sin table per token
     const int per_tok = a.Hq + 2 * a.kv.Hkv;
-    a.rows_per_cta = kv->n_tokens >= 2 * ds->sms ? per_tok : 8;
+    a.rows_per_cta = kv->n_tokens >= 2 * ds->sms ? per_tok : D == 64 ? 32 : 16;
     const dim3 grid((unsigned)kv->n_tokens, (unsigned)((per_tok + a.rows_per_cta - 1) / a.rows_per_cta));
     if (grid.y > 65535) return VTX_ERR_SHAPE;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return D == 64 ? launch_pdl(kv_append_paged_kernel<64>, grid, dim3(256), 0, st, a)
-                   : launch_pdl(kv_append_paged_kernel<128>, grid, dim3(256), 0, st, a);
+    if (rows % 16 == 0)
+        return D == 64 ? launch_pdl(kv_append_paged_kernel<64, true>, grid, dim3(256), 0, st, a)
+                       : launch_pdl(kv_append_paged_kernel<128, true>, grid, dim3(256), 0, st, a);
+    return D == 64 ? launch_pdl(kv_append_paged_kernel<64, false>, grid, dim3(256), 0, st, a)
+                   : launch_pdl(kv_append_paged_kernel<128, false>, grid, dim3(256), 0, st, a);
 }
 
 size_t vtx_flash_attn_paged_workspace(const vtx_paged_kv *kv, int32_t n_head_q) {

@@ -549,7 +549,7 @@ class PagedKv:
         if dev.type != "cuda":
             raise VtxError(-8, "the pools are not on a GPU")
         s = stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(dev.index)
-        if torch.cuda.current_device() == dev.index:
+        if torch._C._cuda_getDevice() == dev.index:
             rc = fn(ctypes.byref(args), *ws, s)
         else:
             with torch.cuda.device(dev):
