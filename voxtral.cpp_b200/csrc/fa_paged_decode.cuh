@@ -5,9 +5,12 @@
 // Every K and V row is read once and does 4 flops a byte per query row, so the
 // call is bound by HBM.  One CTA per (stream, KV head, key split); its 4 warps
 // take tiles of 16 keys in turn, each through a private ring of bulk copies
-// (no CTA barrier in the loop), 16-key tiles never cross a page.  The n * G
-// query rows (token * G + head of the group) are the M operand of mma.sync
-// m16n8k16: S = Q K^T, then the S fragment becomes the A fragment of O += P V.
+// (no CTA barrier in the loop), 16-key tiles never cross a page.  The products run
+// on mma.sync m16n8k16 turned round: S^T = K Q^T and O^T += V^T P^T, with the keys
+// (the dims) as the 16 rows and the n * G query rows (token * G + head of the
+// group), padded to 8 or 16, as the columns.  With the query rows as the MMA's
+// rows half of it would be padding for G <= 8: twice the products and accumulator
+// registers.
 //   F16:  a lane copies one K or V row into a 16-byte padded pitch; ldmatrix.
 //   Q8_0: the 16 rows of a tile are one contiguous block, copied as such.  K's
 //         integers become halves exactly (0x64xx, minus 1152) and every block of
@@ -16,12 +19,12 @@
 //         is rounded to half, so P V has the one rounding that F16 has.  P stays
 //         below 2^6 there, which bounds |scale| by 1023.  The k index of an MMA
 //         may be any permutation: the lanes' words are chosen free of bank
-//         conflicts (keys 2n + tile, words c and c + 4 of a block).
-// Softmax in log2 units with a lazily moved reference m: O is rescaled only
-// when the running maximum passes it by 2^8 (2^6).  The warps' (m, l, O) are
-// merged in shared memory; with several splits every CTA leaves its result in the
-// workspace, and the one that arrives last at the (stream, KV head)'s counter
-// merges them in split order.
+//         conflicts (keys 2n and 2n + 1, words c and c + 4 of a block).
+// Softmax in log2 units with a lazily moved reference m: O is rescaled only when
+// some score passes it by 2^8 (2^6), which one vote per tile finds out.  The
+// warps' (m, l, O) are merged in shared memory; with several splits every CTA
+// leaves its result in the workspace, and the one that arrives last at the
+// (stream, KV head)'s counter merges them in split order.
 #pragma once
 #include <cuda_fp16.h>
 #include <cstdint>
@@ -43,7 +46,7 @@ template <int D, int KVT> struct PagedDecodeCfg {
     static constexpr int KEYS = 16, WARPS = 4;
     static constexpr int ROW = KVT == 1 ? D * 2 : D / 32 * 34;
     static constexpr int PITCH = KVT == 1 ? ROW + 16 : ROW;
-    static constexpr int STAGES = KVT == 1 ? 2 : 4;
+    static constexpr int STAGES = 2;
     static constexpr int STAGE_BYTES = 2 * KEYS * PITCH;
     // the ring, reused for the warp's 16 x D floats at the end
     static constexpr int WARP_BYTES = STAGES * STAGE_BYTES > 16 * D * 4 ? STAGES * STAGE_BYTES : 16 * D * 4;
@@ -75,115 +78,147 @@ __device__ __forceinline__ uint32_t lds_word(const char *p) {
 }
 __device__ __forceinline__ float lds_half(const char *p) { return __half2float(*reinterpret_cast<const __half *>(p)); }
 
-// S of 16 keys: x[nt] = columns of key tile nt (F16: keys 8 nt + col, Q8_0:
-// keys 2 col + nt).
-template <int D, int KVT>
-__device__ __forceinline__ void paged_tile_scores(const char *ks, const uint32_t (&qa)[D / 16][4], float (&x)[2][4],
-                                                  int lane)
+// The transpose of an 8 x 8 matrix of halves held as an MMA fragment.
+__device__ __forceinline__ uint32_t movm_t(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// The two keys of a tile whose scores a lane holds (which = 0, 1).
+template <int KVT>
+__device__ __forceinline__ int paged_tile_key(int lane, int which) {
+    return KVT == 1 ? (lane >> 2) + 8 * which : 2 * (lane >> 2) + which;
+}
+// First dim of the pairs that a lane's Q fragment of k step kc takes (b0; b1: + 8,
+// Q8_0: + 2).
+template <int KVT>
+__device__ __forceinline__ int paged_q_dim(int lane, int kc) {
+    return KVT == 1 ? kc * 16 + 2 * (lane & 3) : (kc >> 1) * 32 + (kc & 1) * 16 + 4 * (lane & 3);
+}
+
+// S^T of 16 keys: x[nc][2 i + j] = key paged_tile_key(i), query row 8 nc + 2c + j.
+template <int D, int KVT, int NC>
+__device__ __forceinline__ void paged_tile_scores(const char *ks, const uint32_t (&qb)[NC][D / 16][2],
+                                                  float (&x)[NC][4], int lane)
 {
     using C = PagedDecodeCfg<D, KVT>;
-    constexpr int KC = D / 16;
     const int c = lane & 3, n = lane >> 2;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[0][i] = x[1][i] = 0.f;
+    for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[nc][i] = 0.f;
     if constexpr (KVT == 1) {
-        const int lrow = lane & 7, lmat = lane >> 3;
-        float y[2][4];
+        const char *p = ks + ((lane & 7) + (lane & 8)) * C::PITCH + (lane >> 4) * 16;
+        float y[NC][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[0][i] = y[1][i] = 0.f;
+        for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-        for (int kc = 0; kc < KC; kc += 2) {
-            uint32_t b0[4], b1[4];
-            ldsm_x4(b0, ks + lrow * C::PITCH + (kc * 16 + lmat * 8) * 2);
-            ldsm_x4(b1, ks + (8 + lrow) * C::PITCH + (kc * 16 + lmat * 8) * 2);
-            mma16816(x[0], qa[kc], b0[0], b0[1]);
-            mma16816(x[1], qa[kc], b1[0], b1[1]);
-            mma16816(y[0], qa[kc + 1], b0[2], b0[3]);
-            mma16816(y[1], qa[kc + 1], b1[2], b1[3]);
+            for (int i = 0; i < 4; ++i) y[nc][i] = 0.f;
+#pragma unroll
+        for (int kc = 0; kc < D / 16; kc += 2) {            // two chains
+            uint32_t k0[4], k1[4];
+            ldsm_x4(k0, p + kc * 32);
+            ldsm_x4(k1, p + kc * 32 + 32);
+#pragma unroll
+            for (int nc = 0; nc < NC; ++nc) {
+                mma16816(x[nc], k0, qb[nc][kc][0], qb[nc][kc][1]);
+                mma16816(y[nc], k1, qb[nc][kc + 1][0], qb[nc][kc + 1][1]);
+            }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[0][i] += y[0][i];
-            x[1][i] += y[1][i];
-        }
+        for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[nc][i] += y[nc][i];
     } else {
 #pragma unroll
         for (int b = 0; b < D / 32; ++b) {
+            const char *p = ks + 2 * n * C::ROW + 34 * b;
+            uint32_t w[2][2];                               // [key][word]
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-                const char *p = ks + (2 * n + nt) * C::ROW + 34 * b + 2 + 4 * c;
-                uint32_t w0, w1, k0, k1, k2, k3;
-                if (b & 1) { w0 = lds_word<false>(p); w1 = lds_word<false>(p + 16); }
-                else { w0 = lds_word<true>(p); w1 = lds_word<true>(p + 16); }
-                q8_halves(w0, k0, k1);
-                q8_halves(w1, k2, k3);
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const char *q = p + i * C::ROW + 2 + 4 * c + 16 * j;
+                    w[i][j] = (b & 1) ? lds_word<false>(q) : lds_word<true>(q);
+                }
+            const float d0 = lds_half(p), d1 = lds_half(p + C::ROW);
+            uint32_t k0[4], k1[4];
+            q8_halves(w[0][0], k0[0], k0[2]);
+            q8_halves(w[1][0], k0[1], k0[3]);
+            q8_halves(w[0][1], k1[0], k1[2]);
+            q8_halves(w[1][1], k1[1], k1[3]);
+#pragma unroll
+            for (int nc = 0; nc < NC; ++nc) {
                 float y[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16816(y, qa[2 * b], k0, k1);
-                mma16816(y, qa[2 * b + 1], k2, k3);
-                const float d0 = lds_half(ks + (4 * c + nt) * C::ROW + 34 * b);
-                const float d1 = lds_half(ks + (4 * c + 2 + nt) * C::ROW + 34 * b);
-                x[nt][0] = fmaf(d0, y[0], x[nt][0]);
-                x[nt][1] = fmaf(d1, y[1], x[nt][1]);
-                x[nt][2] = fmaf(d0, y[2], x[nt][2]);
-                x[nt][3] = fmaf(d1, y[3], x[nt][3]);
+                mma16816(y, k0, qb[nc][2 * b][0], qb[nc][2 * b][1]);
+                mma16816(y, k1, qb[nc][2 * b + 1][0], qb[nc][2 * b + 1][1]);
+                x[nc][0] = fmaf(d0, y[0], x[nc][0]);
+                x[nc][1] = fmaf(d0, y[1], x[nc][1]);
+                x[nc][2] = fmaf(d1, y[2], x[nc][2]);
+                x[nc][3] = fmaf(d1, y[3], x[nc][3]);
             }
         }
     }
 }
 
-// O += P V of 16 keys.  n0, n1: rows of the tile outside [n0, n1) hold anything
-// (Q8_0: their scale is taken as 0; F16: the loader zeroed them).
-template <int D, int KVT, int ROWS>
-__device__ __forceinline__ void paged_tile_pv(const char *vs, const float (&p)[2][4], int n0, int n1,
-                                              float (&o)[D / 8][4], int lane)
+// O^T += V^T P^T of 16 keys; o[nc][mt][2 i + j]: dim paged_o_dim(mt, i), query row
+// 8 nc + 2c + j.  Rows of the tile outside [n0, n1) hold anything (Q8_0: their
+// scale is taken as 0; F16: the loader zeroed them).
+template <int D, int KVT, int NC>
+__device__ __forceinline__ void paged_tile_pv(const char *vs, const float (&p)[NC][4], int n0, int n1,
+                                              float (&o)[NC][D / 16][4], int lane)
 {
     using C = PagedDecodeCfg<D, KVT>;
-    const int c = lane & 3;
+    const int c = lane & 3, n = lane >> 2;
     if constexpr (KVT == 1) {
-        const int lrow = lane & 7, lmat = lane >> 3;
-        const uint32_t pa[4] = {pack_half2(p[0][0], p[0][1]), ROWS > 8 ? pack_half2(p[0][2], p[0][3]) : 0u,
-                                pack_half2(p[1][0], p[1][1]), ROWS > 8 ? pack_half2(p[1][2], p[1][3]) : 0u};
+        uint32_t pb[NC][2];
 #pragma unroll
-        for (int nb = 0; nb < D / 8; nb += 2) {
-            uint32_t bv[4];
-            ldsm_x4_t(bv, vs + ((lmat & 1) * 8 + lrow) * C::PITCH + (nb * 8 + (lmat >> 1) * 8) * 2);
-            mma16816(o[nb], pa, bv[0], bv[1]);
-            mma16816(o[nb + 1], pa, bv[2], bv[3]);
+        for (int nc = 0; nc < NC; ++nc) {
+            pb[nc][0] = movm_t(pack_half2(p[nc][0], p[nc][1]));
+            pb[nc][1] = movm_t(pack_half2(p[nc][2], p[nc][3]));
+        }
+        const char *q = vs + ((lane >> 4) * 8 + (lane & 7)) * C::PITCH + (lane & 8) * 2;
+#pragma unroll
+        for (int mt = 0; mt < D / 16; ++mt) {
+            uint32_t v[4];
+            ldsm_x4_t(v, q + mt * 32);
+#pragma unroll
+            for (int nc = 0; nc < NC; ++nc) mma16816(o[nc][mt], v, pb[nc][0], pb[nc][1]);
         }
     } else {
-        const int n = lane >> 2;
-        const char *v0 = vs + 4 * c * C::ROW;                   // this lane's keys 4c ... 4c + 3
-        const bool all = n0 <= 0 && n1 >= 16;
+        const char *v0 = vs + 4 * c * C::ROW;               // the k pairs: keys (4c, 4c + 2) and (4c + 1, 4c + 3)
+        const char *s0 = vs + 2 * n * C::ROW;               // P's keys: 2n and 2n + 1
+        const bool on0 = 2 * n >= n0 && 2 * n < n1, on1 = 2 * n + 1 >= n0 && 2 * n + 1 < n1;
 #pragma unroll
         for (int b = 0; b < D / 32; ++b) {
-            float d[4];
+            const float d0 = on0 ? lds_half(s0 + 34 * b) : 0.f, d1 = on1 ? lds_half(s0 + C::ROW + 34 * b) : 0.f;
             uint32_t w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                d[j] = lds_half(v0 + j * C::ROW + 34 * b);
-                if (!all && (4 * c + j < n0 || 4 * c + j >= n1)) d[j] = 0.f;
                 const char *q = v0 + j * C::ROW + 34 * b + 2 + 4 * n;
                 w[j] = (b & 1) ? lds_word<false>(q) : lds_word<true>(q);
             }
-            const uint32_t pa[4] = {pack_half2(p[0][0] * d[0], p[0][1] * d[2]),
-                                    ROWS > 8 ? pack_half2(p[0][2] * d[0], p[0][3] * d[2]) : 0u,
-                                    pack_half2(p[1][0] * d[1], p[1][1] * d[3]),
-                                    ROWS > 8 ? pack_half2(p[1][2] * d[1], p[1][3] * d[3]) : 0u};
-            uint32_t x[4], y[4];                                // dims 4n + i of keys (4c, 4c+2) and (4c+1, 4c+3)
-            q8_halves(__byte_perm(w[0], w[2], 0x5140), x[0], x[1]);
-            q8_halves(__byte_perm(w[0], w[2], 0x7362), x[2], x[3]);
-            q8_halves(__byte_perm(w[1], w[3], 0x5140), y[0], y[1]);
-            q8_halves(__byte_perm(w[1], w[3], 0x7362), y[2], y[3]);
+            uint32_t v[2][4];                               // bytes 2 mt and 2 mt + 1 of word n: rows n, n + 8
+            q8_halves(__byte_perm(w[0], w[2], 0x5140), v[0][0], v[0][1]);
+            q8_halves(__byte_perm(w[0], w[2], 0x7362), v[1][0], v[1][1]);
+            q8_halves(__byte_perm(w[1], w[3], 0x5140), v[0][2], v[0][3]);
+            q8_halves(__byte_perm(w[1], w[3], 0x7362), v[1][2], v[1][3]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mma16816(o[4 * b + i], pa, x[i], y[i]);
+            for (int nc = 0; nc < NC; ++nc) {
+                const uint32_t b0 = movm_t(pack_half2(p[nc][0] * d0, p[nc][1] * d0));
+                const uint32_t b1 = movm_t(pack_half2(p[nc][2] * d1, p[nc][3] * d1));
+                mma16816(o[nc][2 * b], v[0], b0, b1);
+                mma16816(o[nc][2 * b + 1], v[1], b0, b1);
+            }
         }
     }
 }
 
-// The head dim of o[nb][j] in lane quad position c (j = 0, 1).
+// The head dim of o[nc][mt][2 i + j].
 template <int KVT>
-__device__ __forceinline__ int paged_o_dim(int nb, int j, int c) {
-    return KVT == 1 ? nb * 8 + 2 * c + j : (nb >> 2) * 32 + 8 * c + 4 * j + (nb & 3);
+__device__ __forceinline__ int paged_o_dim(int mt, int i, int lane) {
+    return KVT == 1 ? mt * 16 + (lane >> 2) + 8 * i : (mt >> 1) * 32 + 4 * (lane >> 2) + 2 * (mt & 1) + i;
 }
 
 // Normalises and writes 4 columns of query row r, and its lse with column 0.
@@ -202,7 +237,7 @@ template <int D, int KVT, int ROWS, bool UF>
 __device__ __forceinline__ void paged_decode_cta(const PagedAttnArgs &a, const PagedSplit &sp)
 {
     using C = PagedDecodeCfg<D, KVT>;
-    constexpr int KC = D / 16, NB = D / 8;
+    constexpr int KC = D / 16, NC = ROWS / 8;
     extern __shared__ __align__(128) char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3;
     char *ring = smem + warp * C::WARP_BYTES;
@@ -261,31 +296,44 @@ __device__ __forceinline__ void paged_decode_cta(const PagedAttnArgs &a, const P
 #pragma unroll
     for (int t = 0; t < C::STAGES; ++t) issue(t);
 
-    uint32_t qa[KC][4];
-    int lo[2], hi[2];
+    // Q fragments: a lane's column is query row 8 nc + lane / 4; its scores are of
+    // rows 8 nc + 2c + j, whose limits these are
+    uint32_t qb[NC][KC][2];
+    int lo[NC][2], hi[NC][2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int r = (lane >> 2) + 8 * u;
-        const bool on = r < rows && (u == 0 || ROWS > 8);
+    for (int nc = 0; nc < NC; ++nc) {
+        const int r = 8 * nc + (lane >> 2);
+        const bool on = r < rows;
         const int tok = on ? r / a.G : 0;
-        hi[u] = on ? (a.causal ? off + tok : s.len - 1) : -1;
-        lo[u] = a.window > 0 ? off + tok - a.window + 1 : 0;
         const char *qp = a.q + (long long)(s.q0 + tok) * a.q_nbt + (long long)(g * a.G + (on ? r % a.G : 0)) * a.q_nbh;
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {
-            // F16: dims 16 kc + 2c and + 8; Q8_0: dims 32 b + 16 (kc odd) + 4c and + 2
-            const int d = KVT == 1 ? kc * 16 + 2 * c : (kc >> 1) * 32 + (kc & 1) * 16 + 4 * c;
-            qa[kc][u] = on ? paged_q2(qp, a.q_f16, d) : 0u;
-            qa[kc][2 + u] = on ? paged_q2(qp, a.q_f16, d + (KVT == 1 ? 8 : 2)) : 0u;
+            const int d = paged_q_dim<KVT>(lane, kc);
+            qb[nc][kc][0] = on ? paged_q2(qp, a.q_f16, d) : 0u;
+            qb[nc][kc][1] = on ? paged_q2(qp, a.q_f16, d + (KVT == 1 ? 8 : 2)) : 0u;
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int r2 = 8 * nc + 2 * c + j, tok2 = r2 / a.G;
+            hi[nc][j] = r2 < rows ? (a.causal ? off + tok2 : s.len - 1) : -1;
+            lo[nc][j] = a.window > 0 ? off + tok2 - a.window + 1 : 0;
         }
     }
-    const int hi_all = a.causal ? off : s.len - 1;              // every token sees [lo_all, hi_all]
+    // every token sees [lo_all, hi_all] (padding rows' results are not read)
+    const int hi_all = a.causal ? off : s.len - 1;
     const int lo_all = a.window > 0 ? off + s.n_new - a.window : 0;
 
-    float o[NB][4];
+    float o[NC][KC][4];
 #pragma unroll
-    for (int i = 0; i < NB; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+        for (int i = 0; i < KC; ++i) o[nc][i][0] = o[nc][i][1] = o[nc][i][2] = o[nc][i][3] = 0.f;
+    float m[NC][2], l[NC][2];
+#pragma unroll
+    for (int nc = 0; nc < NC; ++nc) {
+        m[nc][0] = m[nc][1] = -INFINITY;
+        l[nc][0] = l[nc][1] = 0.f;
+    }
     const float cx = a.scale * kLog2e;
     constexpr float kJump = KVT == 1 ? 8.0f : 6.0f, kBack = KVT == 1 ? 0.0f : 4.0f;
     bool ok = true;
@@ -295,41 +343,50 @@ __device__ __forceinline__ void paged_decode_cta(const PagedAttnArgs &a, const P
         if (!ok) break;
         const char *ks = ring + (t % C::STAGES) * C::STAGE_BYTES, *vs = ks + C::KEYS * C::PITCH;
         const int k0 = cut.lo + 16 * (first + t * C::WARPS);
-        float x[2][4];
-        paged_tile_scores<D, KVT>(ks, qa, x, lane);
+        float x[NC][4];
+        paged_tile_scores<D, KVT, NC>(ks, qb, x, lane);
         const bool inner = k0 >= lo_all && k0 + 15 <= hi_all;
+        bool jump = false;
 #pragma unroll
-        for (int u = 0; u < (ROWS > 8 ? 2 : 1); ++u) {
-            float mx = -INFINITY;
+        for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-            for (int nt2 = 0; nt2 < 2; ++nt2)
+            for (int i = 0; i < 4; ++i) {
+                float &y = x[nc][i];
+                y = paged_logit_t<UF>(y, cx, a.scale, a.softcap);
+                if (!inner) {
+                    const int key = k0 + paged_tile_key<KVT>(lane, i >> 1);
+                    y = key < lo[nc][i & 1] || key > hi[nc][i & 1] ? -INFINITY : y;
+                }
+                jump |= y > m[nc][i & 1] + kJump;
+            }
+        if (__any_sync(0xffffffffu, jump)) {
+#pragma unroll
+            for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    float &y = x[nt2][2 * u + j];
-                    y = paged_logit_t<UF>(y, cx, a.scale, a.softcap);
-                    if (!inner) {
-                        const int key = k0 + (KVT == 1 ? 8 * nt2 + 2 * c + j : 4 * c + 2 * j + nt2);
-                        y = key < lo[u] || key > hi[u] ? -INFINITY : y;
+                    float mx = fmaxf(x[nc][j], x[nc][2 + j]);
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    if (mx > m[nc][j] + kJump) {            // the same in every lane of this row
+                        const float al = ex2(m[nc][j] - (mx - kBack));
+                        m[nc][j] = mx - kBack;
+                        l[nc][j] *= al;
+#pragma unroll
+                        for (int i = 0; i < KC; ++i) { o[nc][i][j] *= al; o[nc][i][2 + j] *= al; }
                     }
-                    mx = fmaxf(mx, y);
                 }
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            if (mx > m[u] + kJump) {                            // uniform within the quad
-                const float al = ex2(m[u] - (mx - kBack));
-                m[u] = mx - kBack;
-                l[u] *= al;
-#pragma unroll
-                for (int i = 0; i < NB; ++i) { o[i][2 * u] *= al; o[i][2 * u + 1] *= al; }
-            }
-            const float mu = m[u] == -INFINITY ? 0.f : m[u];
-#pragma unroll
-            for (int nt2 = 0; nt2 < 2; ++nt2)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) x[nt2][2 * u + j] = ex2(x[nt2][2 * u + j] - mu);
-            l[u] += (x[0][2 * u] + x[0][2 * u + 1]) + (x[1][2 * u] + x[1][2 * u + 1]);
         }
-        paged_tile_pv<D, KVT, ROWS>(vs, x, lo_any - k0, s.len - k0, o, lane);
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float mu = m[nc][j] == -INFINITY ? 0.f : m[nc][j];
+                x[nc][j] = ex2(x[nc][j] - mu);
+                x[nc][2 + j] = ex2(x[nc][2 + j] - mu);
+                l[nc][j] += x[nc][j] + x[nc][2 + j];
+            }
+        paged_tile_pv<D, KVT, NC>(vs, x, lo_any - k0, s.len - k0, o, lane);
         __syncwarp();                                           // every lane has read this stage
         issue(t + C::STAGES);
         done = t + 1;
@@ -341,25 +398,30 @@ __device__ __forceinline__ void paged_decode_cta(const PagedAttnArgs &a, const P
     // ---- merge the warps: each scales its O to the common maximum -------------
     float2 *ml = reinterpret_cast<float2 *>(smem + C::ML_OFF);  // [WARPS][16]
 #pragma unroll
-    for (int u = 0; u < (ROWS > 8 ? 2 : 1); ++u) {
-        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
-        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
-        if (c == 0) ml[warp * 16 + (lane >> 2) + 8 * u] = make_float2(m[u], l[u]);
-    }
+    for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            l[nc][j] += __shfl_xor_sync(0xffffffffu, l[nc][j], 4);
+            l[nc][j] += __shfl_xor_sync(0xffffffffu, l[nc][j], 8);
+            l[nc][j] += __shfl_xor_sync(0xffffffffu, l[nc][j], 16);
+            if (lane < 4) ml[warp * 16 + 8 * nc + 2 * c + j] = make_float2(m[nc][j], l[nc][j]);
+        }
     __syncthreads();
     float *mine = reinterpret_cast<float *>(ring);
 #pragma unroll
-    for (int u = 0; u < (ROWS > 8 ? 2 : 1); ++u) {
-        const int r = (lane >> 2) + 8 * u;
-        float top = -INFINITY;
+    for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-        for (int w = 0; w < C::WARPS; ++w) top = fmaxf(top, ml[w * 16 + r].x);
-        const float f = m[u] == -INFINITY ? 0.f : ex2(m[u] - top);
+        for (int j = 0; j < 2; ++j) {
+            const int r = 8 * nc + 2 * c + j;
+            float top = -INFINITY;
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+            for (int w = 0; w < C::WARPS; ++w) top = fmaxf(top, ml[w * 16 + r].x);
+            const float f = m[nc][j] == -INFINITY ? 0.f : ex2(m[nc][j] - top);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) mine[r * D + paged_o_dim<KVT>(nb, j, c)] = o[nb][2 * u + j] * f;
-    }
+            for (int mt = 0; mt < KC; ++mt)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) mine[r * D + paged_o_dim<KVT>(mt, i, lane)] = o[nc][mt][2 * i + j] * f;
+        }
     __syncthreads();
     const long long work = ((long long)b * a.kv.Hkv + g) * sp.n_splits + split;
     for (int i = threadIdx.x; i < rows * (D / 4); i += 128) {
@@ -455,7 +517,7 @@ __device__ __forceinline__ void paged_decode_cta(const PagedAttnArgs &a, const P
 // be waited for: the few-token streams fill the SMs that its last CTAs leave
 // idle.  The wait comes last instead, so that this kernel's end is both ends.
 template <int D, int KVT, int ROWS, bool UF>
-__global__ void __launch_bounds__(128, 3)
+__global__ void __launch_bounds__(128, KVT == 8 && ROWS == 8 ? 5 : 3)
 fa_paged_decode_kernel(const PagedAttnArgs a, const PagedSplit sp)
 {
     if (!sp.beside) grid_dep_wait();

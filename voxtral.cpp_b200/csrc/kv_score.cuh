@@ -154,18 +154,18 @@ kv_score_kernel(const PagedScoreArgs a)
 // Streams with at most 16 query rows per KV head: the K half of the streaming
 // attention kernel.  A CTA per (stream, KV head, key split), its 4 warps take
 // tiles of 16 keys in turn through private rings of bulk copies; a tile's
-// weights are summed over the row lanes by shuffles and added to the old score,
+// weights are summed over a quad's rows by shuffles and added to the old score,
 // which was loaded before the wait for the tile.
 template <int D, int KVT> struct ScoreStreamCfg {
     using P = PagedDecodeCfg<D, KVT>;
-    static constexpr int STAGES = KVT == 1 ? 3 : 5;
+    static constexpr int STAGES = KVT == 1 ? 2 : 4;
     static constexpr int STAGE_BYTES = 16 * P::PITCH;
     static constexpr int WARP_BYTES = STAGES * STAGE_BYTES;
     static constexpr int BAR_OFF = 4 * WARP_BYTES;
     static constexpr int SMEM = BAR_OFF + 4 * STAGES * 8;
 };
 
-template <int D, int KVT, bool UF>
+template <int D, int KVT, int ROWS, bool UF>
 __global__ void __launch_bounds__(128)
 kv_score_stream_kernel(const PagedScoreArgs a, const PagedSplit sp)
 {
@@ -173,7 +173,7 @@ kv_score_stream_kernel(const PagedScoreArgs a, const PagedSplit sp)
     grid_dep_launch();
     using P = PagedDecodeCfg<D, KVT>;
     using C = ScoreStreamCfg<D, KVT>;
-    constexpr int KC = D / 16;
+    constexpr int KC = D / 16, NC = ROWS / 8;
     extern __shared__ __align__(128) char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 3;
     char *ring = smem + warp * C::WARP_BYTES;
@@ -224,28 +224,36 @@ kv_score_stream_kernel(const PagedScoreArgs a, const PagedSplit sp)
 #pragma unroll
     for (int t = 0; t < C::STAGES; ++t) issue(t);
 
-    uint32_t qa[KC][4];
-    int lo[2], hi[2];
-    float ls[2];
+    // Q fragments of the lane's column, limits and lse of the rows 8 nc + 2c + j that
+    // its scores belong to
+    uint32_t qb[NC][KC][2];
+    int lo[NC][2], hi[NC][2];
+    float ls[NC][2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int r = (lane >> 2) + 8 * u;
+    for (int nc = 0; nc < NC; ++nc) {
+        const int r = 8 * nc + (lane >> 2);
         const bool on = r < rows;
-        const int tok = t0 + (on ? r / a.G : 0), head = g * a.G + (on ? r % a.G : 0);
-        hi[u] = on ? (a.causal ? min(off + tok, limit - 1) : limit - 1) : -1;
-        lo[u] = a.window > 0 ? off + tok - a.window + 1 : 0;
-        const char *qp = a.q + (long long)(s.q0 + tok) * a.q_nbt + (long long)head * a.q_nbh;
-        const float x = on ? a.lse[(long long)(s.q0 + tok) * a.Hq + head] : INFINITY;
-        ls[u] = x == -INFINITY ? INFINITY : x * kLog2e;
+        const char *qp = a.q + (long long)(s.q0 + t0 + (on ? r / a.G : 0)) * a.q_nbt +
+                         (long long)(g * a.G + (on ? r % a.G : 0)) * a.q_nbh;
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {
-            const int d = KVT == 1 ? kc * 16 + 2 * c : (kc >> 1) * 32 + (kc & 1) * 16 + 4 * c;
-            qa[kc][u] = on ? paged_q2(qp, a.q_f16, d) : 0u;
-            qa[kc][2 + u] = on ? paged_q2(qp, a.q_f16, d + (KVT == 1 ? 8 : 2)) : 0u;
+            const int d = paged_q_dim<KVT>(lane, kc);
+            qb[nc][kc][0] = on ? paged_q2(qp, a.q_f16, d) : 0u;
+            qb[nc][kc][1] = on ? paged_q2(qp, a.q_f16, d + (KVT == 1 ? 8 : 2)) : 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r2 = 8 * nc + 2 * c + i;
+            const bool on2 = r2 < rows;
+            const int tok = t0 + (on2 ? r2 / a.G : 0), head = g * a.G + (on2 ? r2 % a.G : 0);
+            hi[nc][i] = on2 ? (a.causal ? min(off + tok, limit - 1) : limit - 1) : -1;
+            lo[nc][i] = a.window > 0 ? off + tok - a.window + 1 : 0;
+            const float x = on2 ? a.lse[(long long)(s.q0 + tok) * a.Hq + head] : INFINITY;
+            ls[nc][i] = x == -INFINITY ? INFINITY : x * kLog2e;
         }
     }
-    // the value (key tile i, column j) that lanes 4v ... 4v + 3 write, v = 2i + j
-    const int v = lane >> 2, mine = KVT == 1 ? 8 * (v >> 1) + 2 * c + (v & 1) : 4 * c + 2 * (v & 1) + (v >> 1);
+    // lanes c = 0, 1 end up with the sums of their two keys
+    const int mine = paged_tile_key<KVT>(lane, c & 1);
     const long long base = ((long long)b * a.kv.Hkv + g) * a.row_cap;
     // tiles nobody sees come first and use no stage
     const int skip = min(nt, (lo_any >> 4) > first ? ((lo_any >> 4) - 1 - first) / 4 + 1 : 0);
@@ -255,7 +263,7 @@ kv_score_stream_kernel(const PagedScoreArgs a, const PagedSplit sp)
     // old scores of the next four tiles: their latency is a tile's whole time
     auto old_of = [&](int t) {
         const int key = 16 * (first + t * 4) + mine;
-        return t < nt && v < 4 && key < limit && a.decay != 0.f ? a.decay * a.score[base + key] : 0.f;
+        return t < nt && c < 2 && key < limit && a.decay != 0.f ? a.decay * a.score[base + key] : 0.f;
     };
     constexpr int U = 4;
     float old[U];
@@ -275,31 +283,22 @@ kv_score_stream_kernel(const PagedScoreArgs a, const PagedSplit sp)
                 ok = __all_sync(0xffffffffu,
                                 mbar_wait(&full[t % C::STAGES], ((t - skip) / C::STAGES) & 1, a.kv.err, VTX_KERR_KV));
                 if (!ok) break;
-                float x[2][4], w[4];
-                paged_tile_scores<D, KVT>(ring + (t % C::STAGES) * C::STAGE_BYTES, qa, x, lane);
+                float x[NC][4], w[2] = {0.f, 0.f};
+                paged_tile_scores<D, KVT, NC>(ring + (t % C::STAGES) * C::STAGE_BYTES, qb, x, lane);
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int k = k0 + (KVT == 1 ? 8 * i + 2 * c + j : 4 * c + 2 * j + i);
-                        float y = 0.f;
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            if (u == 1 && rows <= 8) break;     // uniform
-                            const float p = ex2(paged_logit_t<UF>(x[i][2 * u + j], cx, a.scale, a.softcap) - ls[u]);
-                            y += inner || (k >= lo[u] && k <= hi[u]) ? p : 0.f;
-                        }
-                        w[2 * i + j] = y;
+                    for (int i = 0; i < 4; ++i) {
+                        const int k = k0 + paged_tile_key<KVT>(lane, i >> 1);
+                        const float p = ex2(paged_logit_t<UF>(x[nc][i], cx, a.scale, a.softcap) - ls[nc][i & 1]);
+                        w[i >> 1] += inner || (k >= lo[nc][i & 1] && k <= hi[nc][i & 1]) ? p : 0.f;
                     }
-                // sum over the 8 row lanes, halving the values kept: lane v ends with value v & 3
-                const bool h1 = v & 2, h0 = v & 1;
-                const float a0 = (h1 ? w[2] : w[0]) + __shfl_xor_sync(0xffffffffu, h1 ? w[0] : w[2], 8);
-                const float a1 = (h1 ? w[3] : w[1]) + __shfl_xor_sync(0xffffffffu, h1 ? w[1] : w[3], 8);
-                sum = (h0 ? a1 : a0) + __shfl_xor_sync(0xffffffffu, h0 ? a0 : a1, 4);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                // over the lanes of the quad; lane c keeps key c & 1
+                sum = (c & 1 ? w[1] : w[0]) + __shfl_xor_sync(0xffffffffu, c & 1 ? w[0] : w[1], 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
                 __syncwarp();
             }
-            if (v < 4 && key < limit) a.score_out[base + key] = old[ui] + sum;
+            if (c < 2 && key < limit) a.score_out[base + key] = old[ui] + sum;
             old[ui] = old_of(t + U);
             issue(t + C::STAGES);
             done = t + 1;

@@ -343,27 +343,30 @@ int launch_score(const PagedScoreArgs &a, cudaStream_t st) {
 
 // Few query rows: the splits of the streaming attention kernel (whose K half
 // this is), without partials.
-template <int D, int KVT, bool UF>
+template <int D, int KVT, int ROWS, bool UF>
 int launch_score_stream_t(const PagedScoreArgs &a, const PagedSplit &sp, cudaStream_t st) {
     using C = ScoreStreamCfg<D, KVT>;
     static std::atomic<int> done[kMaxDevices];
-    int rc = allow_smem(kv_score_stream_kernel<D, KVT, UF>, C::SMEM, done);
+    int rc = allow_smem(kv_score_stream_kernel<D, KVT, ROWS, UF>, C::SMEM, done);
     if (rc != VTX_OK) return rc;
     const long long ctas = (long long)a.kv.n_seq * a.kv.Hkv * sp.n_splits;
     if (ctas > 0x7fffffffLL) return VTX_ERR_UNSUPPORTED;
-    return launch_pdl(kv_score_stream_kernel<D, KVT, UF>, dim3((unsigned)ctas), dim3(128), C::SMEM, st, a, sp);
+    return launch_pdl(kv_score_stream_kernel<D, KVT, ROWS, UF>, dim3((unsigned)ctas), dim3(128), C::SMEM, st, a, sp);
 }
 
 template <int D, int KVT>
-int launch_score_stream(const PagedScoreArgs &a, int sms, cudaStream_t st) {
+int launch_score_stream(const PagedScoreArgs &a, int rows, int sms, cudaStream_t st) {
     const long long base = (long long)a.kv.n_seq * a.kv.Hkv;
     const int tiles = std::max(1, (a.kv.max_kv + 15) / 16);
     PagedSplit sp{};
     const long long want = std::max<long long>((4LL * sms + base - 1) / base, (tiles + 63) / 64);
     sp.n_splits = (int)std::min<long long>(want, (tiles + 3) / 4);
     sp.tiles = (tiles + sp.n_splits - 1) / sp.n_splits;
-    return a.softcap != 0.0f ? launch_score_stream_t<D, KVT, true>(a, sp, st)
-                             : launch_score_stream_t<D, KVT, false>(a, sp, st);
+    if (a.softcap != 0.0f)
+        return rows <= 8 ? launch_score_stream_t<D, KVT, 8, true>(a, sp, st)
+                         : launch_score_stream_t<D, KVT, 16, true>(a, sp, st);
+    return rows <= 8 ? launch_score_stream_t<D, KVT, 8, false>(a, sp, st)
+                     : launch_score_stream_t<D, KVT, 16, false>(a, sp, st);
 }
 
 template <int D, int KVT, int NT, bool UF>
@@ -582,8 +585,9 @@ int vtx_kv_score_paged(const vtx_kv_score_paged_args *p, void *stream) {
     const bool f16 = kv->k.type == VTX_TYPE_F16, d64 = kv->k.ne[0] == 64;
     const long long rows = (long long)(p->observe > 0 ? std::min(p->observe, kv->max_new) : kv->max_new) * a.G;
     if (rows <= kFewRows) {
-        if (d64) return f16 ? launch_score_stream<64, 1>(a, ds->sms, st) : launch_score_stream<64, 8>(a, ds->sms, st);
-        return f16 ? launch_score_stream<128, 1>(a, ds->sms, st) : launch_score_stream<128, 8>(a, ds->sms, st);
+        const int r = (int)rows, n = ds->sms;
+        if (d64) return f16 ? launch_score_stream<64, 1>(a, r, n, st) : launch_score_stream<64, 8>(a, r, n, st);
+        return f16 ? launch_score_stream<128, 1>(a, r, n, st) : launch_score_stream<128, 8>(a, r, n, st);
     }
     if (a.q_f16) {
         CUtensorMap m[2];
