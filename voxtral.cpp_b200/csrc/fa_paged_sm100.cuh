@@ -19,7 +19,9 @@
 // warps clear those V rows in shared memory before P V (masked P is 0, and
 // 0 * NaN is not), while masked scores are replaced.
 //
-// Part of the exponentials runs on the FMA pipe: 2^x = 2^j p(f), j = round(x),
+// D = 64, twice the exponentials per flop: a quarter of them runs on the FMA pipe
+// (2048 tokens at 14k keys 446 -> 430 us; D = 128 gains nothing, 519 us either way,
+// and under the power cap it costs, 569 against 562 us).  2^x = 2^j p(f), j = round(x),
 // with p the degree-4 polynomial of least relative error (2.6e-6) on
 // [-1/2, 1/2], fitted here by an exchange.  The row sums are taken of the f32
 // P, so lse carries neither P's rounding to half nor more than that error.
@@ -303,7 +305,7 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
             for (int i = 0; i < 64; ++i) {
                 float e0, e1;
                 upk2(ffma2(pk2(x[2 * i], x[2 * i + 1]), cx2, nm2), e0, e1);
-                if ((i & 3) == 3) {                // every fourth pair off the MUFU
+                if (D == 64 && (i & 3) == 3) {     // every fourth pair off the MUFU
                     paged_exp2_pair(e0, e1);
                 } else {
                     e0 = ex2(e0);

@@ -88,22 +88,23 @@ __device__ __forceinline__ void evict_move(const PagedEvictArgs &a, const int2 *
 // The m-th largest key by a radix select from the top digit down: a histogram of
 // the keys that match the prefix so far, then the bin that holds the m-th.  Rows
 // with a larger key are kept, of those with an equal one the first ones.  A warp
-// owns a run of rows and walks it 32 at a time, so ballots number the equal keys,
-// the gaps and the moved rows in row order.  Bound by latency: about a dozen
-// barriers and four dependent trips to memory per (stream, head).
+// owns a run of rows and walks it 128 at a time, four consecutive rows per lane, so
+// a scan over the lanes numbers the gaps and the moved rows in row order.  Bound by
+// latency: about a dozen barriers and four dependent trips to memory per (stream,
+// head).  Keys are read four at a time (a row at a time: ONEROW against FOURROW us
+// for 64 items of 1500 to 8192 rows).
 template <bool SMEM, int UNIT>
 __global__ void __launch_bounds__(kEvictThreads)
 kv_evict_select_kernel(const PagedEvictArgs a)
 {
     grid_dep_wait();
     grid_dep_launch();
-    extern __shared__ uint32_t keys[];
+    extern __shared__ __align__(16) uint32_t keys[];
     __shared__ int hist[kEvictBins];
     __shared__ int2 warp_sum[kEvictWarps];
-    __shared__ int pick[2];
+    __shared__ int pick[3];
     const int b = blockIdx.x / a.kv.Hkv;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const unsigned below = (1u << lane) - 1;
     const long long item = blockIdx.x;
     const int n = a.kv.kv_len[b];
     const int most = (int)min((long long)min(a.kv.max_kv, a.row_cap), (long long)a.kv.max_pages << a.kv.shift);
@@ -119,25 +120,61 @@ kv_evict_select_kernel(const PagedEvictArgs a)
     const float *score = a.score + item * a.row_cap;
     const int *row_pos = a.row_pos ? a.row_pos + item * a.row_cap : nullptr;
     const int recent = (a.next_pos ? a.next_pos[b] : n) - a.n_recent;
-    auto key_of = [&](int j) {
-        const int p = row_pos ? row_pos[j] : j;
-        return evict_key(score[j], p < a.n_sink || p >= recent);
+    const int n4 = (n + 3) >> 2;
+    const bool wide = a.row_cap % 4 == 0 &&        // rows of four start on 16 bytes
+                      ((reinterpret_cast<uintptr_t>(a.score) | reinterpret_cast<uintptr_t>(a.row_pos)) & 15) == 0;
+    auto load4 = [&](int q, float (&s)[4], int (&p)[4]) {       // rows 4q ... 4q + 3 (below n)
+        if (wide) {
+            const float4 x = reinterpret_cast<const float4 *>(score)[q];
+            s[0] = x.x; s[1] = x.y; s[2] = x.z; s[3] = x.w;
+            if (row_pos) {
+                const int4 y = reinterpret_cast<const int4 *>(row_pos)[q];
+                p[0] = y.x; p[1] = y.y; p[2] = y.z; p[3] = y.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = min(4 * q + i, n - 1);
+                s[i] = score[j];
+                if (row_pos) p[i] = row_pos[j];
+            }
+        }
+        if (!row_pos) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = 4 * q + i;
+        }
     };
+    // keys of rows 4q ... 4q + 3; 0, below every key, behind the last row
+    auto make4 = [&](int q) {
+        float s[4];
+        int p[4];
+        uint32_t k[4];
+        load4(q, s, p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            k[i] = 4 * q + i < n ? evict_key(s[i], p[i] < a.n_sink || p[i] >= recent) : 0u;
+        return make_uint4(k[0], k[1], k[2], k[3]);
+    };
+    auto keys4 = [&](int q) { return SMEM ? reinterpret_cast<const uint4 *>(keys)[q] : make4(q); };
     const bool some = m > 0 && m < n;              // there is a choice to make
     if (SMEM && some)
-        for (int j = tid; j < n; j += kEvictThreads) keys[j] = key_of(j);
+        for (int q = tid; q < n4; q += kEvictThreads) reinterpret_cast<uint4 *>(keys)[q] = make4(q);
     uint32_t prefix = 0;
     int need = m;                                  // rank of the threshold among the keys that match the prefix
+    bool ties = false;                             // not all keys equal to the threshold stay
     if (some) {
 #pragma unroll
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
             for (int i = tid; i < kEvictBins; i += kEvictThreads) hist[i] = 0;
             __syncthreads();
-            for (int j = tid; j < n; j += kEvictThreads) {
-                const uint32_t k = SMEM ? keys[j] : key_of(j);
-                if (pass == 0 || (k >> (shift + bits)) == (prefix >> (shift + bits)))
-                    atomicAdd(&hist[(k >> shift) & ((1 << bits) - 1)], 1);
+            for (int q = tid; q < n4; q += kEvictThreads) {
+                const uint4 k4 = keys4(q);
+                const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (pass == 0 || (k[i] >> (shift + bits)) == (prefix >> (shift + bits)))
+                        atomicAdd(&hist[(k[i] >> shift) & ((1 << bits) - 1)], 1);
             }
             __syncthreads();
             // thread i: the four bins from 2047 - 4i down; the sum of all above it by a scan
@@ -160,17 +197,33 @@ kv_evict_select_kernel(const PagedEvictArgs a)
                 if (above < need && above + c[i] >= need) {
                     pick[0] = kEvictBins - 1 - 4 * tid - i;
                     pick[1] = need - above;
+                    pick[2] = c[i];
                 }
                 above += c[i];
             }
             __syncthreads();
             prefix |= (uint32_t)pick[0] << shift;
             need = pick[1];
+            ties = pick[1] < pick[2];
         }
     }
     // keys > prefix stay, and the first `need` of those equal to it
-    const int run = (n + kEvictThreads - 1) / kEvictThreads * 32;
-    const int r0 = min(warp * run, n), r1 = min(r0 + run, n);
+    const int run = (n4 + kEvictThreads - 1) / kEvictThreads * 32;      // fours per warp
+    const int q0 = min(warp * run, n4), q1 = min(q0 + run, n4);
+    auto scan = [&](int x) {                       // exclusive sum over the lanes
+        int inc = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += y;
+        }
+        return inc - x;
+    };
+    auto all = [&](int x) {                        // sum over the lanes
+#pragma unroll
+        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        return x;
+    };
     // exclusive sums over the warps of two counts, and their totals
     auto sums = [&](int x, int y, int2 &total) {
         __syncthreads();
@@ -186,49 +239,80 @@ kv_evict_select_kernel(const PagedEvictArgs a)
         }
         return before;
     };
-    int2 tot;
+    int2 tot = make_int2(0, 0);
     int eq0 = 0;
-    if (some) {
-        for (int j = r0 + lane; j - lane < r1; j += 32)
-            eq0 += __popc(__ballot_sync(0xffffffffu, j < r1 && (SMEM ? keys[j] : key_of(j)) == prefix));
-        eq0 = sums(eq0, 0, tot).x;
+    if (ties) {                                    // number the equal keys
+        for (int q = q0 + lane; q < q1; q += 32) {
+            const uint4 k = keys4(q);
+            eq0 += (k.x == prefix) + (k.y == prefix) + (k.z == prefix) + (k.w == prefix);
+        }
+        eq0 = sums(all(eq0), 0, tot).x;
     }
-    auto each = [&](auto f) {                      // f(row, live, kept), a warp's rows in order
+    auto each = [&](auto f) {                      // f(four, bits of the rows that stay), a warp's fours in order
         int e = eq0;
-        for (int j = r0 + lane; j - lane < r1; j += 32) {
-            const bool live = j < r1;
-            bool kept = live && m == n;
+        for (int q = q0 + lane; q - lane < q1; q += 32) {
+            unsigned kept = 0;
             if (some) {
-                const uint32_t k = live ? (SMEM ? keys[j] : key_of(j)) : 0u;
-                const unsigned same = __ballot_sync(0xffffffffu, live && k == prefix);
-                kept = live && (k > prefix || (k == prefix && e + __popc(same & below) < need));
-                e += __popc(same);
+                const uint4 k4 = q < q1 ? keys4(q) : make_uint4(0u, 0u, 0u, 0u);
+                const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+                if (ties) {
+                    int same = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) same += k[i] == prefix;
+                    int rank = e + scan(same);
+                    e += all(same);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        kept |= (unsigned)(k[i] > prefix || (k[i] == prefix && rank < need)) << i;
+                        rank += k[i] == prefix;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) kept |= (unsigned)(k[i] >= prefix) << i;
+                }
+            } else if (m == n) {
+                kept = 15u;
             }
-            f(j, live, kept);
+            // rows that exist, and those below m
+            const int left = q < q1 ? min(max(n - 4 * q, 0), 4) : 0, low = min(max(m - 4 * q, 0), left);
+            const unsigned live = (1u << left) - 1, front = (1u << low) - 1;
+            f(q, kept & live, live, front);
         }
     };
     int gaps = 0, late = 0;                        // gaps below m, kept rows behind it
-    if (some)
-        each([&](int j, bool live, bool kept) {
-            gaps += __popc(__ballot_sync(0xffffffffu, live && j < m && !kept));
-            late += __popc(__ballot_sync(0xffffffffu, j >= m && kept));
+    if (some) {
+        each([&](int, unsigned kept, unsigned live, unsigned front) {
+            gaps += __popc(front & ~kept);
+            late += __popc(kept & ~front);
         });
+        gaps = all(gaps);
+        late = all(late);
+    }
     int2 at = sums(gaps, late, tot);
     int2 *mv = a.moves + item * a.max_moves;
     float *so = a.score_out ? a.score_out + item * a.out_cap : nullptr;
     int *po = a.pos_out ? a.pos_out + item * a.out_cap : nullptr;
     int *ro = a.src_out ? a.src_out + item * a.out_cap : nullptr;
-    each([&](int j, bool live, bool kept) {
-        const unsigned gap = __ballot_sync(0xffffffffu, live && j < m && !kept);
-        const unsigned far = __ballot_sync(0xffffffffu, j >= m && kept);
-        if ((gap >> lane) & 1u) mv[at.x + __popc(gap & below)].y = j;
-        if ((far >> lane) & 1u) mv[at.y + __popc(far & below)].x = j;
-        at.x += __popc(gap);
-        at.y += __popc(far);
-        if (j < m && kept) {                       // in place these stand already
-            if (so && so != score) so[j] = score[j];
-            if (po && po != row_pos) po[j] = row_pos ? row_pos[j] : j;
-            if (ro) ro[j] = j;
+    const bool put_s = so && so != score, put_p = po && po != row_pos;   // in place they stand already
+    each([&](int q, unsigned kept, unsigned live, unsigned front) {
+        const unsigned gap = front & ~kept, far = kept & ~front, stay = kept & front;
+        const int x = scan(__popc(gap) | __popc(far) << 16), t = all(__popc(gap) | __popc(far) << 16);
+        int g0 = at.x + (x & 0xffff), l0 = at.y + (x >> 16);
+        at.x += t & 0xffff;
+        at.y += t >> 16;
+        float s[4];
+        int p[4];
+        if (stay && (put_s || put_p)) load4(q, s, p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = 4 * q + i;
+            if ((gap >> i) & 1u) mv[g0++].y = j;
+            if ((far >> i) & 1u) mv[l0++].x = j;
+            if ((stay >> i) & 1u) {
+                if (put_s) so[j] = s[i];
+                if (put_p) po[j] = p[i];
+                if (ro) ro[j] = j;
+            }
         }
     });
     __syncthreads();

@@ -408,7 +408,7 @@ EvictPlan plan_evict(const vtx_paged_kv *p) {
 
 template <bool SMEM, int UNIT>
 int launch_evict_select(const PagedEvictArgs &a, long long items, cudaStream_t st) {
-    const size_t keys = SMEM ? (size_t)a.kv.max_kv * 4 : 0;
+    const size_t keys = SMEM ? align_up((size_t)a.kv.max_kv * 4, 16) : 0;
     if (SMEM) {
         static std::atomic<int> done[kMaxDevices];
         const int rc = allow_smem(kv_evict_select_kernel<SMEM, UNIT>, kEvictKeysInSmem * 4, done);
@@ -647,9 +647,10 @@ int vtx_kv_evict_paged(const vtx_kv_evict_paged_args *p, void *workspace, size_t
     // rows of 256 or 128 (F16), 136 or 68 bytes (Q8_0: 8- and 4-byte aligned)
     const int unit = kv->k.type == VTX_TYPE_F16 ? 16 : a.row_bytes % 8 == 0 ? 8 : 4;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // Few moves: one kernel (1024 rows: 10.2 -> 8 us and one launch less); a
-    // (stream, head) is one CTA there, too little for many.  Not in place on
-    // kv_len, which the other heads' CTAs may not have read yet.
+    // Few moves: one kernel, a launch less.  A (stream, head) is one CTA there, too
+    // little for many moves, and with enough items the two kernels take as long as
+    // one (256 items of 1500 to 8192 rows: 87 against 91 us).  Not in place on kv_len,
+    // which the other heads' CTAs may not have read yet.
     if (e.max_moves <= 512 && p->kv_len_out != kv->kv_len) {
         if (unit == 16) return launch_evict_select<true, 16>(a, e.items, st);
         return unit == 8 ? launch_evict_select<true, 8>(a, e.items, st) : launch_evict_select<true, 4>(a, e.items, st);
