@@ -407,6 +407,8 @@ VTX_API int vtx_attn_out_proj(const vtx_out_proj_args *args, void *stream);
  *   size grids and workspaces.  A stream above a bound is reported and what
  *   exceeds it is not served (but see vtx_flash_attn_paged, which serves a
  *   longer kv_len exactly in most cases).
+ * Reports: vtx_read_device_error gives 40 for a table entry outside the pool, 41
+ * for a length above its bound.
  * page_table, kv_len and q_start are device memory, read by the kernels only:
  * a captured call may be replayed after they changed within the bounds. */
 typedef struct vtx_paged_kv {
@@ -460,7 +462,10 @@ VTX_API int vtx_kv_append_paged(const vtx_kv_append_paged_args *args, void *stre
  * additionally j > kv_len - n + i - W; rows of an evicted cache are not
  * positions, so a window does not fit there).  max_bias must be 0.
  * Hq / Hkv <= 16; base and strides of q and dst multiples of 16 bytes.
- * Rows at or behind kv_len may hold anything, NaN included.
+ * Rows at or behind kv_len, and rows that no token of the stream sees, may hold
+ * anything, NaN included; a row that some token sees and that is not finite in
+ * V may also spoil tokens of its stream that do not see it.  dst must not
+ * overlap q.
  * Rounded to half: P, a F32 q, V of a Q8_0 cache where a stream brings more
  * than 16 query rows (tokens * Hq / Hkv) per KV head, and K there too when
  * max_kv_len >= 1024 (such caches are unpacked into the workspace, and a

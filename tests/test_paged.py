@@ -73,6 +73,7 @@ BAD_CACHES = [
     (dict(k_data=0), -1), (dict(k_data=0x10008), -4), (dict(k_nb3=8 * 16 * 256 + 8, v_nb3=8 * 16 * 256 + 8), -4),
     (dict(k_nb1=264, v_nb1=264), -4), (dict(v_nb2=16 * 256 + 16), -4), (dict(k_nb1=128, v_nb1=128), -4),
     (dict(kv_type=V.Q8_0, k_nb1=144, v_nb1=144), -4),
+    (dict(k_nb3=0, v_nb3=0), -4), (dict(k_nb2=0, v_nb2=0), -4),
     (dict(v_ne3=9), -3), (dict(k_ne2=0, v_ne2=0), -3), (dict(n_seq=-1), -3), (dict(max_kv_len=65), -3),
     (dict(max_new=3), -3), (dict(n_tokens=-1), -3), (dict(max_pages=-1), -3), (dict(kv_len=0), -1), (dict(page_table=0), -1),
 ]
@@ -504,6 +505,122 @@ def test_score(i):
         bad = live & ~(np.abs(got - want) <= tol)
         assert not bad.any(), f"{SCORE[i]}: {bad.sum()} of {live.sum()}, worst {np.abs(got - want)[live].max()}"
     assert V.read_device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_type", ["f16", "q8_0"])
+@pytest.mark.parametrize("streams", [[(2, 50), (1, 9)], [(80, 500), (1, 33)]])
+def test_score_f32_strided_q(kv_type, streams):
+    c = R.build(14, kv_type, streams)
+    lse = R.attend(c)[1].astype(np.float32)
+    want, tol = R.score(c, lse, np.zeros((2, 2, 512)), 512)
+    kv = device_kv(c)
+    T, Hq, D = c["q"].shape
+    wide = torch.randn(T, Hq, 2, D, device="cuda")
+    wide[:, :, 1] = torch.from_numpy(c["q"]).cuda().float()
+    for q in (wide[:, :, 1], wide.half()[:, :, 1]):
+        got = torch.zeros(2, 2, 512, device="cuda")
+        kv.score(q, torch.from_numpy(lse).cuda(), got)
+        assert (np.abs(got.cpu().numpy() - want) <= tol).all()
+
+
+@pytest.mark.gpu
+def test_append_rows_aligned_to_eight_bytes():
+    """Token strides and bases of 8 bytes: the same bits as 16-byte aligned rows."""
+    for kv_type, D in (("f16", 128), ("q8_0", 128), ("f16", 64), ("q8_0", 64)):
+        c = R.build(15, kv_type, [(3, 40), (1, 7)], 8, 2, D, poison=False)
+        rng = np.random.default_rng(2)
+        x = {h: torch.from_numpy(rng.standard_normal((4, h * D)).astype(np.float32)).cuda() for h in (8, 2)}
+        pos = torch.tensor([5, 6, 7, 900], dtype=torch.int32, device="cuda")
+        got = []
+        for pad in (0, 2):
+            kv = device_kv(c)
+            wide = {h: torch.zeros(4, v.shape[1] + 2 * pad, device="cuda") for h, v in x.items()}
+            view = {}
+            for h, v in x.items():
+                wide[h][:, pad:pad + v.shape[1]] = v
+                view[h] = wide[h][:, pad:pad + v.shape[1]].unflatten(1, (h, D))
+            out = torch.zeros(4, 8 * D + 2 * pad, device="cuda")[:, pad:pad + 8 * D].unflatten(1, (8, D))
+            half = torch.zeros(4, 8 * D + 4 * pad, dtype=torch.float16, device="cuda")[:, 2 * pad:2 * pad + 8 * D].unflatten(1, (8, D))
+            kv.append(view[2], view[2], pos, q=view[8], q_out=out)
+            kv.append(view[2], view[2], pos, q=view[8], q_out=half)
+            got.append((kv.k_pool.clone(), kv.v_pool.clone(), out.clone(), half.clone()))
+        for a, b in zip(*got):
+            assert torch.equal(a, b)
+    # rotated in place
+    kv = device_kv(c)
+    q = view[8].clone()
+    kv.append(view[2], view[2], pos, q=q, q_out=q)
+    assert torch.equal(q, got[0][2])
+
+
+@pytest.mark.gpu
+def test_unpacked_cache_past_its_bound():
+    """A chunk over a Q8_0 cache that is unpacked: lengths up to whole pages above
+    max_kv_len are served, longer ones reported."""
+    c = R.build(16, "q8_0", [(40, 1100)])
+    q = torch.from_numpy(c["q"]).cuda()
+    check_attend(c, device_kv(c, max_kv_len=1030).attend(q), None, R.attend(c))
+    assert V.read_device_error() == 0
+    c = R.build(17, "q8_0", [(40, 1500)])
+    device_kv(c, max_kv_len=1030).attend(q)
+    assert V.read_device_error() == 41
+
+
+@pytest.mark.gpu
+def test_many_streams_and_none():
+    """More streams than a search step holds, most without tokens; and no stream at all."""
+    rng = np.random.default_rng(0)
+    streams = [(int(n), int(n + k)) for n, k in zip(rng.choice([0, 0, 0, 1, 2, 9], 150), rng.integers(0, 60, 150))]
+    c = R.build(18, "f16", streams, 4, 1, 64)
+    kv = device_kv(c)
+    q = torch.from_numpy(c["q"]).cuda()
+    lse = torch.empty(q.shape[:2], device="cuda")
+    ref = R.attend(c)
+    check_attend(c, kv.attend(q, lse=lse), lse, ref)
+    T = q.shape[0]
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    rows = torch.zeros(150, 1, max(c["len"]), dtype=torch.int32, device="cuda") - 1
+    kv.append(torch.randn(T, 1, 64, device="cuda"), torch.randn(T, 1, 64, device="cuda"), pos, row_pos=rows)
+    want = np.full(rows.shape, -1)
+    for s, n in enumerate(c["len"]):
+        new = c["start"][s + 1] - c["start"][s]
+        want[s, 0, n - new:n] = np.arange(c["start"][s], c["start"][s + 1])
+    assert np.array_equal(rows.cpu().numpy(), want) and V.read_device_error() == 0
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    none = V.PagedKv(kv.k_pool, kv.v_pool, i32(0, 1), i32(0), i32(1), 4, n_tokens=0, max_new=0)
+    assert none.attend(q[:0]).shape == (0, 4, 64)
+    none.append(torch.zeros(0, 1, 64, device="cuda"), torch.zeros(0, 1, 64, device="cuda"), i32(0))
+    none.score(q[:0], lse[:0], torch.zeros(0, 1, 16, device="cuda"))
+    none.evict(torch.zeros(0, 1, 16, device="cuda"), 8)
+
+
+@pytest.mark.gpu
+def test_score_of_streams_without_tokens_only_decays():
+    c = R.build(19, "f16", [(0, 30), (0, 0), (0, 17)])
+    kv = device_kv(c, n_tokens=0, max_new=0)
+    a = torch.rand(3, 2, 32, device="cuda")
+    b = kv.score(torch.zeros(0, 8, 128, dtype=torch.float16, device="cuda"), torch.zeros(0, 8, device="cuda"), a,
+                 score_out=torch.full_like(a, -1.0), decay=0.5)
+    for s, n in enumerate(c["len"]):
+        assert torch.equal(b[s, :, :n], a[s, :, :n] * 0.5) and (b[s, :, n:] == -1).all()
+
+
+@pytest.mark.gpu
+def test_calls_on_streams_of_their_own():
+    """Two caches worked on from two streams at once, repeatedly: each as alone."""
+    cases = [R.build(20, "f16", [(1, 1500), (1, 700), (30, 600)], 8, 2), R.build(21, "q8_0", [(1, 1800), (1, 40)], 8, 2)]
+    kvs, qs = [device_kv(c) for c in cases], [torch.from_numpy(c["q"]).cuda() for c in cases]
+    alone = [kv.attend(q) for kv, q in zip(kvs, qs)]
+    side = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    outs = [[torch.empty_like(a) for _ in range(20)] for a in alone]
+    for i in range(20):
+        for kv, q, s, o in zip(kvs, qs, side, outs):
+            kv.attend(q, out=o[i], stream=s)
+    torch.cuda.synchronize()
+    for a, o in zip(alone, outs):
+        assert all(torch.equal(a, x) for x in o)
 
 
 def run_evict(c, sc, keep, in_place=False, row_pos=None, next_pos=None, **kw):

@@ -1,17 +1,21 @@
-// fa_paged.cuh — attention of ragged chunks of new tokens over a paged cache
-// with mma.sync, any shape: the decoder node of src/voxtral.cpp:1802 over pages.
+// fa_paged.cuh — attention of ragged chunks of new tokens over a paged cache: what
+// its kernels share, and the one for chunks over short Q8_0 caches (mma.sync): the
+// decoder node of src/voxtral.cpp:1802 over pages.
 //
 //   x_ij = scale * q_i . k_j  (softcap c: c * tanh(x / c)),  j visible to i
 //   O_i  = sum_j e^(x_ij - m_i) v_j / sum_j e^(x_ij - m_i)
 //
-// in one pass over the keys with the running maximum m and sum l of each row
-// in registers.  A CTA owns 64 query rows (row = token * G + head of the group,
-// so every K/V row is read once for the whole group) of one KV head: 4 warps of
-// 16 rows, tiles of 32 keys in shared memory.  F16 rows as they are.  Q8_0: K
-// as its integers (exact halves) with each block's scale applied to that
-// block's f32 sum, so scores and lse carry no rounding of K; V as d * q rounded
-// to half, like P.  It serves chunks over Q8_0 caches that are short; longer ones
-// are unpacked to F16 pages for the tensor-core kernel (paged_unpack_kernel).
+// in one pass over the keys with the running maximum m and sum l of each row in
+// registers.  Four kernels: few query rows per stream, bound by HBM
+// (fa_paged_decode.cuh); chunks over F16 pages on the tensor core
+// (fa_paged_sm100.cuh); chunks over long Q8_0 caches, unpacked to F16 pages first
+// (paged_unpack_kernel) for the same kernel; and here chunks over Q8_0 caches below
+// 1024 rows, where rounding K would show in lse.  A CTA owns 64 query rows (row =
+// token * G + head of the group, so every K/V row is read once for the whole group)
+// of one KV head: 4 warps of 16 rows, tiles of 32 keys in shared memory.  K as its
+// integers (exact halves) with each block's scale applied to that block's f32 sum,
+// so scores and lse carry no rounding of K; V as d * q rounded to half, like P.
+// Loads are not overlapped with the products: 64 rows x 900 keys are a few us.
 #pragma once
 #include <cuda_fp16.h>
 #include <cstdint>
@@ -89,16 +93,16 @@ __device__ __forceinline__ void paged_store2(const PagedAttnArgs &a, int tok, in
 
 constexpr float kLn2 = 0.6931471805599453f;
 
-template <int D, int KVT>
+template <int D>
 __global__ void __launch_bounds__(128)
-fa_paged_kernel(const PagedAttnArgs a)
+fa_paged_q8_kernel(const PagedAttnArgs a)
 {
     grid_dep_wait();
     grid_dep_launch();
     constexpr int KEYS = 32, P = D + 8, KC = D / 16, NB = D / 8;
     __shared__ __align__(16) __half ks[KEYS * P];
     __shared__ __align__(16) __half vs[KEYS * P];
-    __shared__ float kd[KVT == 8 ? D / 32 : 1][KEYS];       // Q8_0: scales of K
+    __shared__ float kd[D / 32][KEYS];                      // scales of K
     const int b = blockIdx.z, g = blockIdx.y;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const PagedSeq s = paged_seq(a.kv, b);
@@ -146,9 +150,9 @@ fa_paged_kernel(const PagedAttnArgs a)
             uint4 kx = make_uint4(0u, 0u, 0u, 0u), vx = kx;
             if (k0 + r >= k_lo && k0 + r <= k_hi) {         // other rows may hold anything: zeros instead
                 const long long at = paged_row(a.kv, b, k0 + r, g);
-                kx = paged_load8<KVT>(a.kv.k + at, c, 1.0f);
-                vx = paged_load8<KVT>(a.kv.v + at, c, KVT == 8 ? q8_scale(a.kv.v + at, c) : 1.0f);
-                if (KVT == 8 && (c & 31) == 0) kd[c >> 5][r] = q8_scale(a.kv.k + at, c);
+                kx = paged_load8<8>(a.kv.k + at, c, 1.0f);
+                vx = paged_load8<8>(a.kv.v + at, c, q8_scale(a.kv.v + at, c));
+                if ((c & 31) == 0) kd[c >> 5][r] = q8_scale(a.kv.k + at, c);
             }
             *reinterpret_cast<uint4 *>(ks + r * P + c) = kx;
             *reinterpret_cast<uint4 *>(vs + r * P + c) = vx;
@@ -162,17 +166,13 @@ fa_paged_kernel(const PagedAttnArgs a)
             for (int kc = 0; kc < KC; kc += 2) {
                 uint32_t bk[4];
                 ldsm_x4(bk, ks + (nt * 8 + lrow) * P + kc * 16 + lmat * 8);
-                if constexpr (KVT == 1) {
-                    mma16816(x[nt], qa[kc], bk[0], bk[1]);
-                    mma16816(x[nt], qa[kc + 1], bk[2], bk[3]);
-                } else {                                    // a block of 32 dims, then its scale
-                    float y[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma16816(y, qa[kc], bk[0], bk[1]);
-                    mma16816(y, qa[kc + 1], bk[2], bk[3]);
-                    const float2 d = *reinterpret_cast<const float2 *>(&kd[kc / 2][nt * 8 + 2 * (lane & 3)]);
+                // a block of 32 dims, then its scale
+                float y[4] = {0.f, 0.f, 0.f, 0.f};
+                mma16816(y, qa[kc], bk[0], bk[1]);
+                mma16816(y, qa[kc + 1], bk[2], bk[3]);
+                const float2 d = *reinterpret_cast<const float2 *>(&kd[kc / 2][nt * 8 + 2 * (lane & 3)]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[nt][i] = fmaf(i & 1 ? d.y : d.x, y[i], x[nt][i]);
-                }
+                for (int i = 0; i < 4; ++i) x[nt][i] = fmaf(i & 1 ? d.y : d.x, y[i], x[nt][i]);
             }
         }
         float mx[2] = {-INFINITY, -INFINITY};

@@ -160,8 +160,9 @@ __device__ __forceinline__ void store_8(void *dst, bool f16, const float (&x)[8]
 // HBM-bound by its bytes: (Hq + 2 Hkv) * D * 4 read and Hq * D * (2 or 4) + 2 Hkv *
 // row bytes written per token.  The way to a row's page (stream of the token, its
 // lengths, the table) is three dependent trips to memory, so a warp loads its first
-// rows before it takes them.  A whole warp per row issued 5900 instructions per
-// token and was bound by them (7639 tokens, Q8_0: 64 us against APPEND_US).
+// rows before it takes them.  7639 tokens, 32 + 2 x 8 heads of 128: 50 us into F16
+// pages (5.6 TB/s), 54 us into Q8_0 (4.9 TB/s); with a whole warp per row the
+// instructions were the bound (5900 warp instructions per token, Q8_0 64 us).
 // Angle of pair i: pos * turns[i] turns, reduced to (-1/2, 1/2] in double (three
 // operations), then sincospi in float: an error of about 1e-7 at any position.
 template <int D, bool W16>

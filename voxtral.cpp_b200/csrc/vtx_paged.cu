@@ -30,7 +30,7 @@ constexpr int kMaxGroup = 16;             // query heads per KV head
 
 int check_pool(const vtx_tensor &t, int row) {
     if (!t.data) return VTX_ERR_NULL;
-    if (t.nb[1] < (size_t)row) return VTX_ERR_STRIDE;
+    if (t.nb[1] < (size_t)row || (t.ne[2] > 1 && !t.nb[2]) || (t.ne[3] > 1 && !t.nb[3])) return VTX_ERR_STRIDE;
     if (reinterpret_cast<uintptr_t>(t.data) % 16 || t.nb[2] % 16 || t.nb[3] % 16) return VTX_ERR_STRIDE;
     if (t.type == VTX_TYPE_Q8_0) return t.nb[0] == 34 && t.nb[1] == (size_t)row ? VTX_OK : VTX_ERR_STRIDE;
     return t.nb[0] == 2 && t.nb[1] % 16 == 0 ? VTX_OK : VTX_ERR_STRIDE;
@@ -174,10 +174,10 @@ int launch_decode_rows(const PagedAttnArgs &a, const DecodePlan &d, cudaStream_t
                        : launch_decode<D, KVT, 16, false>(a, d.split, st);
 }
 
-template <int D, int KVT>
-int launch_attn(const PagedAttnArgs &a, cudaStream_t st) {
+template <int D>
+int launch_attn_q8(const PagedAttnArgs &a, cudaStream_t st) {
     const long long tiles = ((long long)a.kv.max_new * a.G + 63) / 64;
-    return launch_pdl(fa_paged_kernel<D, KVT>, dim3((unsigned)tiles, (unsigned)a.kv.Hkv, (unsigned)a.kv.n_seq),
+    return launch_pdl(fa_paged_q8_kernel<D>, dim3((unsigned)tiles, (unsigned)a.kv.Hkv, (unsigned)a.kv.n_seq),
                       dim3(128), 0, st, a);
 }
 
@@ -280,8 +280,9 @@ PagedView unpacked_view(const PagedView &kv, const TilePlan &t, int D, char *ws)
 
 template <int D>
 int launch_unpack(const PagedAttnArgs &a, const PagedView &out, cudaStream_t st) {
-    return launch_pdl(paged_unpack_kernel<D>, dim3((unsigned)((a.kv.max_kv + 31) / 32), (unsigned)a.kv.Hkv,
-                                                   (unsigned)a.kv.n_seq), dim3(128), 0, st, a, out);
+    return launch_pdl(paged_unpack_kernel<D>,
+                      dim3((unsigned)(out.max_pages * (kUnpackPage / 32)), (unsigned)a.kv.Hkv, (unsigned)a.kv.n_seq),
+                      dim3(128), 0, st, a, out);
 }
 
 // Map of an F16 pool: (dim, row, head, page), boxes of 64 dims x min(page, 128) rows.
@@ -540,7 +541,7 @@ int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, si
         if (d64) rc = uf ? launch_tile<64, true>(m, ta, tp.tile, st) : launch_tile<64, false>(m, ta, tp.tile, st);
         else rc = uf ? launch_tile<128, true>(m, ta, tp.tile, st) : launch_tile<128, false>(m, ta, tp.tile, st);
     } else if (kv->max_new * (long long)a.G > a.min_rows) {
-        rc = d64 ? launch_attn<64, 8>(a, st) : launch_attn<128, 8>(a, st);
+        rc = d64 ? launch_attn_q8<64>(a, st) : launch_attn_q8<128>(a, st);
     }
     if (rc != VTX_OK) return rc;
     if (dp.use) {

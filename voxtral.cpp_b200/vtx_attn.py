@@ -447,9 +447,11 @@ class PagedKv:
     int32 (n_seq, max_pages), kv_len: int32 (n_seq,), q_start: int32
     (n_seq + 1,), contiguous on the pools' device: the kernels read them, so
     they may change between calls (and between replays of a captured call)
-    within n_tokens, max_new and max_kv_len (default: the table's capacity).
-    Workspaces are made here once; calls on one PagedKv must not overlap on
-    the GPU.  Inputs and outputs stay the caller's and are not copied."""
+    within n_tokens, max_new and max_kv_len (default: the table's capacity; the
+    tighter it is, the better the work is cut).  Workspaces are made here once
+    (with a synchronisation, so outside of captures); calls on one PagedKv must
+    not overlap on the GPU, and it must live until they are done.  Inputs and
+    outputs stay the caller's and are not copied."""
 
     def __init__(self, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor,
                  q_start: torch.Tensor, n_head_q: int, *, n_tokens: int, max_new: int,
@@ -476,13 +478,16 @@ class PagedKv:
         self.c = c
         self.max_kv_len = c.max_kv_len
         self._lib = load()
-        need = [self._lib.vtx_flash_attn_paged_workspace(ctypes.byref(c), n_head_q),
-                self._lib.vtx_kv_evict_paged_workspace(ctypes.byref(c))]
+        with torch.cuda.device(self.dev if self.dev.type == "cuda" else -1):     # plans follow the device's SMs
+            need = [self._lib.vtx_flash_attn_paged_workspace(ctypes.byref(c), n_head_q),
+                    self._lib.vtx_kv_evict_paged_workspace(ctypes.byref(c))]
         if ctypes.c_size_t(-1).value in need:
             raise VtxError(-3, "paged cache rejected")
         # attention's holds arrival counters: zero once, left zeroed by every call
         self.workspace = torch.zeros(max(need[0], 256), dtype=torch.uint8, device=self.dev)
         self.evict_workspace = torch.empty(max(need[1], 256), dtype=torch.uint8, device=self.dev)
+        if self.dev.type == "cuda":                 # the first call may be on another stream
+            torch.cuda.current_stream(self.dev).synchronize()
         self._ws, self._evict_ws = ((w.data_ptr(), w.numel()) for w in (self.workspace, self.evict_workspace))
         # argument blocks, made once: a call only sets its tensors
         self._q_shape = (n_tokens, n_head_q, self.head_dim)
