@@ -466,11 +466,13 @@ VTX_API int vtx_kv_append_paged(const vtx_kv_append_paged_args *args, void *stre
  * anything, NaN included; a row that some token sees and that is not finite in
  * V may also spoil tokens of its stream that do not see it.  dst must not
  * overlap q.
- * Rounded to half: P, a F32 q, V of a Q8_0 cache where a stream brings more
- * than 16 query rows (tokens * Hq / Hkv) per KV head, and K there too when
- * max_kv_len >= 1024 (such caches are unpacked into the workspace, and a
- * kv_len above max_kv_len is reported).  Everything else is F32.  A Q8_0
- * scale of V above 1023 overflows.
+ * Rounded to half: P (times the scale of V for a Q8_0 cache) and a F32 q.
+ * Everything else is F32, the values of a Q8_0 cache included.  Its scales may
+ * reach 511 (larger ones overflow a half); below 2^-14 those of V cost bits of
+ * P.  A Q8_0 cache with max_kv_len >= 96 of which a stream may bring more than
+ * 16 query rows (max_new * Hq / Hkv) per KV head is unpacked into the workspace
+ * (4 bytes per value, n_seq * max_kv_len rows; not above 4 GiB), and a kv_len
+ * above max_kv_len is then reported.
  * workspace: 256-byte aligned, vtx_flash_attn_paged_workspace bytes (they
  * depend on kv's sizes and bounds and on n_head_q alone).  Zero it once before
  * its first call (cudaMemset): it holds arrival counters, which every call

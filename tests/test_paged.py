@@ -555,6 +555,39 @@ def test_append_rows_aligned_to_eight_bytes():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("streams,D,kw,opt", [
+    ([(30, 90), (1, 60), (17, 17)], 128, {}, {}),                            # short: the pages as they are
+    ([(95, 95)], 64, {}, dict(softcap=4.0)),
+    ([(33, 96), (1, 900), (129, 1401)], 128, {}, {}),                        # unpacked
+    ([(200, 777), (5, 5), (0, 40)], 64, {}, dict(window=100)),
+    ([(70, 640)], 128, {}, dict(softcap=4.0)),
+    ([(70, 640)], 64, {}, dict(causal=False)),
+    ([(140, 700), (1, 300)], 128, dict(max_kv_len=1 << 21), {}),             # too large a copy for the bound
+    ([(140, 700), (1, 300)], 64, dict(max_kv_len=1 << 22), {}),
+])
+def test_attend_q8_chunks_round_p_alone(streams, D, kw, opt):
+    """Chunks over Q8_0 caches: neither K nor V is rounded, only P (in the short
+    form P times 64 times V's scale, whose subnormals cost up to 2^-25 / 64 of a
+    scale, 2 |v| for scales of 1/64 and more)."""
+    c = R.build(31, "q8_0", streams, 8, 2, D, 16)
+    if kw:                                                  # as many pages as the bound asks for
+        wide = np.zeros((len(streams), kw["max_kv_len"] // 16), np.int32)
+        wide[:, :c["table"].shape[1]] = c["table"]
+        c["table"] = wide
+    q = torch.from_numpy(c["q"]).cuda()
+    lse = torch.empty(q.shape[:2], device="cuda")
+    kv = device_kv(c, **kw)
+    ref = R.attend(c, **opt)
+    tol, ltol = R.attend_tolerance(ref, 1)
+    named = {("logit_softcap" if k == "softcap" else k): v for k, v in opt.items()}
+    out = kv.attend(q, lse=lse, out=torch.empty_like(q, dtype=torch.float32), **named).double().cpu().numpy()
+    assert (np.abs(out - ref[0]) <= tol + ref[4] * 2.0 ** -24).all()
+    fin = np.isfinite(ref[1])
+    assert (np.abs(lse.cpu().numpy()[fin] - ref[1][fin]) <= ltol[fin]).all()
+    assert V.read_device_error() == 0
+
+
+@pytest.mark.gpu
 def test_unpacked_cache_past_its_bound():
     """A chunk over a Q8_0 cache that is unpacked: lengths up to whole pages above
     max_kv_len are served, longer ones reported."""

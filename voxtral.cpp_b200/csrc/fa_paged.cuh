@@ -6,16 +6,16 @@
 //   O_i  = sum_j e^(x_ij - m_i) v_j / sum_j e^(x_ij - m_i)
 //
 // in one pass over the keys with the running maximum m and sum l of each row in
-// registers.  Four kernels: few query rows per stream, bound by HBM
-// (fa_paged_decode.cuh); chunks over F16 pages on the tensor core
-// (fa_paged_sm100.cuh); chunks over long Q8_0 caches, unpacked to F16 pages first
-// (paged_unpack_kernel) for the same kernel; and here chunks over Q8_0 caches below
-// 1024 rows, where rounding K would show in lse.  A CTA owns 64 query rows (row =
-// token * G + head of the group, so every K/V row is read once for the whole group)
-// of one KV head: 4 warps of 16 rows, tiles of 32 keys in shared memory.  K as its
-// integers (exact halves) with each block's scale applied to that block's f32 sum,
-// so scores and lse carry no rounding of K; V as d * q rounded to half, like P.
-// Loads are not overlapped with the products: 64 rows x 900 keys are a few us.
+// registers.  Three kernels: few query rows per stream, bound by HBM
+// (fa_paged_decode.cuh); chunks on the tensor core (fa_paged_sm100.cuh), over F16
+// pages or over Q8_0 ones that paged_unpack_kernel has split into pairs of halves;
+// and here chunks over short Q8_0 caches.  A CTA owns 64 query rows (row = token * G
+// + head of the group, so every K/V row is read once for the whole group) of one KV
+// head: 4 warps of 16 rows, tiles of 32 keys in shared memory.  K and V as their
+// integers (exact halves): K's scales are applied to each block's f32 sum, V's to P
+// before its one rounding to half, 64-fold so that a small scale keeps P out of the
+// subnormals.  So only P (and a F32 q) is rounded.  Loads are not overlapped with
+// the products: over 95 keys there is little to overlap.
 #pragma once
 #include <cuda_fp16.h>
 #include <cstdint>
@@ -102,7 +102,7 @@ fa_paged_q8_kernel(const PagedAttnArgs a)
     constexpr int KEYS = 32, P = D + 8, KC = D / 16, NB = D / 8;
     __shared__ __align__(16) __half ks[KEYS * P];
     __shared__ __align__(16) __half vs[KEYS * P];
-    __shared__ float kd[D / 32][KEYS];                      // scales of K
+    __shared__ float kd[D / 32][KEYS], vd[D / 32][KEYS];    // scales of K, 64 times V's
     const int b = blockIdx.z, g = blockIdx.y;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const PagedSeq s = paged_seq(a.kv, b);
@@ -151,8 +151,13 @@ fa_paged_q8_kernel(const PagedAttnArgs a)
             if (k0 + r >= k_lo && k0 + r <= k_hi) {         // other rows may hold anything: zeros instead
                 const long long at = paged_row(a.kv, b, k0 + r, g);
                 kx = paged_load8<8>(a.kv.k + at, c, 1.0f);
-                vx = paged_load8<8>(a.kv.v + at, c, q8_scale(a.kv.v + at, c));
-                if ((c & 31) == 0) kd[c >> 5][r] = q8_scale(a.kv.k + at, c);
+                vx = paged_load8<8>(a.kv.v + at, c, 1.0f);
+            }
+            if ((c & 31) == 0) {
+                const bool in = k0 + r >= k_lo && k0 + r <= k_hi;
+                const long long at = in ? paged_row(a.kv, b, k0 + r, g) : 0;
+                kd[c >> 5][r] = in ? q8_scale(a.kv.k + at, c) : 0.f;
+                vd[c >> 5][r] = in ? 64.0f * q8_scale(a.kv.v + at, c) : 0.f;
             }
             *reinterpret_cast<uint4 *>(ks + r * P + c) = kx;
             *reinterpret_cast<uint4 *>(vs + r * P + c) = vx;
@@ -197,24 +202,32 @@ fa_paged_q8_kernel(const PagedAttnArgs a)
 #pragma unroll
             for (int i = 0; i < NB; ++i) { o[i][2 * u] *= al; o[i][2 * u + 1] *= al; }
         }
-        uint32_t pa[KEYS / 16][4];
 #pragma unroll
         for (int nt = 0; nt < KEYS / 8; ++nt) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[nt][i] = ex2(x[nt][i] - mu[i >> 1]);
             l[0] += x[nt][0] + x[nt][1];
             l[1] += x[nt][2] + x[nt][3];
-            pa[nt / 2][(nt & 1) * 2] = pack_half2(x[nt][0], x[nt][1]);
-            pa[nt / 2][(nt & 1) * 2 + 1] = pack_half2(x[nt][2], x[nt][3]);
         }
 #pragma unroll
         for (int kk = 0; kk < KEYS / 16; ++kk)
 #pragma unroll
-            for (int nb = 0; nb < NB; nb += 2) {
-                uint32_t bv[4];
-                ldsm_x4_t(bv, vs + (kk * 16 + (lmat & 1) * 8 + lrow) * P + nb * 8 + (lmat >> 1) * 8);
-                mma16816(o[nb], pa[kk], bv[0], bv[1]);
-                mma16816(o[nb + 1], pa[kk], bv[2], bv[3]);
+            for (int nb = 0; nb < NB; nb += 4) {            // a block of 32 dims: its scales go into P
+                uint32_t pa[4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float2 d = *reinterpret_cast<const float2 *>(&vd[nb / 4][kk * 16 + h * 8 + 2 * (lane & 3)]);
+                    const float *p = x[kk * 2 + h];
+                    pa[2 * h] = pack_half2(p[0] * d.x, p[1] * d.y);
+                    pa[2 * h + 1] = pack_half2(p[2] * d.x, p[3] * d.y);
+                }
+#pragma unroll
+                for (int n2 = nb; n2 < nb + 4; n2 += 2) {
+                    uint32_t bv[4];
+                    ldsm_x4_t(bv, vs + (kk * 16 + (lmat & 1) * 8 + lrow) * P + n2 * 8 + (lmat >> 1) * 8);
+                    mma16816(o[n2], pa, bv[0], bv[1]);
+                    mma16816(o[n2 + 1], pa, bv[2], bv[3]);
+                }
             }
     }
 #pragma unroll
@@ -222,7 +235,7 @@ fa_paged_q8_kernel(const PagedAttnArgs a)
         l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
         l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
         if (row[u] >= rows) continue;
-        const float inv = l[u] == 0.f ? 0.f : 1.f / l[u];
+        const float inv = l[u] == 0.f ? 0.f : 0.015625f / l[u];
         const int head = g * a.G + row[u] % a.G, t = s.q0 + tok[u];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -242,9 +255,14 @@ __device__ __forceinline__ void q8_lds8(const char *p, uint32_t (&h)[4]) {
 }
 
 // Copies the Q8_0 pages of the streams that bring more than a.min_rows query rows
-// into F16 pages of 256 rows in `out` (stream s, page p: page s * out.max_pages +
-// p), values d * q rounded to half: 272 bytes read and 512 written per row and
-// KV head, next to 4 * 128 flops per query row for each of those rows.
+// into pages of 128 keys in `out` (stream s, page p: page s * out.max_pages + p).  A
+// value d * q of 18 bits becomes hi = it rounded to half and lo = the rest, exact
+// down to 2^-25; 64 rows of hi, then the same keys' 64 rows of lo, so that a tile of
+// 128 rows is a product over hi and lo at once.  (hi alone halves the products, but
+// its rounding of V doubles the output's squared error and K's grows with the
+// logits: 2.2 times the error of an F32 computation rounded to half at 1400 keys,
+// with lo 1.2 times.)  272 bytes read and 1024 written per row and KV head, next to
+// 8 * 128 flops per query row for each of those rows.
 // Grid (32-row ranges, Hkv, n_seq), 128 threads.
 template <int D>
 __global__ void __launch_bounds__(128)
@@ -276,13 +294,20 @@ paged_unpack_kernel(const PagedAttnArgs a, const PagedView out)
         const __half d = *reinterpret_cast<const __half *>(blk);
         uint32_t h[4];
         q8_lds8(blk + 2 + (c & 3) * 8, h);
+        const __half2 d2 = __half2half2(d);
+        uint32_t rest[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const __half2 x = __hmul2(*reinterpret_cast<const __half2 *>(&h[j]), __half2half2(d));
+            const __half2 q = *reinterpret_cast<const __half2 *>(&h[j]);
+            const __half2 x = __hmul2(q, d2), y = __hfma2(q, d2, __hneg2(x));
             h[j] = *reinterpret_cast<const uint32_t *>(&x);
+            rest[j] = *reinterpret_cast<const uint32_t *>(&y);
         }
-        char *dst = (sel ? out.v : out.k) + paged_row(out, b, r0 + r, g) + c * 16;
+        const int row = r0 + r;
+        char *dst = (sel ? out.v : out.k) + (long long)paged_page(out, b, row) * out.nb3 + (long long)g * out.nb2 +
+                    (long long)((row & 64) * 2 + (row & 63)) * out.nb1 + c * 16;
         *reinterpret_cast<uint4 *>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4 *>(dst + 64 * out.nb1) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
     }
 }
 

@@ -5,10 +5,10 @@
 //
 // A CTA owns a group of two 128-row Q tiles (one, when pairs would leave SMs idle)
 // of one stream and KV head (row = token * G + head of the group, T = 128 / G
-// tokens a tile) and one split of its key tiles of 128.  Two softmax warpgroups, one per Q tile (a thread per
-// row = TMEM lane), take turns on the tensor core; a third warpgroup holds the
-// TMA and the MMA warp and gives its registers away (setmaxnreg).  Per key tile
-// and Q tile: S = Q K^T into TMEM, P = 2^(x - m) over S's first half columns,
+// tokens a tile) and one split of its key tiles of 128.  Two softmax warpgroups, one
+// per Q tile (a thread per row = TMEM lane), take turns on the tensor core; a third
+// warpgroup holds the TMA and the MMA warp and gives its registers away
+// (setmaxnreg).  Per key tile and Q tile: S = Q K^T into TMEM, P = 2^(x - m) over S's first half columns,
 // O += P V with P read from TMEM.  Shared memory: both Q tiles, and a ring of K
 // and V tiles, all in the 128-byte swizzle.
 //
@@ -18,6 +18,11 @@
 // other pages outside the group's key range may hold anything, so the softmax
 // warps clear those V rows in shared memory before P V (masked P is 0, and
 // 0 * NaN is not), while masked scores are replaced.
+//
+// LO: an unpacked Q8_0 cache, whose tiles hold 64 keys as 64 rows of hi and 64 of lo
+// (value = hi + lo).  S's two halves are added before the softmax and P is stored
+// twice, so both products stay as they are; 2048 tokens at 14k keys 1017 us next to
+// 516 over F16 pages, as twice the products have it.
 //
 // D = 64, twice the exponentials per flop: a quarter of them runs on the FMA pipe
 // (2048 tokens at 14k keys 446 -> 430 us; D = 128 gains nothing, 519 us either way,
@@ -47,11 +52,12 @@ struct PagedTile {
     int groups;               // bound on the groups of all streams
     int n_splits, min_tiles;  // splits of a group's key tiles at most, key tiles per split at least
     int whole;                // (group, head) items that are not split, the first ones
+    int shift;                // log2 of the keys of a tile: 7, or 6 where a key has two rows
     float *part_o, *part_ml;  // [n_splits][n_tokens][Hq][D], ... [2] (m, l)
 };
 
 template <int D> struct PagedTileCfg {
-    static constexpr int BN = 128, SUB = D / 64;
+    static constexpr int SUB = D / 64;
     static constexpr int TILE = 128 * D * 2;
     static constexpr int STAGES = D == 64 ? 4 : 2;
     static constexpr int Q_OFF = 0, K_OFF = 2 * TILE, V_OFF = K_OFF + STAGES * TILE;
@@ -99,20 +105,21 @@ __device__ __forceinline__ PagedRange paged_range(const PagedSeq &s, int tok0, c
     const int off = s.len - s.n_new, last = min(s.n_new, tok0 + tl.tokens) - 1;
     r.hi = a.causal ? off + last : s.len - 1;
     r.lo = a.window > 0 ? max(0, off + tok0 - a.window + 1) : 0;
-    r.j0 = r.hi >= r.lo ? r.lo >> 7 : 0;
-    r.j1 = r.hi >= r.lo ? (r.hi >> 7) + 1 : 0;
+    r.j0 = r.hi >= r.lo ? r.lo >> tl.shift : 0;
+    r.j1 = r.hi >= r.lo ? (r.hi >> tl.shift) + 1 : 0;
     const int most = cut ? tl.n_splits : 1;
     r.per = max(tl.min_tiles, (r.j1 - r.j0 + most - 1) / most);
     r.n = max(1, (r.j1 - r.j0 + r.per - 1) / r.per);
     return r;
 }
 
-template <int D, bool UF>
+template <int D, bool UF, bool LO>
 __global__ void __launch_bounds__(PagedTileCfg<D>::NTHREADS, 1)
 fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                       const __grid_constant__ CUtensorMap tmQ, const PagedAttnArgs a, const PagedTile tl)
 {
     using C = PagedTileCfg<D>;
+    constexpr int KEYS = LO ? 64 : 128;            // of a tile
     extern __shared__ __align__(1024) char smem_raw[];
     char *smem = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *q_full = reinterpret_cast<uint64_t *>(smem + C::BAR_OFF);
@@ -245,7 +252,7 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
             ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], it & 1, a.kv.err, VTX_KERR_S));
             if (!ok) break;
             tc_fence_after();
-            float x[128];
+            float x[KEYS];
             {
                 uint32_t raw[128];
 #pragma unroll
@@ -253,24 +260,25 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
                     tmem_ld32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&raw[c * 32]));
                 tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 128; ++i) x[i] = __uint_as_float(raw[i]);
+                for (int i = 0; i < KEYS; ++i)
+                    x[i] = LO ? __uint_as_float(raw[i]) + __uint_as_float(raw[(i + 64) % 128]) : __uint_as_float(raw[i]);
             }
-            const int k0 = (jb + it) * C::BN;
+            const int k0 = (jb + it) * KEYS;
             if (UF) {
 #pragma unroll
-                for (int i = 0; i < 128; ++i) x[i] = paged_logit(x[i], a.scale, a.softcap);
+                for (int i = 0; i < KEYS; ++i) x[i] = paged_logit(x[i], a.scale, a.softcap);
             }
-            const bool full = !row_ok || (k0 >= lo && k0 + C::BN - 1 <= hi);
+            const bool full = !row_ok || (k0 >= lo && k0 + KEYS - 1 <= hi);
             if (__any_sync(0xffffffffu, !full)) {
 #pragma unroll
-                for (int i = 0; i < 128; ++i) x[i] = (k0 + i < lo || k0 + i > hi) ? -INFINITY : x[i];
+                for (int i = 0; i < KEYS; ++i) x[i] = (k0 + i < lo || k0 + i > hi) ? -INFINITY : x[i];
             }
             // V rows outside the group's key range hold anything: clear them
-            if (k0 < rg.lo || k0 + C::BN - 1 > rg.hi) {
+            if (k0 < rg.lo || k0 + KEYS - 1 > rg.hi) {
                 const int st = it % C::STAGES;
                 ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (it / C::STAGES) & 1, a.kv.err, VTX_KERR_KV));
                 if (!ok) break;
-                if (k0 + r < rg.lo || k0 + r > rg.hi) {
+                if (const int key = k0 + (r & (KEYS - 1)); key < rg.lo || key > rg.hi) {
                     char *v = smem + C::V_OFF + st * C::TILE + r * 128;
 #pragma unroll
                     for (int i = 0; i < C::SUB * 8; ++i)
@@ -281,9 +289,10 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
             float mx8[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                mx8[k] = fmaxf(x[16 * k], x[16 * k + 1]);
+                constexpr int W = KEYS / 8;
+                mx8[k] = fmaxf(x[W * k], x[W * k + 1]);
 #pragma unroll
-                for (int i = 2; i < 16; i += 2) mx8[k] = fmax3(mx8[k], x[16 * k + i], x[16 * k + i + 1]);
+                for (int i = 2; i < W; i += 2) mx8[k] = fmax3(mx8[k], x[W * k + i], x[W * k + i + 1]);
             }
             const float mx = fmax3(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]),
                                    fmaxf(mx8[6], mx8[7])) * cx;
@@ -300,9 +309,9 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
             const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
             const uint64_t cx2 = pk2(cx, cx), nm2 = pk2(neg_m, neg_m);
             uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
-            uint32_t pk[64];
+            uint32_t pk[KEYS / 2];
 #pragma unroll
-            for (int i = 0; i < 64; ++i) {
+            for (int i = 0; i < KEYS / 2; ++i) {
                 float e0, e1;
                 upk2(ffma2(pk2(x[2 * i], x[2 * i + 1]), cx2, nm2), e0, e1);
                 if (D == 64 && (i & 3) == 3) {     // every fourth pair off the MUFU
@@ -320,7 +329,7 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
                 l_run += sa + sb;
             }
             tmem_st32(s_addr, *reinterpret_cast<const uint32_t(*)[32]>(&pk[0]));
-            tmem_st32(s_addr + 32, *reinterpret_cast<const uint32_t(*)[32]>(&pk[32]));
+            tmem_st32(s_addr + 32, *reinterpret_cast<const uint32_t(*)[32]>(&pk[LO ? 0 : 32]));
             // tcgen05.ld / st are warp-collective: the warp rescales when any row needs it
             if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll
@@ -418,14 +427,14 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
                 }
                 __syncwarp();
             }
-            const int rows_box = min(128, 1 << a.kv.shift), per_tile = 128 / rows_box;   // boxes of a half-width tile
-            const int mask = (1 << a.kv.shift) - 1;
+            const int rows_box = LO ? 128 : min(128, 1 << a.kv.shift), per_tile = 128 / rows_box;   // boxes of a half-width tile
+            const int mask = (1 << a.kv.shift) - 1, rows = LO ? 2 : 1;       // rows of a key
             // lane = box of a tile; 64 boxes at most (16-row pages: 8 pages x SUB x {K, V} = 32 for D = 128)
             const int kvsel = lane / (per_tile * C::SUB);                   // 0: K, 1: V, more: idle
             const int sub = (lane / per_tile) % C::SUB, pg = lane % per_tile;
             const bool mine = kvsel < 2;
             auto page_at = [&](int it) -> int {    // this lane's page of tile it, -1: none needed
-                const int y = (jb + it) * C::BN + pg * rows_box;
+                const int y = (jb + it) * KEYS + pg * rows_box;
                 if (!mine || it >= n_iter || y > rg.hi || y + rows_box <= rg.lo) return -1;
                 return max(paged_page(a.kv, b, y), 0);
             };
@@ -445,10 +454,10 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
                 }
                 __syncwarp();
                 if (cur >= 0) {
-                    const int y = (jb + it) * C::BN + pg * rows_box;
+                    const int y = ((jb + it) * KEYS + pg * rows_box & mask) * rows;
                     char *dst = smem + (kvsel ? C::V_OFF : C::K_OFF) + st * C::TILE + sub * 16384 + pg * rows_box * 128;
-                    if (kvsel) tma_load_4d(dst, &tmV, &v_full[st], sub * 64, y & mask, g, cur);
-                    else tma_load_4d(dst, &tmK, &k_full[st], sub * 64, y & mask, g, cur);
+                    if (kvsel) tma_load_4d(dst, &tmV, &v_full[st], sub * 64, y, g, cur);
+                    else tma_load_4d(dst, &tmK, &k_full[st], sub * 64, y, g, cur);
                 }
                 __syncwarp();
             }

@@ -185,16 +185,18 @@ int launch_attn_q8(const PagedAttnArgs &a, cudaStream_t st) {
 
 // The tensor-core kernel, when a stream may bring more rows than the streaming
 // kernel takes: F16 caches, and Q8_0 caches of kUnpackFrom rows or more, whose
-// pages it reads as an F16 copy in the workspace.  K is rounded to half there,
-// which moves a row's lse by about 2^-12 / sqrt(visible keys), hence the bound; and
-// below it mma.sync on the pages is as fast.  Copies above kUnpackBytes: no.
-constexpr int kUnpackFrom = 1024, kUnpackPage = 256;
-constexpr size_t kUnpackBytes = size_t(2) << 30;
+// pages it reads as pairs of halves (value = hi + lo) in the workspace.  Over
+// shorter ones mma.sync on the pages is as fast and takes no workspace (prompts of
+// 32, 64, 96 and 128 tokens, 8 KV heads: 8.3, 12.0, 15.7 and 19.3 us there, 13.7,
+// 13.6, 15.0 and 15.1 unpacked; 391: 52 and 22).  It also takes what would need
+// more than kUnpackBytes of workspace (128 tokens at 14k: 1630 and 109 us).
+constexpr int kUnpackFrom = 96, kUnpackPage = 128;
+constexpr size_t kUnpackBytes = size_t(4) << 30;
 
 struct TilePlan {
     bool use;
     PagedTile tile;
-    int unpack;               // pages of kUnpackPage rows per stream, 0: none
+    int unpack;               // pages of kUnpackPage keys per stream, 0: none
     size_t o_bytes, u_bytes, bytes;   // partial O, one unpacked pool, all
 };
 
@@ -203,7 +205,7 @@ TilePlan plan_tile(const vtx_paged_kv *p, int G, int Hq, int min_rows, int sms) 
     const int Hkv = (int)p->k.ne[2], D = (int)p->k.ne[0];
     if (p->k.type == VTX_TYPE_Q8_0 && p->max_kv_len >= kUnpackFrom) {
         t.unpack = (p->max_kv_len + kUnpackPage - 1) / kUnpackPage;
-        t.u_bytes = (size_t)p->n_seq * t.unpack * kUnpackPage * Hkv * D * 2;
+        t.u_bytes = (size_t)p->n_seq * t.unpack * kUnpackPage * Hkv * D * 4;
         if (2 * t.u_bytes > kUnpackBytes) t.unpack = 0;
     }
     t.use = (p->k.type == VTX_TYPE_F16 || t.unpack) && p->max_new * (long long)G > min_rows && p->n_seq > 0;
@@ -227,7 +229,8 @@ TilePlan plan_tile(const vtx_paged_kv *p, int G, int Hq, int min_rows, int sms) 
     // One stream: its groups are about equal, so whole waves count, and full waves
     // are left whole.  Several: lengths spread, so the average load plus half a
     // CTA's time.
-    const int tiles = std::max(1, (p->max_kv_len + 127) / 128);
+    t.tile.shift = t.unpack ? 6 : 7;
+    const int tiles = std::max(1, (p->max_kv_len + (1 << t.tile.shift) - 1) >> t.tile.shift);
     const double tile_us = D == 128 ? 2.1 : 1.6, cta_us = 6.0;
     const double row_us = (double)D * 8 / 5e6;               // one row, one split
     const long long items = (long long)t.tile.groups * Hkv;
@@ -268,15 +271,15 @@ TilePlan plan_tile(const vtx_paged_kv *p, int G, int Hq, int min_rows, int sms) 
     return t;
 }
 
-// The F16 copy of a Q8_0 cache, at the end of the tile plan's workspace.
+// The unpacked copy of a Q8_0 cache, two rows of halves for each of its own, at the end of the tile plan's workspace.
 PagedView unpacked_view(const PagedView &kv, const TilePlan &t, int D, char *ws) {
     PagedView u = kv;
     u.k = ws + t.bytes - 2 * t.u_bytes;
     u.v = u.k + t.u_bytes;
-    u.nb1 = D * 2; u.nb2 = (long long)kUnpackPage * D * 2; u.nb3 = u.nb2 * kv.Hkv;
+    u.nb1 = D * 2; u.nb2 = (long long)kUnpackPage * D * 4; u.nb3 = u.nb2 * kv.Hkv;
     u.table = nullptr;
     u.max_pages = t.unpack; u.n_pages = kv.n_seq * t.unpack;
-    u.shift = 8;
+    u.shift = 7;
     return u;
 }
 
@@ -288,10 +291,11 @@ int launch_unpack(const PagedAttnArgs &a, const PagedView &out, cudaStream_t st)
 }
 
 // Map of an F16 pool: (dim, row, head, page), boxes of 64 dims x min(page, 128) rows.
-int encode_pool_map(CUtensorMap *m, const PagedView &kv, void *pool, int D) {
+// key_rows: rows that a key has (2 in an unpacked copy).
+int encode_pool_map(CUtensorMap *m, const PagedView &kv, void *pool, int D, int key_rows = 1) {
     PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
     if (!enc) return VTX_ERR_CUDA;
-    const long long page = 1LL << kv.shift;                   // extent-1 axes: any legal stride
+    const long long page = (long long)key_rows << kv.shift;                   // extent-1 axes: any legal stride
     const long long s2 = kv.Hkv > 1 ? kv.nb2 : kv.nb1 * page, s3 = kv.n_pages > 1 ? kv.nb3 : s2 * kv.Hkv;
     cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)page, (cuuint64_t)kv.Hkv, (cuuint64_t)kv.n_pages};
     cuuint64_t strides[3] = {(cuuint64_t)kv.nb1, (cuuint64_t)s2, (cuuint64_t)s3};
@@ -317,18 +321,24 @@ int encode_paged_q_map(CUtensorMap *m, const vtx_tensor *q, int G, int T) {
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? VTX_OK : VTX_ERR_STRIDE;
 }
 
-template <int D, bool UF>
+template <int D, bool UF, bool LO>
 int launch_tile(const CUtensorMap (&m)[3], const PagedAttnArgs &a, const PagedTile &tl, cudaStream_t st) {
     using C = PagedTileCfg<D>;
     static std::atomic<int> done[kMaxDevices];
-    int rc = allow_smem(fa_paged_sm100_kernel<D, UF>, C::SMEM, done);
+    int rc = allow_smem(fa_paged_sm100_kernel<D, UF, LO>, C::SMEM, done);
     if (rc != VTX_OK) return rc;
     const long long items = (long long)tl.groups * a.kv.Hkv;
     const long long ctas = tl.whole + (items - tl.whole) * tl.n_splits;
     if (ctas > 0x7fffffffLL) return VTX_ERR_UNSUPPORTED;
     if (ctas == 0) return VTX_OK;
-    return launch_pdl(fa_paged_sm100_kernel<D, UF>, dim3((unsigned)ctas), dim3(C::NTHREADS), C::SMEM, st, m[0], m[1],
+    return launch_pdl(fa_paged_sm100_kernel<D, UF, LO>, dim3((unsigned)ctas), dim3(C::NTHREADS), C::SMEM, st, m[0], m[1],
                       m[2], a, tl);
+}
+
+template <int D>
+int launch_tile_any(const CUtensorMap (&m)[3], const PagedAttnArgs &a, const TilePlan &t, bool uf, cudaStream_t st) {
+    if (t.unpack) return uf ? launch_tile<D, true, true>(m, a, t.tile, st) : launch_tile<D, false, true>(m, a, t.tile, st);
+    return uf ? launch_tile<D, true, false>(m, a, t.tile, st) : launch_tile<D, false, false>(m, a, t.tile, st);
 }
 
 template <int D>
@@ -533,15 +543,15 @@ int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, si
             if (rc != VTX_OK) return rc;
         }
         CUtensorMap m[3];
-        rc = encode_pool_map(&m[0], ta.kv, ta.kv.k, D);
-        if (rc == VTX_OK) rc = encode_pool_map(&m[1], ta.kv, ta.kv.v, D);
+        rc = encode_pool_map(&m[0], ta.kv, ta.kv.k, D, tp.unpack ? 2 : 1);
+        if (rc == VTX_OK) rc = encode_pool_map(&m[1], ta.kv, ta.kv.v, D, tp.unpack ? 2 : 1);
         m[2] = m[0];                                          // an F32 q is read by the softmax warps
         if (rc == VTX_OK && a.q_f16) rc = encode_paged_q_map(&m[2], q, a.G, tp.tile.T);
         if (rc != VTX_OK) return rc;
         // tanh, or a scale that the row maximum cannot carry: logits formed first
         const bool uf = a.softcap != 0.0f || !(a.scale > 0.0f);
-        if (d64) rc = uf ? launch_tile<64, true>(m, ta, tp.tile, st) : launch_tile<64, false>(m, ta, tp.tile, st);
-        else rc = uf ? launch_tile<128, true>(m, ta, tp.tile, st) : launch_tile<128, false>(m, ta, tp.tile, st);
+        if (d64) rc = launch_tile_any<64>(m, ta, tp, uf, st);
+        else rc = launch_tile_any<128>(m, ta, tp, uf, st);
     } else if (kv->max_new * (long long)a.G > a.min_rows) {
         rc = d64 ? launch_attn_q8<64>(a, st) : launch_attn_q8<128>(a, st);
     }
