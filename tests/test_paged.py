@@ -193,6 +193,15 @@ def test_call_refusals_without_device(lib):
     assert evict(ws=0) == -6 and evict(ws=0x100010) == -6 and evict(n=16) == -6
 
 
+@pytest.mark.parametrize("nb1,nb2", [(0, 0), (512, 0), (256, 32 * 512), (512, 496)])
+def test_overlapping_output_rows_are_refused(lib, nb1, nb2):
+    c, p = _kv(), V.params(0.1, causal=True)
+    q, d = _tensor(V.F16, [128, 2, 32, 1], [2, 32 * 256, 256, 0]), _tensor(V.F32, [128, 32, 2, 1], [4, nb1, nb2, 0], 0x80000)
+    a = V.FlashAttnPagedArgs()
+    a.kv, a.q, a.dst, a.params = (ctypes.addressof(x) for x in (c, q, d, p))
+    assert lib.vtx_flash_attn_paged(B(a), 0x100000, 1 << 40, None) == -4
+
+
 def test_python_refusals(lib):
     k = torch.zeros(4, 2, 16, 64, dtype=torch.float16)
     i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
@@ -731,6 +740,27 @@ def test_evict_more_rows_than_fit_in_shared_memory():
     c["k_pool"] = rng.standard_normal((-(-n // 256), 1, 256, 64)).astype(np.float16)
     c["v_pool"] = rng.standard_normal(c["k_pool"].shape).astype(np.float16)
     run_evict(c, np.round(rng.standard_normal((1, 1, n)) * 20).astype(np.float32), 20000, n_sink=4, n_recent=100)
+
+
+@pytest.mark.gpu
+def test_tensors_of_another_device_are_refused():
+    """Every tensor of a call is checked to lie where the pools do, before any launch."""
+    c = R.build(33, "f16", [(2, 20)])
+    kv = device_kv(c)
+    q, pos = torch.from_numpy(c["q"]).cuda(), torch.zeros(2, dtype=torch.int32, device="cuda")
+    k, sc = torch.zeros(2, 2, 128, device="cuda"), torch.zeros(1, 2, 32, device="cuda")
+    lse, n = torch.zeros(2, 8, device="cuda"), torch.zeros(1, dtype=torch.int32)
+    for call in (lambda: V.PagedKv(kv.k_pool, kv.v_pool.cpu(), kv.page_table, kv.kv_len, kv.q_start, 8, n_tokens=2, max_new=2),
+                 lambda: V.PagedKv(kv.k_pool, kv.v_pool, kv.page_table, kv.kv_len.cpu(), kv.q_start, 8, n_tokens=2, max_new=2),
+                 lambda: kv.append(k.cpu(), k, pos), lambda: kv.append(k, k.cpu(), pos), lambda: kv.append(k, k, pos.cpu()),
+                 lambda: kv.append(k, k, pos, q=q.float().cpu()), lambda: kv.append(k, k, pos, q=q.float(), q_out=q.cpu()),
+                 lambda: kv.append(k, k, pos, score=sc.cpu()), lambda: kv.append(k, k, pos, row_pos=sc.int().cpu()),
+                 lambda: kv.attend(q.cpu()), lambda: kv.attend(q, out=q.cpu()), lambda: kv.attend(q, lse=lse.cpu()),
+                 lambda: kv.score(q, lse.cpu(), sc), lambda: kv.score(q, lse, sc.cpu()),
+                 lambda: kv.score(q, lse, sc, score_out=sc.cpu()), lambda: kv.evict(sc.cpu(), 8),
+                 lambda: kv.evict(sc, 8, n), lambda: kv.evict(sc, 8, next_pos=n), lambda: kv.evict(sc, 8, src_out=sc.int().cpu())):
+        with pytest.raises(V.VtxError):
+            call()
 
 
 @pytest.mark.gpu

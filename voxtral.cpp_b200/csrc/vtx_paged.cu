@@ -128,8 +128,8 @@ struct DecodePlan {
 
 // Splits over (streams x KV heads): one wave of three CTAs per SM for one stream,
 // or where two would leave fewer than 40 tiles each (8 streams of 4000: 39.8 -> 30.2
-// us); else two, which spreads ragged lengths more
-// evenly; at most 128 tiles (2048 keys) each, and at least one tile per warp.
+// us); else two, which spreads ragged lengths more evenly; at most 128 tiles (2048
+// keys) each, and at least one tile per warp.
 DecodePlan plan_decode(const vtx_paged_kv *p, int G, int sms) {
     DecodePlan d{};
     // the only stream may bring more tokens than fit: then all go one way
@@ -505,6 +505,8 @@ int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, si
     if (d->type != VTX_TYPE_F32 && d->type != VTX_TYPE_F16) return VTX_ERR_TYPE;
     if (d->ne[0] != q->ne[0] || d->ne[1] != q->ne[2] || d->ne[2] != q->ne[1] || d->ne[3] != 1) return VTX_ERR_SHAPE;
     if (d->nb[0] != (size_t)elem_size(d->type)) return VTX_ERR_STRIDE;
+    for (int i = 1; i < 3; ++i)                               // rows of dst must not overlap
+        if (d->ne[i] > 1 && d->nb[i] < (size_t)d->ne[0] * d->nb[0]) return VTX_ERR_STRIDE;
     if (kv->n_tokens == 0 || kv->n_seq == 0) return VTX_OK;
     if (!d->data) return VTX_ERR_NULL;
     if (reinterpret_cast<uintptr_t>(d->data) % 16 || d->nb[1] % 16 || d->nb[2] % 16) return VTX_ERR_STRIDE;

@@ -456,11 +456,12 @@ class PagedKv:
     def __init__(self, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor,
                  q_start: torch.Tensor, n_head_q: int, *, n_tokens: int, max_new: int,
                  max_kv_len: Optional[int] = None):
-        if k_pool.dim() != 4 or v_pool.shape != k_pool.shape or v_pool.dtype != k_pool.dtype:
+        if k_pool.dim() != 4 or v_pool.shape != k_pool.shape or v_pool.dtype != k_pool.dtype or \
+                v_pool.device != k_pool.device:
             raise VtxError(-3, "k_pool and v_pool must be (n_pages, n_head_kv, page_size, D) alike")
         if k_pool.dtype not in (torch.float16, torch.uint8):
             raise VtxError(-2, "pools must be float16 or Q8_0 bytes")
-        self.dev = k_pool.device
+        self.dev, self._on = k_pool.device, k_pool.get_device()
         n_seq = kv_len.shape[0]
         for t, shape in ((page_table, (n_seq, page_table.shape[-1])), (kv_len, (n_seq,)), (q_start, (n_seq + 1,))):
             if t.dtype != torch.int32 or not t.is_contiguous() or t.device != self.dev or tuple(t.shape) != shape:
@@ -549,6 +550,12 @@ class PagedKv:
         p.scale = self.head_dim ** -0.5 if scale is None else scale
         p.logit_softcap, p.causal, p.window = softcap, 1 if causal else 0, window
 
+    def _made(self, t: torch.Tensor, stream: Optional[torch.cuda.Stream]) -> torch.Tensor:
+        """A result allocated here on the current stream and written on `stream`."""
+        if stream is not None and self.dev.type == "cuda":
+            t.record_stream(stream)
+        return t
+
     def _call(self, fn, args, stream: Optional[torch.cuda.Stream], *ws) -> None:
         dev = self.dev
         if dev.type != "cuda":
@@ -578,9 +585,13 @@ class PagedKv:
             raise VtxError(-4, f"k and v must be {self._kv_shape} float32 with heads contiguous")
         if positions.dtype != torch.int32 or positions.shape != (self.n_tokens,) or not positions.is_contiguous():
             raise VtxError(-3, "positions must be contiguous int32, one per token")
+        if not k.get_device() == v.get_device() == positions.get_device() == self._on:
+            raise VtxError(-3, f"k, v and positions must be on {self.dev}")
         if q is not None:
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=torch.float16, device=q.device)
+                q_out = self._made(torch.empty(q.shape, dtype=torch.float16, device=self.dev), stream)
+            if not q.get_device() == q_out.get_device() == self._on:
+                raise VtxError(-3, f"q and q_out must be on {self.dev}")
             qs, os_, kind = q.stride(), q_out.stride(), _ROW_TYPES.get(q_out.dtype)
             if q.shape != self._q_shape or q_out.shape != self._q_shape or qs[2] != 1 or qs[1] != D or os_[2] != 1 or \
                     os_[1] != D or q.dtype != torch.float32 or kind is None:
@@ -608,7 +619,7 @@ class PagedKv:
         optional float32 (n_tokens, n_head_q) that receives ln sum exp.  scale
         defaults to D ** -0.5."""
         if out is None:
-            out = torch.empty(self._q_shape, dtype=torch.float32, device=self.dev)
+            out = self._made(torch.empty(self._q_shape, dtype=torch.float32, device=self.dev), stream)
         self._rows(q, "q", self._q, self._q_nb, 1, 2)
         self._rows(out, "out", self._dst, self._dst_nb, 2, 1)
         self._set_params(scale, causal, window, logit_softcap)
@@ -617,8 +628,9 @@ class PagedKv:
         return out
 
     def _check_lse(self, lse: torch.Tensor) -> int:
-        if lse.shape != self._q_shape[:2] or lse.dtype != torch.float32 or not lse.is_contiguous():
-            raise VtxError(-3, "lse must be a contiguous float32 (n_tokens, n_head_q) tensor")
+        if lse.shape != self._q_shape[:2] or lse.dtype != torch.float32 or not lse.is_contiguous() or \
+                lse.get_device() != self._on:
+            raise VtxError(-3, f"lse must be a contiguous float32 (n_tokens, n_head_q) tensor on {self.dev}")
         return lse.data_ptr()
 
     def score(self, q: torch.Tensor, lse: torch.Tensor, score: torch.Tensor, score_out: Optional[torch.Tensor] = None,
@@ -650,8 +662,9 @@ class PagedKv:
         if kv_len_out is None:
             kv_len_out = self.kv_len
         for t, what in ((kv_len_out, "kv_len_out"), (next_pos, "next_pos")):
-            if t is not None and (t.dtype != torch.int32 or t.shape != (self.n_seq,) or not t.is_contiguous()):
-                raise VtxError(-3, f"{what} must be contiguous int32, one per stream")
+            if t is not None and (t.dtype != torch.int32 or t.shape != (self.n_seq,) or not t.is_contiguous() or
+                                  t.get_device() != self._on):
+                raise VtxError(-3, f"{what} must be contiguous int32 on {self.dev}, one per stream")
         a = self._evict
         a.row_cap = self._array(row_pos, torch.int32, "row_pos", self._array(score, torch.float32, "score", None))
         cap = self._array(pos_out, torch.int32, "pos_out", self._array(score_out, torch.float32, "score_out", None))
