@@ -4,8 +4,9 @@
 // kv_evict_select_kernel finds them (one CTA per (stream, head)), writes the new
 // score / position / source arrays and the list of moves; kv_evict_move_kernel
 // copies the K and V rows of the moves and writes the new lengths.  With few
-// moves the first kernel does that too (UNIT > 0).  A move takes a kept row at or behind m to a gap below m, so no row
-// is both read and written and the moves run in any order.
+// moves the first kernel does that too (UNIT > 0).  A move takes a kept row at or
+// behind m to a gap below m, so no row is both read and written and the moves run
+// in any order.
 #pragma once
 #include <cuda_fp16.h>
 #include <cstdint>
