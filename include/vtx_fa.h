@@ -427,7 +427,8 @@ typedef struct vtx_paged_kv {
  * keep full accuracy (vtx_kv_append follows ggml's float recurrence).
  * - q / k / v: n_tokens rows of heads x head_dim F32 (heads contiguous, token
  *   stride *_nb1 bytes).  q_out: F32 or F16 rows of n_head_q x head_dim (NULL:
- *   only K and V); an F32 q_out may be q itself.
+ *   only K and V), written for tokens of no stream too; an F32 q_out may be q
+ *   itself.
  * - positions[t]: the RoPE position of token t (not its row: an evicted
  *   cache has fewer rows than positions).
  * - row_pos / score (each optional): [n_seq][n_head_kv][row_cap] arrays; the

@@ -764,6 +764,56 @@ def test_tensors_of_another_device_are_refused():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("streams", [[(6, 4), (2, 30)], [(40, 30), (1, 9)]])
+def test_widest_window_is_none(streams):
+    """The largest window, with streams of more tokens than rows too."""
+    c = R.build(34, "f16", streams)
+    q = torch.from_numpy(c["q"]).cuda()
+    T = q.shape[0]
+    outs = []
+    for w in (0, 2 ** 31 - 1):
+        kv, lse = device_kv(c), torch.empty(T, 8, device="cuda")
+        out = kv.attend(q, lse=lse, window=w)
+        sc = [kv.score(x, lse, torch.zeros(2, 2, 64, device="cuda"), window=w) for x in (q, q.float())]
+        outs.append([out, lse, *sc])
+    ref = R.attend(c)
+    check_attend(c, outs[1][0], outs[1][1], ref)
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+@pytest.mark.gpu
+def test_append_rotates_queries_of_no_stream():
+    """q_out is written for every token, with K and V going nowhere."""
+    c = R.build(35, "f16", [(3, 20)])
+    kv = device_kv(c)
+    q, k, pos = torch.randn(3, 8, 128).cuda(), torch.randn(3, 2, 128).cuda(), torch.tensor([5, 6, 900], dtype=torch.int32).cuda()
+    want = kv.append(k, k, pos, q=q)
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    none = V.PagedKv(kv.k_pool, kv.v_pool, i32(0, 1), i32(0), i32(1), 8, n_tokens=3, max_new=0)
+    before = kv.k_pool.clone()
+    assert torch.equal(none.append(k, k, pos, q=q), want)
+    kv.q_start.zero_()
+    assert torch.equal(kv.append(k, k, pos, q=q), want)
+    assert torch.equal(kv.k_pool.view(torch.int16), before.view(torch.int16)) and V.read_device_error() == 0
+
+
+@pytest.mark.gpu
+def test_evict_lengths_over_next_pos():
+    """kv_len_out may be next_pos: every head still protects the recent rows."""
+    rng = np.random.default_rng(36)
+    c = R.build(36, "f16", [(0, 900)] * 40, 8, 4, 64)
+    sc = torch.from_numpy(rng.random((40, 4, 900), np.float32)).cuda()
+    got = []
+    for alias in (False, True):
+        kv = device_kv(c, n_tokens=0, max_new=0)
+        nxt = kv.kv_len.clone()
+        src = torch.zeros(40, 4, 100, dtype=torch.int32, device="cuda")
+        n = kv.evict(sc, 100, nxt if alias else kv.kv_len.clone(), n_recent=64, next_pos=nxt, src_out=src)
+        got.append((n.cpu(), src.cpu()))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]) and (got[0][0] == 100).all()
+
+
+@pytest.mark.gpu
 def test_evict_reports_a_length_above_its_bound():
     c = R.build(13, "f16", [(0, 100), (0, 40)], 4, 2, 64, poison=False)
     kv = device_kv(c, max_kv_len=64, n_tokens=0, max_new=0)

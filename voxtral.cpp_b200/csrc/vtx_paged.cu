@@ -444,8 +444,8 @@ int vtx_kv_append_paged(const vtx_kv_append_paged_args *p, void *stream) {
     if (p->q_out && p->n_head_q < 1) return VTX_ERR_SHAPE;
     if (!(p->freq_base > 0.0f) || !std::isfinite(p->freq_base)) return VTX_ERR_UNSUPPORTED;
     if ((p->row_pos || p->score) && p->row_cap < kv->max_kv_len) return VTX_ERR_SHAPE;
-    if (kv->n_tokens == 0 || kv->n_seq == 0) return VTX_OK;
-    if (!p->k || !p->v || !p->positions || !kv->q_start || (p->q_out && !p->q)) return VTX_ERR_NULL;
+    if (kv->n_tokens == 0) return VTX_OK;
+    if (!p->k || !p->v || !p->positions || (kv->n_seq > 0 && !kv->q_start) || (p->q_out && !p->q)) return VTX_ERR_NULL;
     const size_t kvrow = (size_t)kv->k.ne[2] * D * 4, qrow = (size_t)p->n_head_q * D;
     if (p->k_nb1 < kvrow || p->v_nb1 < kvrow) return VTX_ERR_STRIDE;
     const unsigned long long rows =
@@ -528,7 +528,8 @@ int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, si
     a.lse = p->lse;
     a.Hq = Hq; a.G = Hq / a.kv.Hkv;
     a.scale = p->params->scale; a.softcap = p->params->logit_softcap;
-    a.causal = p->params->causal != 0; a.window = p->params->window;
+    a.causal = p->params->causal != 0;
+    a.window = std::min(p->params->window, 1 << 30);          // sums with lengths stay in range
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool f16 = kv->k.type == VTX_TYPE_F16, d64 = kv->k.ne[0] == 64;
     // chunks first (their CTAs are long), few-token streams beside them
@@ -595,7 +596,8 @@ int vtx_kv_score_paged(const vtx_kv_score_paged_args *p, void *stream) {
     a.decay = p->decay; a.observe = p->observe;
     a.Hq = (int)p->q->ne[2]; a.G = a.Hq / a.kv.Hkv;
     a.scale = p->params->scale; a.softcap = p->params->logit_softcap;
-    a.causal = p->params->causal != 0; a.window = p->params->window;
+    a.causal = p->params->causal != 0;
+    a.window = std::min(p->params->window, 1 << 30);          // sums with lengths stay in range
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool f16 = kv->k.type == VTX_TYPE_F16, d64 = kv->k.ne[0] == 64;
     const long long rows = (long long)(p->observe > 0 ? std::min(p->observe, kv->max_new) : kv->max_new) * a.G;
@@ -664,9 +666,9 @@ int vtx_kv_evict_paged(const vtx_kv_evict_paged_args *p, void *workspace, size_t
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // Few moves: one kernel, a launch less.  A (stream, head) is one CTA there, too
     // little for many moves, and with enough items the two kernels take as long as
-    // one (256 items of 1500 to 8192 rows: 87 against 91 us).  Not in place on kv_len,
-    // which the other heads' CTAs may not have read yet.
-    if (e.max_moves <= 512 && p->kv_len_out != kv->kv_len) {
+    // one (256 items of 1500 to 8192 rows: 87 against 91 us).  Not in place on kv_len
+    // or next_pos, which the other heads' CTAs may not have read yet.
+    if (e.max_moves <= 512 && p->kv_len_out != kv->kv_len && p->kv_len_out != p->next_pos) {
         if (unit == 16) return launch_evict_select<true, 16>(a, e.items, st);
         return unit == 8 ? launch_evict_select<true, 8>(a, e.items, st) : launch_evict_select<true, 4>(a, e.items, st);
     }
