@@ -62,8 +62,9 @@ template <int D> struct PagedTileCfg {
     static constexpr int STAGES = D == 64 ? 4 : 2;
     static constexpr int Q_OFF = 0, K_OFF = 2 * TILE, V_OFF = K_OFF + STAGES * TILE;
     static constexpr int BAR_OFF = V_OFF + STAGES * TILE;
-    static constexpr int NBARS = 1 + 3 * STAGES + 6;
-    static constexpr int SMEM = BAR_OFF + NBARS * 8 + 32 + 1024;       // + alignment slack
+    static constexpr int NBARS = 1 + 4 * STAGES + 6;
+    static constexpr int ML_OFF = BAR_OFF + NBARS * 8 + 32;            // (m, l) of the second warpgroup's rows
+    static constexpr int SMEM = ML_OFF + 1024 + 1024;                  // + alignment slack
     static constexpr int NTHREADS = 384, TMA_WARP = 8, MMA_WARP = 9;
     static constexpr int REG_SOFTMAX = 224, REG_PRODUCER = 56;         // 256 x 224 + 128 x 56 = 384 x 168
     __host__ __device__ static constexpr int s_col(int t) { return t * 128; }
@@ -125,8 +126,9 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     uint64_t *q_full = reinterpret_cast<uint64_t *>(smem + C::BAR_OFF);
     uint64_t *k_full = q_full + 1;
     uint64_t *v_full = k_full + C::STAGES;
-    uint64_t *kv_empty = v_full + C::STAGES;
-    uint64_t *s_full = kv_empty + C::STAGES;       // [2]
+    uint64_t *k_empty = v_full + C::STAGES;
+    uint64_t *v_empty = k_empty + C::STAGES;
+    uint64_t *s_full = v_empty + C::STAGES;        // [2]
     uint64_t *p_full = s_full + 2;                 // [2]
     uint64_t *o_tile = p_full + 2;                 // [2]
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(o_tile + 2);
@@ -144,7 +146,8 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
         for (int i = 0; i < C::STAGES; ++i) {
             mbar_init(&k_full[i], 1);
             mbar_init(&v_full[i], 1);
-            mbar_init(&kv_empty[i], 1);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_empty[i], 1);
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&s_full[t], 1);
@@ -215,10 +218,11 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     if (warp < 8) {
         setmaxnreg_inc<C::REG_SOFTMAX>();
         // =================== softmax warpgroups ===============================
-        const int t = warp >> 2, r = tid & 127;
-        const int tok = tok0 + t * tl.T + r / a.G, head = g * a.G + r % a.G;
+        // with two Q tiles a warpgroup each; with one the warpgroups take its key tiles in turn
+        const int t = warp >> 2, r = tid & 127, step = two ? 1 : 2, it0 = two ? 0 : t;
+        const int tok = tok0 + (two ? t * tl.T : 0) + r / a.G, head = g * a.G + r % a.G;
         const bool row_ok = r < tl.T * a.G && tok < n_serve;
-        const int iters = t == 0 || two ? n_iter : 0;
+        const int iters = (n_iter - it0 + step - 1) / step;
         bool ok = true;
         int lo = 1, hi = 0;
         if (row_ok) {
@@ -231,6 +235,7 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) {
                 uint4 pk = make_uint4(0u, 0u, 0u, 0u);
+                if (t == 1 && !two) break;
                 if (row_ok) {
                     const float4 x = *reinterpret_cast<const float4 *>(src + c * 32);
                     const float4 y = *reinterpret_cast<const float4 *>(src + c * 32 + 16);
@@ -248,8 +253,8 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
         const float cx = UF ? 1.0f : a.scale * kLog2e;
         float m_run = -INFINITY, l_run = 0.0f;
 
-        for (int it = 0; it < iters; ++it) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], it & 1, a.kv.err, VTX_KERR_S));
+        for (int i0 = 0, it = it0; i0 < iters; ++i0, it += step) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], i0 & 1, a.kv.err, VTX_KERR_S));
             if (!ok) break;
             tc_fence_after();
             float x[KEYS];
@@ -301,7 +306,7 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
             if (mx > m_run + 8.0f) {               // the reference moves only on a 2^8 jump
                 if (m_run != -INFINITY) {
                     alpha = ex2(m_run - mx);
-                    rescale = it > 0;
+                    rescale = i0 > 0;
                 }
                 m_run = mx;
                 l_run *= alpha;
@@ -353,10 +358,29 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
             tc_fence_after();
         }
         if (m_run == -INFINITY) l_run = 0.0f;      // saw nothing (the sum holds 2^-125s)
+        float f0 = 1.0f, f1 = 0.0f;                // weights of this warpgroup's O and the other one's
+        const bool join = !two && n_iter > 1;
+        if (join) {                                // the first warpgroup takes the second one's sums in
+            float2 *ml = reinterpret_cast<float2 *>(smem + C::ML_OFF);
+            if (t == 1) ml[r] = make_float2(m_run, l_run);
+            asm volatile("bar.sync 3, 256;" ::: "memory");
+            if (t == 0) {
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_tile[1], 0, a.kv.err, VTX_KERR_O));
+                tc_fence_after();
+                const float2 y = ml[r];
+                const float top = fmaxf(m_run, y.x);
+                f0 = m_run == -INFINITY ? 0.0f : ex2(m_run - top);
+                f1 = y.x == -INFINITY ? 0.0f : ex2(y.x - top);
+                m_run = top;
+                l_run = l_run * f0 + y.y * f1;
+            }
+        }
         const bool part = rg.n > 1;
         const float inv = part ? 1.0f : (l_run == 0.0f ? 0.0f : 1.0f / l_run);
+        f0 *= inv;
+        f1 *= inv;
         const long long row = (long long)(s.q0 + tok) * a.Hq + head;
-        if (row_ok && ok) {
+        if (row_ok && ok && (t == 0 || two)) {
             if (part)
                 reinterpret_cast<float2 *>(tl.part_ml)[(long long)split * a.kv.n_tokens * a.Hq + row] =
                     make_float2(m_run, l_run);
@@ -383,7 +407,13 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
                         }
                         float y[32];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(o[i]) * inv;
+                        for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(o[i]) * f0;
+                        if (join) {
+                            tmem_ld32(o_addr + D + c0 / (f16 ? 2 : 4) + c * 32, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) y[i] = fmaf(__uint_as_float(o[i]), f1, y[i]);
+                        }
                         if (f16) {
 #pragma unroll
                             for (int q = 0; q < 4; ++q)
@@ -438,34 +468,37 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
                 if (!mine || it >= n_iter || y > rg.hi || y + rows_box <= rg.lo) return -1;
                 return max(paged_page(a.kv, b, y), 0);
             };
-            int issued = 0, next = page_at(0);
+            // K's stage is free after Q K^T, V's after P V: K is loaded first
+            int issued[2] = {0, 0}, next = page_at(0);
             for (int it = 0; it < n_iter; ++it) {
                 const int st = it % C::STAGES, cur = next;
                 next = page_at(it + 1);
-                if (it >= C::STAGES &&
-                    !__all_sync(0xffffffffu, mbar_wait(&kv_empty[st], ((it / C::STAGES) - 1) & 1, a.kv.err, VTX_KERR_KV)))
-                    break;
-                issued = it + 1;
                 const unsigned live = __ballot_sync(0xffffffffu, cur >= 0);
-                if (lane == 0) {
-                    const int n = __popc(live) / 2;                         // K's boxes; V has the same
-                    mbar_arrive_expect_tx(&k_full[st], (uint32_t)(n * rows_box * 128));
-                    mbar_arrive_expect_tx(&v_full[st], (uint32_t)(n * rows_box * 128));
+                const uint32_t bytes = (uint32_t)(__popc(live) / 2 * rows_box * 128);       // of K's boxes; V has the same
+                const int y = ((jb + it) * KEYS + pg * rows_box & mask) * rows;
+                bool good = true;
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    if (it >= C::STAGES)
+                        good = __all_sync(0xffffffffu, mbar_wait(kv ? &v_empty[st] : &k_empty[st],
+                                                                 ((it / C::STAGES) - 1) & 1, a.kv.err, VTX_KERR_KV));
+                    if (!good) break;
+                    issued[kv] = it + 1;
+                    uint64_t *bar = kv ? &v_full[st] : &k_full[st];
+                    if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+                    __syncwarp();
+                    if (cur >= 0 && kvsel == kv)
+                        tma_load_4d(smem + (kv ? C::V_OFF : C::K_OFF) + st * C::TILE + sub * 16384 + pg * rows_box * 128,
+                                    kv ? &tmV : &tmK, bar, sub * 64, y, g, cur);
+                    __syncwarp();
                 }
-                __syncwarp();
-                if (cur >= 0) {
-                    const int y = ((jb + it) * KEYS + pg * rows_box & mask) * rows;
-                    char *dst = smem + (kvsel ? C::V_OFF : C::K_OFF) + st * C::TILE + sub * 16384 + pg * rows_box * 128;
-                    if (kvsel) tma_load_4d(dst, &tmV, &v_full[st], sub * 64, y, g, cur);
-                    else tma_load_4d(dst, &tmK, &k_full[st], sub * 64, y, g, cur);
-                }
-                __syncwarp();
+                if (!good) break;
             }
             // the last loads must have landed before shared memory is released
-            for (int it = max(0, issued - C::STAGES); it < issued; ++it) {
-                mbar_wait(&k_full[it % C::STAGES], (it / C::STAGES) & 1, a.kv.err, VTX_KERR_KV);
-                mbar_wait(&v_full[it % C::STAGES], (it / C::STAGES) & 1, a.kv.err, VTX_KERR_KV);
-            }
+            for (int kv = 0; kv < 2; ++kv)
+                for (int it = max(0, issued[kv] - C::STAGES); it < issued[kv]; ++it)
+                    mbar_wait(kv ? &v_full[it % C::STAGES] : &k_full[it % C::STAGES], (it / C::STAGES) & 1, a.kv.err,
+                              VTX_KERR_KV);
             if (a.q_f16 && n_iter > 0) mbar_wait(q_full, 0, a.kv.err, VTX_KERR_Q);
         } else if (warp == C::MMA_WARP && n_iter > 0) {
             // =================== MMA issuer (warp converged, one elected lane) =
@@ -478,11 +511,11 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
             const uint32_t lo_k = ((sbase + C::K_OFF) >> 4) | (1u << 16);
             const uint32_t lo_v = ((sbase + C::V_OFF) >> 4) | ((16384u >> 4) << 16);   // LBO: next 64 columns
             constexpr uint32_t T16 = C::TILE >> 4;
-            const int nt = two ? 2 : 1;
+            const int nt = two ? 2 : min(2, n_iter);                    // warpgroups at work
             bool good = __all_sync(0xffffffffu, mbar_wait(q_full, 0, a.kv.err, VTX_KERR_Q));
             tc_fence_after();
-            auto issue_qk = [&](int t, int st) {
-                const uint32_t d = tmem + C::s_col(t), q = lo_q + t * T16, k = lo_k + st * T16;
+            auto issue_qk = [&](int qt, int t, int st) {                // Q tile qt into warpgroup t's S
+                const uint32_t d = tmem + C::s_col(t), q = lo_q + qt * T16, k = lo_k + st * T16;
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
                     const uint32_t ko = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
@@ -496,25 +529,55 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
                 for (int kk = 0; kk < 8; ++kk)
                     mma_f16_ts_w(lead, d, p + kk * 8, desc64(v + kk * (2048 >> 4), HI), IDESC_PV, kk > 0 ? 1u : acc);
             };
-            for (int it = 0; it <= n_iter && good; ++it) {
-                const int st = it % C::STAGES, pst = (it + C::STAGES - 1) % C::STAGES;
-                for (int t = 0; t < nt && good; ++t) {
-                    if (it > 0) {
-                        if (t == 0) good = __all_sync(0xffffffffu, mbar_wait(&v_full[pst], ((it - 1) / C::STAGES) & 1, a.kv.err, VTX_KERR_KV));
-                        if (good) good = __all_sync(0xffffffffu, mbar_wait(&p_full[t], (it - 1) & 1, a.kv.err, VTX_KERR_P));
+            auto wait_k = [&](int it) {
+                return __all_sync(0xffffffffu, mbar_wait(&k_full[it % C::STAGES], (it / C::STAGES) & 1, a.kv.err, VTX_KERR_KV));
+            };
+            auto wait_v = [&](int it) {
+                return __all_sync(0xffffffffu, mbar_wait(&v_full[it % C::STAGES], (it / C::STAGES) & 1, a.kv.err, VTX_KERR_KV));
+            };
+            auto wait_p = [&](int t, int i) {
+                return __all_sync(0xffffffffu, mbar_wait(&p_full[t], i & 1, a.kv.err, VTX_KERR_P));
+            };
+            if (two) {
+                for (int it = 0; it <= n_iter && good; ++it) {
+                    for (int t = 0; t < 2 && good; ++t) {
+                        if (it > 0) {
+                            if (t == 0) good = wait_v(it - 1);
+                            if (good) good = wait_p(t, it - 1);
+                            if (!good) break;
+                            tc_fence_after();
+                            issue_pv(t, (it - 1) % C::STAGES, it > 1 ? 1u : 0u);
+                            if (it == n_iter) mma_commit_w(lead, &o_tile[t]);
+                        }
+                        if (it < n_iter) {
+                            if (t == 0) good = wait_k(it);
+                            if (!good) break;
+                            tc_fence_after();
+                            issue_qk(t, t, it % C::STAGES);
+                        }
+                    }
+                    if (good && it > 0) mma_commit_w(lead, &v_empty[(it - 1) % C::STAGES]);
+                    if (good && it < n_iter) mma_commit_w(lead, &k_empty[it % C::STAGES]);
+                }
+            } else {                               // key tile i is warpgroup i % 2's
+                for (int it = 0; it < n_iter + 2 && good; ++it) {
+                    const int t = it & 1, j = it - 2;
+                    if (j >= 0) {
+                        good = wait_v(j) && wait_p(t, j >> 1);
                         if (!good) break;
                         tc_fence_after();
-                        issue_pv(t, pst, it > 1 ? 1u : 0u);
-                        if (it == n_iter) mma_commit_w(lead, &o_tile[t]);
+                        issue_pv(t, j % C::STAGES, j > 1 ? 1u : 0u);
+                        if (j + 2 >= n_iter) mma_commit_w(lead, &o_tile[t]);
+                        mma_commit_w(lead, &v_empty[j % C::STAGES]);
                     }
                     if (it < n_iter) {
-                        if (t == 0) good = __all_sync(0xffffffffu, mbar_wait(&k_full[st], (it / C::STAGES) & 1, a.kv.err, VTX_KERR_KV));
+                        good = wait_k(it);
                         if (!good) break;
                         tc_fence_after();
-                        issue_qk(t, st);
+                        issue_qk(0, t, it % C::STAGES);
+                        mma_commit_w(lead, &k_empty[it % C::STAGES]);
                     }
                 }
-                if (good && it > 0) mma_commit_w(lead, &kv_empty[pst]);
             }
             if (!good) {                           // release the write-back after a failed wait
                 for (int t = 0; t < nt; ++t) mma_commit_w(lead, &o_tile[t]);
