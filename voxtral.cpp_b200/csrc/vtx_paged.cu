@@ -215,23 +215,26 @@ TilePlan plan_tile(const vtx_paged_kv *p, int G, int Hq, int min_rows, int sms) 
     // streams with more than min_rows rows, and what rounding each up to whole groups adds
     const long long streams = std::min<long long>(p->n_seq, p->n_tokens / (min_rows / G + 1));
     auto groups_of = [&](long long tokens) { return (p->n_tokens + streams * (tokens - 1)) / tokens; };
-    // single Q tiles over short caches while they fit on the SMs at once (a prompt of
-    // 391 tokens, 8 KV heads: 104 CTAs instead of 56, 14.8 us instead of 15.9; over
-    // 14k keys pairs win, which share K and V and the tensor core: 512 tokens 154
-    // against 211 us)
-    const long long pair = groups_of(t.tile.T) * Hkv <= sms && p->max_kv_len <= 1024 ? t.tile.T : 2 * t.tile.T;
+    // single Q tiles while they fit on the SMs at once (a prompt of 391 tokens, 8 KV
+    // heads: 104 CTAs instead of 56, 13.3 us instead of 15.9; 391 at 1600 rows 27 and
+    // 36, 512 at 13.8k 133 and 139); beyond that pairs, which share K and V (2048 at
+    // 14k: 504 us)
+    const long long pair = groups_of(t.tile.T) * Hkv <= sms ? t.tile.T : 2 * t.tile.T;
     t.tile.tokens = (int)pair;
     t.tile.groups = (int)groups_of(pair);
     t.tile.min_tiles = 2;
     // Splits of a group's key tiles: the number of least estimated time.  A key
-    // tile of a group takes about 2.1 us (D = 128), a CTA's start and end 6; a
-    // merge writes and reads a split's rows at about 5 TB/s and costs a launch.
+    // tile of a group takes about 2.1 us (D = 128), half of that where the group is
+    // one Q tile (32 tokens at 700 rows: 17.9 us by 2.1, 15.0 by 1.0), a CTA's start
+    // and end 6; a merge writes and reads a split's rows at about 5 TB/s and costs a
+    // launch.
     // One stream: its groups are about equal, so whole waves count, and full waves
     // are left whole.  Several: lengths spread, so the average load plus half a
     // CTA's time.
     t.tile.shift = t.unpack ? 6 : 7;
     const int tiles = std::max(1, (p->max_kv_len + (1 << t.tile.shift) - 1) >> t.tile.shift);
-    const double tile_us = D == 128 ? 2.1 : 1.6, cta_us = 6.0;
+    const bool one_tile = pair == t.tile.T || p->max_new <= t.tile.T;
+    const double tile_us = (one_tile ? 1.0 : 2.1) * (D == 128 ? 1.0 : 0.76), cta_us = 6.0;
     const double row_us = (double)D * 8 / 5e6;               // one row, one split
     const long long items = (long long)t.tile.groups * Hkv;
     double best = 1e30, one = 1e30;
