@@ -344,10 +344,15 @@ int launch_tile_any(const CUtensorMap (&m)[3], const PagedAttnArgs &a, const Til
     return uf ? launch_tile<D, true, false>(m, a, t.tile, st) : launch_tile<D, false, false>(m, a, t.tile, st);
 }
 
+// A warp per query row for few rows (20 tokens of 32 heads at 12k rows 28.3 -> 24.3
+// us, 70 at 6k 29.9 -> 27.5), else per four of them, which look the stream up once
+// (192 tokens: 32.8 us, a warp per row 33.9).
 template <int D>
-int launch_tile_combine(const PagedAttnArgs &a, const PagedTile &tl, cudaStream_t st) {
-    return launch_pdl(fa_paged_tile_combine_kernel<D>, dim3((unsigned)a.kv.n_tokens, (unsigned)((a.Hq + 31) / 32)),
-                      dim3(256), 0, st, a, tl);
+int launch_tile_combine(const PagedAttnArgs &a, const PagedTile &tl, int sms, cudaStream_t st) {
+    const unsigned T = (unsigned)a.kv.n_tokens, Hq = (unsigned)a.Hq;
+    if ((long long)T * Hq <= 16LL * sms)
+        return launch_pdl(fa_paged_tile_combine_kernel<D, 1>, dim3(T, (Hq + 7) / 8), dim3(256), 0, st, a, tl);
+    return launch_pdl(fa_paged_tile_combine_kernel<D, 4>, dim3(T, (Hq + 31) / 32), dim3(256), 0, st, a, tl);
 }
 
 template <int D, int KVT>
@@ -573,7 +578,7 @@ int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, si
         if (rc != VTX_OK) return rc;
     }
     if (!tp.use || tp.tile.n_splits == 1) return VTX_OK;
-    return d64 ? launch_tile_combine<64>(ta, tp.tile, st) : launch_tile_combine<128>(ta, tp.tile, st);
+    return d64 ? launch_tile_combine<64>(ta, tp.tile, ds->sms, st) : launch_tile_combine<128>(ta, tp.tile, ds->sms, st);
 }
 
 int vtx_kv_score_paged(const vtx_kv_score_paged_args *p, void *stream) {
