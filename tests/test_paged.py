@@ -597,6 +597,40 @@ def test_attend_q8_chunks_round_p_alone(streams, D, kw, opt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kv_type", ["f16", "q8_0"])
+@pytest.mark.parametrize("new,D,Hq,Hkv,opt", [
+    (20, 128, 8, 2, {}), (33, 64, 8, 2, dict(window=190)), (17, 128, 8, 8, dict(causal=False)),
+    (9, 64, 16, 1, dict(softcap=4.0)), (40, 128, 8, 2, {})])
+def test_attend_one_query_tile(kv_type, new, D, Hq, Hkv, opt):
+    """One Q tile over an odd and an even number of key tiles, alone and together, one
+    stream with fewer rows than tokens."""
+    lengths = [new, 127, 128, 200, 300, 500, 650, 1300, 7]
+    c = R.build(37, kv_type, [(new, n) for n in lengths], Hq, Hkv, D, 32)
+    q, named = torch.from_numpy(c["q"]).cuda(), {("logit_softcap" if k == "softcap" else k): v for k, v in opt.items()}
+    ref = R.attend(c, **opt)
+    tol, ltol = R.attend_tolerance(ref, 1)
+    # Q8_0 below 96 rows: P is rounded after V's scale went in, with subnormals of its own
+    tol = tol + ref[4] * 2.0 ** -24
+    up = lambda x: torch.from_numpy(np.ascontiguousarray(x)).cuda()  # noqa: E731
+    out = torch.empty(q.shape, dtype=torch.float32, device="cuda")
+    lse = torch.empty(q.shape[:2], device="cuda")
+    one, one_lse = torch.empty_like(out), torch.empty_like(lse)
+    kv = device_kv(c)
+    kv.attend(q, out=out, lse=lse, **named)
+    for s, n in enumerate(lengths):
+        rows = slice(s * new, (s + 1) * new)
+        alone = V.PagedKv(kv.k_pool, kv.v_pool, up(c["table"][s:s + 1]), up(np.array([n], np.int32)),
+                          up(np.array([0, new], np.int32)), Hq, n_tokens=new, max_new=new, max_kv_len=n)
+        alone.attend(q[rows].float(), out=one[rows], lse=one_lse[rows], **named)
+    for o, e in ((out, lse), (one, one_lse)):
+        o, e = o.double().cpu().numpy(), e.double().cpu().numpy()
+        assert (np.abs(o - ref[0]) <= tol).all()
+        fin = np.isfinite(ref[1])
+        assert np.array_equal(np.isneginf(e), ~fin) and (np.abs(e[fin] - ref[1][fin]) <= ltol[fin]).all()
+    assert V.read_device_error() == 0
+
+
+@pytest.mark.gpu
 def test_unpacked_cache_past_its_bound():
     """A chunk over a Q8_0 cache that is unpacked: lengths up to whole pages above
     max_kv_len are served, longer ones reported."""
