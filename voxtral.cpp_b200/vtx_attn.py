@@ -462,6 +462,7 @@ class PagedKv:
         if k_pool.dtype not in (torch.float16, torch.uint8):
             raise VtxError(-2, "pools must be float16 or Q8_0 bytes")
         self.dev, self._on = k_pool.device, k_pool.get_device()
+        self._only = self.dev.type == "cuda" and torch.cuda.device_count() == 1      # always the current one
         n_seq = kv_len.shape[0]
         for t, shape in ((page_table, (n_seq, page_table.shape[-1])), (kv_len, (n_seq,)), (q_start, (n_seq + 1,))):
             if t.dtype != torch.int32 or not t.is_contiguous() or t.device != self.dev or tuple(t.shape) != shape:
@@ -504,6 +505,7 @@ class PagedKv:
         self._score, self._evict = KvScorePagedArgs(), KvEvictPagedArgs()
         for a in (self._append, self._attend, self._score, self._evict):
             a.kv = adr
+        self._refs = [ctypes.byref(a) for a in (self._append, self._attend, self._score, self._evict)]
         self._attend.q, self._attend.dst, self._attend.params = at(self._q), at(self._dst), at(self._params)
         self._score.q, self._score.params = at(self._q), at(self._params)
 
@@ -528,7 +530,7 @@ class PagedKv:
     def _rows(self, t: torch.Tensor, what: str, d: VtxTensor, nb, token: int, head: int) -> None:
         """Puts a (n_tokens, n_head_q, D) float32 / float16 view into descriptor d."""
         st, kind = t.stride(), _ROW_TYPES.get(t.dtype)
-        if t.shape != self._q_shape or st[2] != 1 or t.device != self.dev:
+        if t.shape != self._q_shape or st[2] != 1 or t.get_device() != self._on:
             raise VtxError(-3, f"{what} must be {self._q_shape} on {self.dev}, last axis contiguous")
         if kind is None:
             raise VtxError(-2, f"{what}: dtype {t.dtype}")
@@ -541,7 +543,7 @@ class PagedKv:
             return cap
         shape = t.shape
         if len(shape) != 3 or shape[0] != self.n_seq or shape[1] != self.n_head_kv or t.dtype != dtype or \
-                not t.is_contiguous() or t.device != self.dev or (cap is not None and shape[2] != cap):
+                not t.is_contiguous() or t.get_device() != self._on or (cap is not None and shape[2] != cap):
             raise VtxError(-3, f"{what} must be a contiguous ({self.n_seq}, {self.n_head_kv}, rows) {dtype} tensor")
         return shape[2]
 
@@ -560,12 +562,12 @@ class PagedKv:
         dev = self.dev
         if dev.type != "cuda":
             raise VtxError(-8, "the pools are not on a GPU")
-        s = stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(dev.index)
-        if torch._C._cuda_getDevice() == dev.index:
-            rc = fn(ctypes.byref(args), *ws, s)
+        s = stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._on)
+        if self._only or torch._C._cuda_getDevice() == self._on:
+            rc = fn(args, *ws, s)
         else:
             with torch.cuda.device(dev):
-                rc = fn(ctypes.byref(args), *ws, s)
+                rc = fn(args, *ws, s)
         if rc != 0:
             raise VtxError(rc, fn.__name__)
 
@@ -608,7 +610,7 @@ class PagedKv:
         a.row_cap = self._array(score, torch.float32, "score", self._array(row_pos, torch.int32, "row_pos", None)) or 0
         a.row_pos = row_pos.data_ptr() if row_pos is not None else None
         a.score = score.data_ptr() if score is not None else None
-        self._call(self._lib.vtx_kv_append_paged, a, stream)
+        self._call(self._lib.vtx_kv_append_paged, self._refs[0], stream)
         return q_out
 
     def attend(self, q: torch.Tensor, out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, *,
@@ -624,7 +626,7 @@ class PagedKv:
         self._rows(out, "out", self._dst, self._dst_nb, 2, 1)
         self._set_params(scale, causal, window, logit_softcap)
         self._attend.lse = self._check_lse(lse) if lse is not None else None
-        self._call(self._lib.vtx_flash_attn_paged, self._attend, stream, *self._ws)
+        self._call(self._lib.vtx_flash_attn_paged, self._refs[1], stream, *self._ws)
         return out
 
     def _check_lse(self, lse: torch.Tensor) -> int:
@@ -647,7 +649,7 @@ class PagedKv:
         a = self._score
         a.lse, a.score, a.score_out = self._check_lse(lse), score.data_ptr(), out.data_ptr()
         a.row_cap, a.observe, a.decay = cap, observe, decay
-        self._call(self._lib.vtx_kv_score_paged, a, stream)
+        self._call(self._lib.vtx_kv_score_paged, self._refs[2], stream)
         return out
 
     def evict(self, score: torch.Tensor, keep: int, kv_len_out: Optional[torch.Tensor] = None, *, n_sink: int = 0,
@@ -673,7 +675,7 @@ class PagedKv:
         a.score, a.row_pos, a.next_pos, a.kv_len_out = score.data_ptr(), ptr(row_pos), ptr(next_pos), kv_len_out.data_ptr()
         a.score_out, a.pos_out, a.src_out = ptr(score_out), ptr(pos_out), ptr(src_out)
         a.keep, a.n_sink, a.n_recent = keep, n_sink, n_recent
-        self._call(self._lib.vtx_kv_evict_paged, a, stream, *self._evict_ws)
+        self._call(self._lib.vtx_kv_evict_paged, self._refs[3], stream, *self._evict_ws)
         return kv_len_out
 
 
