@@ -92,8 +92,8 @@ __device__ __forceinline__ void evict_move(const PagedEvictArgs &a, const int2 *
 // owns a run of rows and walks it 128 at a time, four consecutive rows per lane, so
 // a scan over the lanes numbers the gaps and the moved rows in row order.  Bound by
 // latency: about a dozen barriers and four dependent trips to memory per (stream,
-// head).  Keys are read four at a time: 64 items of 1500 to 8192 rows take 24.6
-// us with their moves, 38 a row at a time.
+// head), so rows are read four at a time and four such loads together (64 items of
+// 1500 to 8192 rows with their moves 38 -> 24.6 -> 22.6 us, 256 items 78 -> 71).
 template <bool SMEM, int UNIT>
 __global__ void __launch_bounds__(kEvictThreads)
 kv_evict_select_kernel(const PagedEvictArgs a)
@@ -146,20 +146,34 @@ kv_evict_select_kernel(const PagedEvictArgs a)
         }
     };
     // keys of rows 4q ... 4q + 3; 0, below every key, behind the last row
-    auto make4 = [&](int q) {
-        float s[4];
-        int p[4];
+    auto key4 = [&](int q, const float (&s)[4], const int (&p)[4]) {
         uint32_t k[4];
-        load4(q, s, p);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             k[i] = 4 * q + i < n ? evict_key(s[i], p[i] < a.n_sink || p[i] >= recent) : 0u;
         return make_uint4(k[0], k[1], k[2], k[3]);
     };
+    auto make4 = [&](int q) {
+        float s[4];
+        int p[4];
+        load4(q, s, p);
+        return key4(q, s, p);
+    };
     auto keys4 = [&](int q) { return SMEM ? reinterpret_cast<const uint4 *>(keys)[q] : make4(q); };
     const bool some = m > 0 && m < n;              // there is a choice to make
-    if (SMEM && some)
-        for (int q = tid; q < n4; q += kEvictThreads) reinterpret_cast<uint4 *>(keys)[q] = make4(q);
+    constexpr int B = UNIT == 0 ? 4 : 1;           // trips to memory at once (UNIT > 0: one is all there is)
+    if (SMEM && some) {
+        for (int qb = tid; qb < n4; qb += B * kEvictThreads) {
+            float s[B][4];
+            int p[B][4];
+#pragma unroll
+            for (int i = 0; i < B; ++i)
+                if (qb + i * kEvictThreads < n4) load4(qb + i * kEvictThreads, s[i], p[i]);
+#pragma unroll
+            for (int i = 0; i < B; ++i)
+                if (const int q = qb + i * kEvictThreads; q < n4) reinterpret_cast<uint4 *>(keys)[q] = key4(q, s[i], p[i]);
+        }
+    }
     uint32_t prefix = 0;
     int need = m;                                  // rank of the threshold among the keys that match the prefix
     bool ties = false;                             // not all keys equal to the threshold stay
@@ -317,11 +331,26 @@ kv_evict_select_kernel(const PagedEvictArgs a)
         }
     });
     __syncthreads();
-    for (int i = tid; i < tot.x; i += kEvictThreads) {
-        const int2 x = mv[i];
-        if (so) so[x.y] = score[x.x];
-        if (po) po[x.y] = row_pos ? row_pos[x.x] : x.x;
-        if (ro) ro[x.y] = x.x;
+    for (int ib = tid; ib < tot.x; ib += B * kEvictThreads) {
+        int2 x[B];
+        float s[B];
+        int p[B];
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+            if (ib + i * kEvictThreads < tot.x) x[i] = mv[ib + i * kEvictThreads];
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            if (ib + i * kEvictThreads >= tot.x) break;
+            if (so) s[i] = score[x[i].x];
+            p[i] = po && row_pos ? row_pos[x[i].x] : x[i].x;
+        }
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            if (ib + i * kEvictThreads >= tot.x) break;
+            if (so) so[x[i].y] = s[i];
+            if (po) po[x[i].y] = p[i];
+            if (ro) ro[x[i].y] = x[i].x;
+        }
     }
     if constexpr (UNIT == 0) {
         if (tid == 0) a.counts[item] = make_int2(tot.x, m);
