@@ -24,8 +24,8 @@
 //
 // LO: an unpacked Q8_0 cache, whose tiles hold 64 keys as 64 rows of hi and 64 of lo
 // (value = hi + lo).  S's two halves are added before the softmax and P is stored
-// twice, so both products stay as they are; 2048 tokens at 14k keys 1017 us next to
-// 516 over F16 pages, as twice the products have it.
+// twice, so both products stay as they are; 2048 tokens at 14k keys 833 us next to
+// 502 over F16 pages, for twice the products.
 //
 // D = 64, twice the exponentials per flop: a quarter of them runs on the FMA pipe
 // (2048 tokens at 14k keys 446 -> 430 us; D = 128 gained nothing, 519 us either way,

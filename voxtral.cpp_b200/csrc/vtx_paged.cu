@@ -217,8 +217,7 @@ TilePlan plan_tile(const vtx_paged_kv *p, int G, int Hq, int min_rows, int sms) 
     auto groups_of = [&](long long tokens) { return (p->n_tokens + streams * (tokens - 1)) / tokens; };
     // single Q tiles while they fit on the SMs at once (a prompt of 391 tokens, 8 KV
     // heads: 104 CTAs instead of 56, 13.3 us instead of 15.9; 391 at 1600 rows 27 and
-    // 36, 512 at 13.8k 133 and 139); beyond that pairs, which share K and V (2048 at
-    // 14k: 504 us)
+    // 36, 512 at 13.8k 133 and 139); beyond that pairs, which share K and V
     const long long pair = groups_of(t.tile.T) * Hkv <= sms ? t.tile.T : 2 * t.tile.T;
     t.tile.tokens = (int)pair;
     t.tile.groups = (int)groups_of(pair);
@@ -248,8 +247,8 @@ TilePlan plan_tile(const vtx_paged_kv *p, int G, int Hq, int min_rows, int sms) 
                                   (s > 1 ? (items - whole) * 256.0 * s * row_us + 3.0 : 0.0);
                 if (s == 1) one = us;
                 // launches of full waves are short of power, not of SMs: a small gain
-                // is none there (2048 tokens at 14k: 519 us whole, 530 with the last
-                // wave split; 1184 tokens: 394 and 290)
+                // is none there (2048 tokens at 14k: 501 us whole, 516 with the last
+                // wave split; 1184 tokens: 360 and 287)
                 if (us < best && (s == 1 || items < sms || us < 0.85 * one)) {
                     best = us;
                     t.tile.n_splits = s;
