@@ -397,7 +397,9 @@ VTX_API int vtx_attn_out_proj(const vtx_out_proj_args *args, void *stream);
  *   that is outside [0, n_pages) is reported through vtx_read_device_error;
  *   reads then take page 0 and writes are dropped.
  * - kv_len[s]: rows of stream s, this step's new ones included; at most
- *   max_pages * page_size (a longer one is reported and cut there).
+ *   max_pages * page_size.  A longer one is reported; its tokens keep their
+ *   rows, and rows behind the table do not exist: append drops them, and no
+ *   token sees them.
  * - q_start: stream s brings the tokens [q_start[s], q_start[s+1]) of the
  *   packed token arrays, possibly none; n of them go to (append) or stand in
  *   (the other calls) its rows kv_len[s] - n ... kv_len[s] - 1.  A token whose

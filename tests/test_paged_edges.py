@@ -1,0 +1,116 @@
+"""The paged decoder cache at the edges of what its header allows."""
+import numpy as np
+import pytest
+
+import paged_ref as R
+import vtx_attn as V
+from test_paged import BASE, device_kv
+
+torch = pytest.importorskip("torch")
+
+
+def up(x):
+    return torch.from_numpy(np.ascontiguousarray(x)).cuda()
+
+
+def close(got, want, tol):
+    got = got.double().cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        bad = ~((np.abs(got - want) <= tol) | (np.isneginf(got) & np.isneginf(want)))
+    assert not bad.any(), f"{bad.sum()} of {bad.size} out of bounds, first at {np.argwhere(bad)[0]}"
+
+
+# ---- a kv_len above the table's capacity --------------------------------------------
+
+def beyond(seed, kv_type, streams, page, *shape):
+    """A case whose tables end at their last whole page, and its lengths with `streams`' third entries added."""
+    c = R.build(seed, kv_type, [x[:2] for x in streams], *shape, page, poison=False)
+    most = max(c["len"]) // page
+    c["table"] = np.ascontiguousarray(c["table"][:, :most])
+    c["len"] = [x[1] + x[2] for x in streams]
+    return c, most * page
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_type", ["f16", "q8_0"])
+@pytest.mark.parametrize("new,over", [(1, 1), (1, 40), (3, 1), (5, 3), (40, 7), (40, 90)])
+def test_append_beyond_the_table_is_dropped(kv_type, new, over):
+    """Token i of n goes to row kv_len - n + i; one at or behind the capacity is
+    dropped and reported, and the rows in front of it are not touched."""
+    c, cap = beyond(50, kv_type, [(new, 64, over), (2, 30, 0)], 16, 8, 2, 128)
+    kv = device_kv(c, max_kv_len=cap)
+    before = [p.clone() for p in (kv.k_pool, kv.v_pool)]
+    f = lambda h: torch.randn(new + 2, h, 128, device="cuda")  # noqa: E731
+    score, row_pos = torch.full((2, 2, cap), 9.0, device="cuda"), torch.full((2, 2, cap), -9, dtype=torch.int32, device="cuda")
+    k, v, pos = f(2), f(2), torch.arange(1000, 1002 + new, dtype=torch.int32, device="cuda")
+    kv.append(k, v, pos, BASE, row_pos=row_pos, score=score)
+    assert V.read_device_error() == 41
+    want_pos = np.full((2, 2, cap), -9)
+    for t in range(new):
+        if cap + over - new + t < cap:
+            want_pos[0, :, cap + over - new + t] = 1000 + t
+    want_pos[1, :, 28:30] = [1000 + new, 1001 + new]
+    assert np.array_equal(row_pos.cpu().numpy(), want_pos)
+    assert np.array_equal(score.cpu().numpy(), np.where(want_pos >= 0, 0.0, 9.0))
+    written = {(int(c["table"][s, r // 16]), r % 16) for s in (0, 1) for r in np.flatnonzero(want_pos[s, 0] >= 0)}
+    for now, old in zip((kv.k_pool, kv.v_pool), before):
+        changed = (now.view(torch.uint8) != old.view(torch.uint8)).any(3).any(1)
+        assert {tuple(x) for x in changed.nonzero().tolist()} == written
+
+
+BEYOND = [
+    ("f16", [(1, 64, 3), (2, 30, 0)], 8, 2, 128, {}), ("q8_0", [(4, 64, 2), (1, 64, 9)], 8, 2, 64, {}),
+    ("f16", [(1, 960, 5)], 8, 2, 128, dict(window=40)), ("f16", [(4, 64, 40), (1, 20, 0)], 8, 2, 128, dict(window=20)),
+    ("f16", [(40, 64, 9), (1, 33, 0)], 8, 2, 128, {}), ("f16", [(300, 960, 100)], 8, 2, 64, dict(window=130)),
+    ("f16", [(40, 64, 60)], 8, 2, 128, dict(window=10)), ("f16", [(40, 64, 9), (3, 50, 0)], 8, 2, 128, dict(causal=False)),
+    ("q8_0", [(40, 64, 9), (1, 33, 0)], 8, 2, 128, {}), ("q8_0", [(40, 64, 60)], 8, 2, 128, dict(window=10)),
+    ("q8_0", [(90, 960, 20), (1, 100, 0)], 8, 2, 64, {}), ("q8_0", [(90, 960, 70)], 8, 2, 128, dict(window=50)),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", range(len(BEYOND)))
+def test_attend_and_score_beyond_the_table(i):
+    """A stream longer than its table keeps its tokens' rows: each sees the rows that exist of those it may see."""
+    kv_type, streams, Hq, Hkv, D, opt = BEYOND[i]
+    c, cap = beyond(60 + i, kv_type, streams, 16, Hq, Hkv, D)
+    kv = device_kv(c, max_kv_len=cap)
+    q = up(c["q"])
+    lse = torch.empty(q.shape[:2], device="cuda")
+    out = kv.attend(q, lse=lse, **opt)
+    assert V.read_device_error() == 41
+    ref = R.attend(c, **opt)
+    tol, ltol = R.attend_tolerance(ref, 1)
+    close(out, ref[0], tol + ref[4] * 2.0 ** -22)
+    close(lse, ref[1], ltol)
+    c["len"] = [min(n, cap) for n in c["len"]]                # rows that the sums run over
+    for x in (q, q.float()):
+        got = kv.score(x, up(ref[1].astype(np.float32)), torch.zeros(len(streams), Hkv, cap, device="cuda"), **opt)
+        assert V.read_device_error() == 41
+        want, stol = score_beyond(c, streams, ref[1].astype(np.float32), cap, opt)
+        close(got, want, stol)
+
+
+def score_beyond(c, streams, lse, cap, opt):
+    """R.score with the rows' offsets of the uncut lengths."""
+    want, tol = np.zeros((2, len(streams), c["Hkv"], cap))
+    for s, (new, n, over) in enumerate(streams):
+        one = dict(c, len=[n + over], table=c["table"][s:s + 1], start=np.array([0, new], np.int32),
+                   q=c["q"][c["start"][s]:c["start"][s + 1]])
+        wide = cap + over                                       # entries behind the table stay 0
+        kr = R.values(R.rows_of(c["k_pool"], c["table"][s], c["len"][s]))
+        rows = c["len"][s]
+        for h in range(c["Hq"]):
+            q = one["q"][:, h].astype(np.float64)
+            k = kr[h // (c["Hq"] // c["Hkv"])]
+            x = R.scores(q, k, n + over - new, c["D"] ** -0.5, opt.get("causal", True), opt.get("window", 0), 0.0)
+            ls = lse[c["start"][s]:c["start"][s + 1], h].astype(np.float64)[:, None]
+            with np.errstate(invalid="ignore"):
+                p = np.where(np.isneginf(ls) | np.isneginf(x), 0.0, np.exp(x - ls))
+            e = (c["D"] + 8) * 2.0 ** -24 * c["D"] ** -0.5 * (np.abs(q) @ np.abs(k).T)
+            e = e + 2.0 ** -20 * (1 + np.where(np.isinf(x), 0, np.abs(x)) + np.abs(np.where(np.isinf(ls), 0, ls)))
+            g = h // (c["Hq"] // c["Hkv"])
+            want[s, g, :rows] += p.sum(0)
+            tol[s, g, :rows] += (p * e).sum(0)
+        assert wide >= rows
+    return want, tol + np.abs(want) * 2.0 ** -20 + 1e-30

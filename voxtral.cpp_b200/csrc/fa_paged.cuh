@@ -111,17 +111,17 @@ fa_paged_q8_kernel(const PagedAttnArgs a)
     const int r_first = blockIdx.x * 64;
     if (r_first >= rows || rows <= a.min_rows) return;
 
-    const int off = s.len - s.n_new;                        // row of token 0
+    const int off = s.off;                                  // row of token 0
     int row[2], tok[2], lo[2], hi[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         row[u] = r_first + warp * 16 + (lane >> 2) + 8 * u;
         tok[u] = row[u] / a.G;
-        hi[u] = row[u] < rows ? (a.causal ? off + tok[u] : s.len - 1) : -1;
+        hi[u] = row[u] < rows ? (a.causal ? min(off + tok[u], s.len - 1) : s.len - 1) : -1;
         lo[u] = a.window > 0 ? off + tok[u] - a.window + 1 : 0;
     }
     const int t_first = r_first / a.G, t_last = (min(r_first + 64, rows) - 1) / a.G;
-    const int k_hi = a.causal ? off + t_last : s.len - 1;
+    const int k_hi = a.causal ? min(off + t_last, s.len - 1) : s.len - 1;
     const int k_lo = a.window > 0 ? max(0, off + t_first - a.window + 1) : 0;
 
     uint32_t qa[KC][4];
@@ -274,8 +274,8 @@ paged_unpack_kernel(const PagedAttnArgs a, const PagedView out)
     __shared__ __align__(16) char raw[2 * 32 * ROW];
     const int b = blockIdx.z, g = blockIdx.y, r0 = blockIdx.x * 32;
     const PagedSeq s = paged_seq(a.kv, b);
-    const int end = min(s.len, out.max_pages << out.shift);
-    const int lo = a.window > 0 ? s.len - s.n_new - a.window + 1 : 0;
+    const int end = min(s.len, out.cap);
+    const int lo = a.window > 0 ? s.off - a.window + 1 : 0;
     if (s.n_new * a.G <= a.min_rows || r0 >= end || r0 + 32 <= lo) return;
     // groups of 16 rows are contiguous in a page
     constexpr int CH = 16 * ROW / 16;

@@ -62,7 +62,7 @@ struct PagedCut {
 };
 __device__ __forceinline__ PagedCut paged_cut(const PagedSeq &s, int causal, int window, const PagedSplit &sp) {
     PagedCut c;
-    c.lo = window > 0 && causal ? max(0, s.len - s.n_new - window + 1) & ~15 : 0;
+    c.lo = window > 0 && causal ? max(0, s.off - window + 1) & ~15 : 0;
     c.nt = max(0, s.len - c.lo + 15) >> 4;
     c.per = max(sp.tiles, (c.nt + sp.n_splits - 1) / sp.n_splits);
     c.n = max(1, (c.nt + c.per - 1) / c.per);
@@ -254,7 +254,7 @@ __device__ __forceinline__ void paged_decode_cta(const PagedAttnArgs &a, const P
     const int t_end = min(cut.per * (split + 1), cut.nt);
     const int first = cut.per * split + warp;                   // this warp's tiles: first, first + WARPS, ...
     const int nt = t_end > first ? (t_end - first + C::WARPS - 1) / C::WARPS : 0;
-    const int off = s.len - s.n_new;
+    const int off = s.off;
     const int lo_any = a.window > 0 ? max(0, off - a.window + 1) : 0;   // rows that some token sees
 
     if (lane < C::STAGES) mbar_init(&full[lane], 1);
@@ -315,12 +315,12 @@ __device__ __forceinline__ void paged_decode_cta(const PagedAttnArgs &a, const P
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int r2 = 8 * nc + 2 * c + j, tok2 = r2 / a.G;
-            hi[nc][j] = r2 < rows ? (a.causal ? off + tok2 : s.len - 1) : -1;
+            hi[nc][j] = r2 < rows ? (a.causal ? min(off + tok2, s.len - 1) : s.len - 1) : -1;
             lo[nc][j] = a.window > 0 ? off + tok2 - a.window + 1 : 0;
         }
     }
     // every token sees [lo_all, hi_all] (padding rows' results are not read)
-    const int hi_all = a.causal ? off : s.len - 1;
+    const int hi_all = a.causal ? min(off, s.len - 1) : s.len - 1;
     const int lo_all = a.window > 0 ? off + s.n_new - a.window : 0;
 
     float o[NC][KC][4];

@@ -106,9 +106,9 @@ struct PagedRange {
 __device__ __forceinline__ PagedRange paged_range(const PagedSeq &s, int tok0, const PagedAttnArgs &a,
                                                   const PagedTile &tl, bool cut) {
     PagedRange r;
-    const int off = s.len - s.n_new, last = min(s.n_new, tok0 + tl.tokens) - 1;
-    r.hi = a.causal ? off + last : s.len - 1;
-    r.lo = a.window > 0 ? max(0, off + tok0 - a.window + 1) : 0;
+    const int last = min(s.n_new, tok0 + tl.tokens) - 1;
+    r.hi = a.causal ? min(s.off + last, s.len - 1) : s.len - 1;
+    r.lo = a.window > 0 ? max(0, s.off + tok0 - a.window + 1) : 0;
     r.j0 = r.hi >= r.lo ? r.lo >> tl.shift : 0;
     r.j1 = r.hi >= r.lo ? (r.hi >> tl.shift) + 1 : 0;
     const int most = cut ? tl.n_splits : 1;
@@ -216,7 +216,7 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int off = s.len - s.n_new;
+    const int off = s.off;
 
     if (warp < 8) {
         setmaxnreg_inc<C::REG_SOFTMAX>();
@@ -229,7 +229,7 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
         bool ok = true;
         int lo = 1, hi = 0;
         if (row_ok) {
-            hi = a.causal ? off + tok : s.len - 1;
+            hi = a.causal ? min(off + tok, s.len - 1) : s.len - 1;
             lo = a.window > 0 ? max(0, off + tok - a.window + 1) : 0;
         }
         char *qtile = smem + C::Q_OFF + t * C::TILE;

@@ -108,7 +108,7 @@ kv_evict_select_kernel(const PagedEvictArgs a)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const long long item = blockIdx.x;
     const int n = a.kv.kv_len[b];
-    const int most = (int)min((long long)min(a.kv.max_kv, a.row_cap), (long long)a.kv.max_pages << a.kv.shift);
+    const int most = min(min(a.kv.max_kv, a.row_cap), a.kv.cap);
     if (n < 0 || n > most) {                       // nothing of this stream is touched
         if (tid == 0) {
             paged_report(a.kv, VTX_KERR_BOUND);

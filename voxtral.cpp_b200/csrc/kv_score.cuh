@@ -50,7 +50,7 @@ kv_score_kernel(const PagedScoreArgs a)
     const int k0 = blockIdx.x * 128 + warp * 32;
     if (k0 >= limit) return;
 
-    const int off = s.len - s.n_new;
+    const int off = s.off;
     int t0 = a.observe > 0 ? max(0, s.n_new - a.observe) : 0;
     const int lo_any = t0 < s.n_new ? (a.window > 0 ? off + t0 - a.window + 1 : 0) : limit;   // nobody sees keys below
 
@@ -185,11 +185,11 @@ kv_score_stream_kernel(const PagedScoreArgs a, const PagedSplit sp)
     if (threadIdx.x == 0 && split == 0 && (s.len > min(a.row_cap, a.kv.max_kv) || s.n_new > a.kv.max_new))
         paged_report(a.kv, VTX_KERR_BOUND);
     const int limit = min(s.len, a.row_cap);
-    const int off = s.len - s.n_new;
+    const int off = s.off;
     const int t0 = max(s.n_new - a.kv.max_new, a.observe > 0 ? max(0, s.n_new - a.observe) : 0);
     const int rows = (s.n_new - t0) * a.G;
     const int lo_any = rows == 0 ? limit : (a.window > 0 ? max(0, off + t0 - a.window + 1) : 0);
-    const PagedCut cut = paged_cut(PagedSeq{s.q0, s.n_new, limit}, 0, 0, sp);
+    const PagedCut cut = paged_cut(PagedSeq{s.q0, s.n_new, limit, off}, 0, 0, sp);
     if (split >= cut.n) return;
     const int t_end = min(cut.per * (split + 1), cut.nt);
     const int first = cut.per * split + warp;

@@ -90,7 +90,7 @@ kv_score_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     if (blockIdx.x == 0 && tid == 0 && s.len > min(a.row_cap, a.kv.max_kv)) paged_report(a.kv, VTX_KERR_BOUND);
     const int k0 = blockIdx.x * 128 * NT;
     if (k0 >= limit) return;
-    const int off = s.len - s.n_new;
+    const int off = s.off;
     const int ta = a.observe > 0 ? max(0, s.n_new - a.observe) : 0;     // first token that counts
     const int lo_any = ta < s.n_new ? (a.window > 0 ? max(0, off + ta - a.window + 1) : 0) : limit;
     int t0 = ta, t1 = s.n_new;

@@ -20,14 +20,17 @@ struct PagedView {
     const int *table, *kv_len, *q_start;   // table NULL: stream s owns pages s * max_pages ...
     int n_seq, n_tokens, max_new, max_kv;
     int max_pages, n_pages, shift;         // page_size = 1 << shift
+    int cap;                               // rows that a stream can have
     int Hkv;
     int *err;
 };
 
-// One stream's lengths, cut to what the arrays hold: tokens q0 .. q0 + n_new
-// of the packed arrays stand in rows len - n_new .. len - 1.
+// One stream: tokens q0 .. q0 + n_new of the packed arrays stand in rows off ..
+// off + n_new - 1, and its table holds the rows below len.  off follows the kv_len
+// as given, so a stream longer than its table keeps its tokens' rows: those at or
+// behind len do not exist.
 struct PagedSeq {
-    int q0, n_new, len;
+    int q0, n_new, len, off;
 };
 
 __device__ __forceinline__ void paged_report(const PagedView &kv, int code) {
@@ -39,8 +42,8 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedView &kv, int b) {
     const int a = kv.q_start[b], e = kv.q_start[b + 1], n = kv.kv_len[b];
     s.q0 = min(max(a, 0), kv.n_tokens);
     s.n_new = min(max(e, s.q0), kv.n_tokens) - s.q0;
-    const long long cap = (long long)kv.max_pages << kv.shift;
-    s.len = (int)min((long long)max(n, 0), cap);
+    s.len = min(max(n, 0), kv.cap);
+    s.off = max(n, 0) - s.n_new;
     if (s.len != n) paged_report(kv, VTX_KERR_BOUND);
     return s;
 }
@@ -203,7 +206,8 @@ kv_append_paged_kernel(const __grid_constant__ KvAppendPagedArgs a)
     int row = -1;
     if (b < a.kv.n_seq) {
         const PagedSeq s = paged_seq(a.kv, b);
-        if (t >= s.q0 && t < s.q0 + s.n_new) row = s.len - s.n_new + (t - s.q0);
+        if (t >= s.q0 && t < s.q0 + s.n_new) row = s.off + (t - s.q0);
+        if (row >= s.len) row = -1;                         // behind the table: dropped (and reported)
         if (row >= 0 && row >= a.row_cap && (a.row_pos || a.score)) {
             paged_report(a.kv, VTX_KERR_BOUND);
             row = -1;

@@ -70,6 +70,7 @@ PagedView view_of(const vtx_paged_kv *p, const DeviceState *ds) {
     v.n_seq = p->n_seq; v.n_tokens = p->n_tokens; v.max_new = p->max_new; v.max_kv = p->max_kv_len;
     v.max_pages = p->max_pages; v.n_pages = (int)p->k.ne[3];
     while ((1 << v.shift) < (int)p->k.ne[1]) ++v.shift;
+    v.cap = v.max_pages << v.shift;
     v.Hkv = (int)p->k.ne[2];
     v.err = ds->err;
     return v;
@@ -282,6 +283,7 @@ PagedView unpacked_view(const PagedView &kv, const TilePlan &t, int D, char *ws)
     u.table = nullptr;
     u.max_pages = t.unpack; u.n_pages = kv.n_seq * t.unpack;
     u.shift = 7;
+    u.cap = (int)std::min<long long>(kv.cap, (long long)t.unpack << 7);       // what was unpacked
     return u;
 }
 
