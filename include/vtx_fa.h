@@ -478,9 +478,12 @@ VTX_API int vtx_kv_append_paged(const vtx_kv_append_paged_args *args, void *stre
  * above max_kv_len is then reported.
  * workspace: 256-byte aligned, vtx_flash_attn_paged_workspace bytes (they
  * depend on kv's sizes and bounds and on n_head_q alone).  Zero it once before
- * its first call (cudaMemset): it holds arrival counters, which every call
- * leaves at zero; a call with other sizes or bounds needs it zeroed again.
- * Calls that share one must not overlap on the GPU. */
+ * its first call (cudaMemset): it begins with arrival counters, which every call
+ * leaves at zero.  One workspace, as large as the largest of them needs, serves
+ * calls of any sizes, bounds and caches in turn (those of several layers, prompts
+ * and single tokens), with up to 65536 pairs of a stream and a KV head; a call
+ * with more needs it zeroed again when one with fewer came between.  Calls that
+ * share one must not overlap on the GPU. */
 typedef struct vtx_flash_attn_paged_args {
     const vtx_paged_kv *kv;
     const vtx_tensor *q;

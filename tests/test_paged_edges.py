@@ -114,3 +114,41 @@ def score_beyond(c, streams, lse, cap, opt):
             tol[s, g, :rows] += (p * e).sum(0)
         assert wide >= rows
     return want, tol + np.abs(want) * 2.0 ** -20 + 1e-30
+
+
+# ---- one workspace under several descriptors ------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_type", ["f16", "q8_0"])
+def test_one_workspace_for_prompts_and_steps(kv_type):
+    """Descriptors of other bounds, sizes and streams take turns on one workspace
+    that was zeroed once: a split chunk, a split step of one token, many
+    streams, a chunk beside tokens; twice."""
+    cases = [R.build(90, kv_type, x, 8, 2) for x in ([(40, 2000)], [(1, 2000)], [(1, 900 + 50 * i) for i in range(9)],
+                                                     [(30, 700), (1, 1500), (2, 600)], [(3, 2500)])]
+    kvs = [device_kv(c) for c in cases]
+    ws = torch.zeros(max(kv.workspace.numel() for kv in kvs), dtype=torch.uint8, device="cuda")
+    for kv in kvs:
+        kv._ws = (ws.data_ptr(), ws.numel())
+    refs = [R.attend(c) for c in cases]
+    for _ in range(2):
+        for c, kv, ref in zip(cases, kvs, refs):
+            q = up(c["q"])
+            out, lse = torch.full(q.shape, 7.0, device="cuda"), torch.full(q.shape[:2], 7.0, device="cuda")
+            kv.attend(q, out=out, lse=lse)
+            tol, ltol = R.attend_tolerance(ref, 1)
+            close(out, ref[0], tol + ref[4] * 2.0 ** -22)
+            close(lse, ref[1], ltol)
+    assert V.read_device_error() == 0
+
+
+@pytest.mark.gpu
+def test_results_repeat_themselves():
+    """The same call gives the same bits, whatever ran in between."""
+    for kv_type in ("f16", "q8_0"):
+        for streams in ([(1, 1500)] * 5, [(200, 1500), (1, 900), (3, 40)], [(391, 391)], [(20, 3000)]):
+            c = R.build(95, kv_type, streams, 8, 2)
+            kv, q = device_kv(c), up(c["q"])
+            first = kv.attend(q)
+            for _ in range(5):
+                assert torch.equal(first, kv.attend(q))

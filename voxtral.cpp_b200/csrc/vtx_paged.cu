@@ -124,7 +124,7 @@ struct DecodePlan {
     bool use;                 // the streaming kernel is launched
     int rows;                 // its row count, 8 or 16
     PagedSplit split;
-    size_t c_bytes, o_bytes, bytes;   // counters, partial O, all
+    size_t o_bytes, bytes;    // partial O, with (m, l)
 };
 
 // Splits over (streams x KV heads): one wave of three CTAs per SM for one stream,
@@ -150,11 +150,19 @@ DecodePlan plan_decode(const vtx_paged_kv *p, int G, int sms) {
     d.split.tiles = (int)((tiles + want - 1) / want);
     if (want > 1) {
         const size_t rows = (size_t)base * want * d.rows;
-        d.c_bytes = align_up((size_t)base * 4, 256);
         d.o_bytes = align_up(rows * p->k.ne[0] * 4, 256);
-        d.bytes = d.c_bytes + d.o_bytes + align_up(rows * 8, 256);
+        d.bytes = d.o_bytes + align_up(rows * 8, 256);
     }
     return d;
+}
+
+// The attention workspace begins with the arrival counters of the streaming kernel's
+// splits, a word per stream and KV head, at least kArrivals of them whatever the plan:
+// nothing else is ever put there, so they stay zero between calls of any sizes.
+constexpr size_t kArrivals = 65536;
+
+size_t arrival_bytes(const vtx_paged_kv *p, size_t rest) {
+    return rest ? align_up(std::max((size_t)p->n_seq * (size_t)p->k.ne[2], kArrivals) * 4, 256) : 0;
 }
 
 template <int D, int KVT, int ROWS, bool UF>
@@ -503,7 +511,8 @@ size_t vtx_flash_attn_paged_workspace(const vtx_paged_kv *kv, int32_t n_head_q) 
         return (size_t)-1;
     const int G = n_head_q / (int)kv->k.ne[2], sms = current_sms();
     const DecodePlan d = plan_decode(kv, G, sms);
-    return d.bytes + plan_tile(kv, G, n_head_q, d.use ? d.rows : 0, sms).bytes;
+    const size_t rest = d.bytes + plan_tile(kv, G, n_head_q, d.use ? d.rows : 0, sms).bytes;
+    return arrival_bytes(kv, rest) + rest;
 }
 
 int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, size_t workspace_bytes, void *stream) {
@@ -529,7 +538,7 @@ int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, si
     if (rc != VTX_OK) return rc;
     DecodePlan dp = plan_decode(kv, Hq / (int)kv->k.ne[2], ds->sms);
     TilePlan tp = plan_tile(kv, Hq / (int)kv->k.ne[2], Hq, dp.use ? dp.rows : 0, ds->sms);
-    const size_t need = dp.bytes + tp.bytes;
+    const size_t first = arrival_bytes(kv, dp.bytes + tp.bytes), need = first + dp.bytes + tp.bytes;
     if (workspace_bytes < need || (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256)))
         return VTX_ERR_WORKSPACE;
     PagedAttnArgs a{};
@@ -549,7 +558,7 @@ int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, si
     a.min_rows = dp.use ? dp.rows : 0;
     PagedAttnArgs ta = a;                                     // what the tensor-core kernel reads
     if (tp.use) {
-        char *ws = static_cast<char *>(workspace) + dp.bytes;
+        char *ws = static_cast<char *>(workspace) + first + dp.bytes;
         tp.tile.part_o = reinterpret_cast<float *>(ws);
         tp.tile.part_ml = reinterpret_cast<float *>(ws + tp.o_bytes);
         const int D = (int)kv->k.ne[0];
@@ -575,8 +584,8 @@ int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *p, void *workspace, si
     if (dp.use) {
         char *ws = static_cast<char *>(workspace);
         dp.split.arrived = reinterpret_cast<unsigned *>(ws);
-        dp.split.part_o = reinterpret_cast<float *>(ws + dp.c_bytes);
-        dp.split.part_ml = reinterpret_cast<float *>(ws + dp.c_bytes + dp.o_bytes);
+        dp.split.part_o = reinterpret_cast<float *>(ws + first);
+        dp.split.part_ml = reinterpret_cast<float *>(ws + first + dp.o_bytes);
         dp.split.beside = kv->max_new * (long long)a.G > a.min_rows;
         rc = d64 ? (f16 ? launch_decode_rows<64, 1>(a, dp, st) : launch_decode_rows<64, 8>(a, dp, st))
                  : (f16 ? launch_decode_rows<128, 1>(a, dp, st) : launch_decode_rows<128, 8>(a, dp, st));
