@@ -467,8 +467,8 @@ VTX_API int vtx_kv_append_paged(const vtx_kv_append_paged_args *args, void *stre
  * Hq / Hkv <= 16; base and strides of q and dst multiples of 16 bytes.
  * Rows at or behind kv_len, and rows that no token of the stream sees, may hold
  * anything, NaN included; a row that some token sees and that is not finite in
- * V may also spoil tokens of its stream that do not see it.  dst must not
- * overlap q.
+ * V may also spoil tokens of its stream that do not see it.  A row with a score
+ * of NaN has NaN in dst and in lse.  dst must not overlap q.
  * Rounded to half: P (times the scale of V for a Q8_0 cache) and a F32 q.
  * Everything else is F32, the values of a Q8_0 cache included.  Its scales may
  * reach 511 (larger ones overflow a half); below 2^-14 those of V cost bits of
@@ -504,7 +504,8 @@ VTX_API int vtx_flash_attn_paged(const vtx_flash_attn_paged_args *args, void *wo
  * = n counts only the last n new tokens of each stream (0: all).  score and
  * score_out: F32 [n_seq][n_head_kv][row_cap], the same array or two disjoint
  * ones; with decay 0 score may be NULL.  Entries at or behind kv_len are left
- * alone.  A token whose lse is -inf counts nothing. */
+ * alone.  A token whose lse is -inf counts nothing, one whose lse is NaN makes
+ * NaN of the entries that it sees. */
 typedef struct vtx_kv_score_paged_args {
     const vtx_paged_kv *kv;
     const vtx_tensor *q;                /* as in vtx_flash_attn_paged */

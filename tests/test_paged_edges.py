@@ -116,6 +116,57 @@ def score_beyond(c, streams, lse, cap, opt):
     return want, tol + np.abs(want) * 2.0 ** -20 + 1e-30
 
 
+# ---- scores that are not finite ---------------------------------------------------------
+
+# streaming: one split and many, drafts; chunks: one Q tile, pairs, splits; short and unpacked Q8_0
+FINITE = [("f16", [(1, 60), (3, 50)], 8, 2, 128), ("f16", [(1, 3000)], 8, 2, 64), ("q8_0", [(2, 700), (1, 9)], 8, 2, 128),
+          ("f16", [(40, 300), (1, 70)], 8, 2, 64), ("f16", [(40, 300)], 8, 2, 128), ("f16", [(33, 2500)], 8, 2, 64),
+          ("f16", [(33, 2500)], 8, 2, 128), ("f16", [(700, 700)], 20, 20, 64), ("f16", [(700, 700)], 20, 20, 128),
+          ("q8_0", [(40, 80)], 8, 2, 64), ("q8_0", [(40, 300), (20, 120)], 8, 2, 64), ("q8_0", [(33, 2500)], 8, 2, 128)]
+
+
+def finite_case(i):
+    kv_type, streams, Hq, Hkv, D = FINITE[i]
+    c = R.build(80 + i, kv_type, streams, Hq, Hkv, D, 16)
+    ref = R.attend(c)
+    tol, ltol = R.attend_tolerance(ref, 1)
+    return c, ref, tol + ref[4] * 2.0 ** -22, ltol
+
+
+def check_finite(c, kv, q, ref, tol, ltol, nan, what):
+    """Rows of `nan` (tokens, heads) hold NaN throughout, the others what the reference says."""
+    out, lse = torch.full(q.shape, 3.0, device="cuda"), torch.full(q.shape[:2], 3.0, device="cuda")
+    kv.attend(q, out=out, lse=lse)
+    o, e = out.double().cpu().numpy(), lse.double().cpu().numpy()
+    assert np.array_equal(np.isnan(e), nan), f"{what}: lse NaN at {np.argwhere(np.isnan(e) != nan)[:4]}"
+    assert np.isnan(o[nan]).all(), f"{what}: {(~np.isnan(o[nan])).sum()} values of NaN rows are not NaN"
+    close(out[up(~nan)], ref[0][~nan], tol[~nan])
+    close(lse[up(~nan)], ref[1][~nan], ltol[~nan])
+    return lse
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", range(len(FINITE)))
+def test_query_rows_of_nan(i):
+    """A NaN in a query row: its result and lse are NaN, as are the scores of the rows it sees; no other changes."""
+    c, ref, tol, ltol = finite_case(i)
+    kv, q = device_kv(c), up(c["q"])
+    T, Hq, D = q.shape
+    G = Hq // c["Hkv"]
+    for t, h, d in ((0, 1, slice(None)), (T - 1, Hq - 1, 5), (T // 2, 0, D - 1)):
+        bad = q.clone()
+        bad[t, h, d] = float("nan")
+        nan = np.zeros((T, Hq), bool)
+        nan[t, h] = True
+        lse = check_finite(c, kv, bad, ref, tol, ltol, nan, f"{FINITE[i]} token {t}")
+        s = int(np.searchsorted(c["start"][1:], t, side="right"))
+        sc = kv.score(bad, lse, torch.zeros(len(c["len"]), c["Hkv"], max(c["len"]), device="cuda"))
+        want = np.zeros(sc.shape, bool)
+        want[s, h // G, :c["len"][s] - (c["start"][s + 1] - t) + 1] = True
+        assert np.array_equal(torch.isnan(sc).cpu().numpy(), want)
+    assert V.read_device_error() == 0
+
+
 # ---- one workspace under several descriptors ------------------------------------------------
 
 @pytest.mark.gpu

@@ -433,7 +433,7 @@ __device__ __forceinline__ void paged_decode_cta(const PagedAttnArgs &a, const P
 #pragma unroll
         for (int w = 0; w < C::WARPS; ++w) {
             const float2 y = ml[w * 16 + r];
-            if (y.x != -INFINITY) tot += y.y * ex2(y.x - top);
+            tot += y.x == -INFINITY ? y.y : y.y * ex2(y.x - top);       // NaN where all its scores were
             const float4 v = *reinterpret_cast<const float4 *>(smem + w * C::WARP_BYTES + (r * D + d) * 4);
             acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
         }
@@ -483,14 +483,14 @@ __device__ __forceinline__ void paged_decode_cta(const PagedAttnArgs &a, const P
             float mx = top;
 #pragma unroll
             for (int u = 0; u < U; ++u) mx = fmaxf(mx, y[u].x);
-            if (mx == -INFINITY) continue;
-            const float f0 = ex2(top - mx);
+            const float ref = mx == -INFINITY ? 0.f : mx;       // nothing seen, or NaN alone, which stays NaN
+            const float f0 = ex2(top - ref);
             acc.x *= f0; acc.y *= f0; acc.z *= f0; acc.w *= f0;
             tot *= f0;
             top = mx;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float f = ex2(y[u].x - mx);
+                const float f = ex2(y[u].x - ref);
                 tot = fmaf(f, y[u].y, tot);
                 acc.x = fmaf(f, v[u].x, acc.x); acc.y = fmaf(f, v[u].y, acc.y);
                 acc.z = fmaf(f, v[u].z, acc.z); acc.w = fmaf(f, v[u].w, acc.w);

@@ -360,7 +360,8 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_tile[t], 0, a.kv.err, VTX_KERR_O));
             tc_fence_after();
         }
-        if (m_run == -INFINITY) l_run = 0.0f;      // saw nothing (the sum holds 2^-125s)
+        // saw nothing: the sum holds 2^-125s (NaN where every score was, which stays)
+        if (m_run == -INFINITY && l_run == l_run) l_run = 0.0f;
         float f0 = 1.0f, f1 = 0.0f;                // weights of this warpgroup's O and the other one's
         const bool join = !two && n_iter > 1;
         if (join) {                                // the first warpgroup takes the second one's sums in
