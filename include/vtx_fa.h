@@ -468,7 +468,8 @@ VTX_API int vtx_kv_append_paged(const vtx_kv_append_paged_args *args, void *stre
  * Rows at or behind kv_len, and rows that no token of the stream sees, may hold
  * anything, NaN included; a row that some token sees and that is not finite in
  * V may also spoil tokens of its stream that do not see it.  A row with a score
- * of NaN has NaN in dst and in lse.  dst must not overlap q.
+ * of NaN or +inf has NaN in dst and in lse; one of -inf counts nothing.  dst must
+ * not overlap q.
  * Rounded to half: P (times the scale of V for a Q8_0 cache) and a F32 q.
  * Everything else is F32, the values of a Q8_0 cache included.  Its scales may
  * reach 511 (larger ones overflow a half); below 2^-14 those of V cost bits of

@@ -167,6 +167,66 @@ def test_query_rows_of_nan(i):
     assert V.read_device_error() == 0
 
 
+def set_key(kv, c, s, row, value):
+    """Sets a key's first value (F16) or first scale (Q8_0); returns what undoes it."""
+    page, at = int(c["table"][s, row // c["page"]]), row % c["page"]
+    old = kv.k_pool[page, :, at].clone()
+    if c["kv"] == "f16":
+        kv.k_pool[page, :, at, 0] = value
+    else:
+        kv.k_pool[page, :, at, :2] = torch.tensor([value], dtype=torch.float16).view(torch.uint8).cuda()
+
+    def undo():
+        kv.k_pool[page, :, at] = old
+    return undo
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", range(len(FINITE)))
+def test_keys_of_nan(i):
+    """A NaN key makes NaN of every token that sees it, wherever in a tile it stands, and of no other."""
+    c, ref, tol, ltol = finite_case(i)
+    kv, q = device_kv(c), up(c["q"])
+    for s, n in enumerate(c["len"]):
+        new = int(c["start"][s + 1] - c["start"][s])
+        for row in sorted({0, 6, 7, 14, n // 3, n // 2 | 7, n - new, n - 1} & set(range(n))):
+            undo = set_key(kv, c, s, row, float("nan"))
+            nan = np.zeros(q.shape[:2], bool)
+            nan[c["start"][s]:c["start"][s + 1]] = (row <= n - new + np.arange(new))[:, None]
+            check_finite(c, kv, q, ref, tol, ltol, nan, f"{FINITE[i]} stream {s} row {row}")
+            undo()
+    assert V.read_device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", [i for i, x in enumerate(FINITE) if x[0] == "f16"])
+def test_infinite_scores(i):
+    """A score of +inf makes NaN of its token's result and lse, one of -inf counts nothing."""
+    c, _, _, _ = finite_case(i)
+    c["q"][:, :, 0] = np.where(np.random.default_rng(i).random(c["q"].shape[:2]) < 0.3, 1, -1)
+    _, _, _, err, _ = R.attend(c)
+    kv, q = device_kv(c), up(c["q"])
+    s, n = len(c["len"]) - 1, c["len"][-1]
+    new = int(c["start"][s + 1] - c["start"][s])
+    for row in sorted({0, 7, n // 2 | 6, n - 1} & set(range(n))):
+        far = dict(c, k_pool=c["k_pool"].copy())               # a weight of exactly 0 where q is -1
+        far["k_pool"][c["table"][s, row // 16], :, row % 16, 0] = 60000
+        out, lse, a, _, tiny = R.attend(far)
+        alone = c["start"][s] + row - (n - new) if row == 0 else -1      # the token that sees this key and no other
+        if alone >= c["start"][s]:
+            down = c["q"][alone, :, 0] < 0
+            out[alone, down], lse[alone, down] = 0.0, -np.inf
+        ref = (out, lse, a, err, tiny)
+        tol, ltol = R.attend_tolerance(ref, 1)
+        undo = set_key(kv, c, s, row, float("inf"))
+        nan = np.zeros(q.shape[:2], bool)
+        t = slice(c["start"][s], c["start"][s + 1])
+        nan[t] = (row <= n - new + np.arange(new))[:, None] & (c["q"][t, :, 0] > 0)
+        check_finite(c, kv, q, ref, tol + ref[4] * 2.0 ** -22, ltol, nan, f"{FINITE[i]} row {row}")
+        undo()
+    assert V.read_device_error() == 0
+
+
 # ---- one workspace under several descriptors ------------------------------------------------
 
 @pytest.mark.gpu

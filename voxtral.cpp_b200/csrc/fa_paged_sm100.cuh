@@ -74,7 +74,15 @@ template <int D> struct PagedTileCfg {
     __host__ __device__ static constexpr int o_col(int t) { return 256 + t * D; }
 };
 
-// 2^x of a pair on the FMA pipe, x <= ~8; below -125 the result is about 2^-125.
+// Maximum that keeps a NaN.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 2^x of a pair on the FMA pipe, x <= ~8; below -125, and for a NaN, the result is
+// about 2^-125.
 __device__ __forceinline__ void paged_exp2_pair(float &a, float &b) {
     const float kRound = 12582912.0f;                    // 1.5 * 2^23
     a = fmaxf(a, -125.0f);
@@ -298,12 +306,12 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 constexpr int W = KEYS / 8;
-                mx8[k] = fmaxf(x[W * k], x[W * k + 1]);
+                mx8[k] = max3_nan(x[W * k], x[W * k + 1], x[W * k + 1]);
 #pragma unroll
-                for (int i = 2; i < W; i += 2) mx8[k] = fmax3(mx8[k], x[W * k + i], x[W * k + i + 1]);
+                for (int i = 2; i < W; i += 2) mx8[k] = max3_nan(mx8[k], x[W * k + i], x[W * k + i + 1]);
             }
-            const float mx = fmax3(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]),
-                                   fmaxf(mx8[6], mx8[7])) * cx;
+            const float mx = max3_nan(max3_nan(mx8[0], mx8[1], mx8[2]), max3_nan(mx8[3], mx8[4], mx8[5]),
+                                      max3_nan(mx8[6], mx8[7], mx8[7])) * cx;
             bool rescale = false;
             float alpha = 1.0f;
             if (mx > m_run + 8.0f) {               // the reference moves only on a 2^8 jump
@@ -336,6 +344,7 @@ fa_paged_sm100_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
                 upk2(fadd2(fadd2(sum2[0], sum2[1]), fadd2(sum2[2], sum2[3])), sa, sb);
                 l_run += sa + sb;
             }
+            if (!(mx < INFINITY)) l_run = NAN;     // a score of NaN or +inf, which the polynomial would lose
             tmem_st32(s_addr, *reinterpret_cast<const uint32_t(*)[32]>(&pk[0]));
             tmem_st32(s_addr + 32, *reinterpret_cast<const uint32_t(*)[32]>(&pk[LO ? 0 : 32]));
             // tcgen05.ld / st are warp-collective: the warp rescales when any row needs it
