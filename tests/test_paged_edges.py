@@ -263,3 +263,86 @@ def test_results_repeat_themselves():
             first = kv.attend(q)
             for _ in range(5):
                 assert torch.equal(first, kv.attend(q))
+
+
+# ---- results made on another stream -----------------------------------------------------------
+
+class FakeStreams:
+    """torch.cuda's streams and allocations on a machine without a GPU: which
+    stream was current when a tensor was made, and which others were noted on it."""
+
+    def __init__(self, monkeypatch):
+        self.current, self.made, self.noted = ["main"], [], []
+        empty, here = torch.empty, self
+
+        class Context:
+            def __init__(self, stream):
+                self.stream = stream
+
+            def __enter__(self):
+                here.current.append(self.stream)
+
+            def __exit__(self, *_):
+                here.current.pop()
+
+        def fake_empty(*shape, **kw):
+            kw["device"] = "cpu"
+            here.made.append(here.current[-1])
+            return empty(*shape, **kw)
+
+        monkeypatch.setattr(torch.cuda, "stream", Context)
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda *_: here.current[-1])
+        monkeypatch.setattr(torch, "empty", fake_empty)
+        monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: here.noted.append(s), raising=False)
+
+
+class SideStream:
+    cuda_stream = 77
+
+
+def host_kv(call, n_seq=1, n_tokens=2):
+    """A PagedKv over host memory whose calls go to `call(args, ...)`."""
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.float16)
+    kv = V.PagedKv(k, k.clone(), i32(n_seq, 2), i32(n_seq), i32(n_seq + 1), 4, n_tokens=n_tokens, max_new=n_tokens)
+
+    class Lib:
+        vtx_flash_attn_paged = vtx_kv_append_paged = vtx_kv_score_paged = vtx_kv_evict_paged = staticmethod(call)
+
+    kv._lib, kv.dev, kv._only = Lib, torch.device("cuda"), True
+    return kv
+
+
+def test_results_come_from_the_memory_of_the_stream_that_writes_them(monkeypatch):
+    """A block of the current stream's memory may still be in use there; a result
+    for another stream is made in that stream's, and the current one noted on it."""
+    kv = host_kv(lambda *_: 0)
+    q, k, pos = torch.zeros(2, 4, 64), torch.zeros(2, 2, 64), torch.zeros(2, dtype=torch.int32)
+    side = SideStream()
+    fake = FakeStreams(monkeypatch)
+    kv.attend(q, stream=side)
+    kv.append(k, k, pos, q=q, stream=side)
+    assert fake.made == [side, side] and fake.noted == ["main", "main"] and fake.current == ["main"]
+
+
+@pytest.mark.gpu
+def test_results_made_for_another_stream_are_their_own():
+    """Work queued on the current stream writes a block that was freed a moment ago;
+    a call on another stream with a result of that size is not touched by it."""
+    c = R.build(96, "f16", [(20, 300), (1, 700)], 8, 2)
+    kv, q = device_kv(c), up(c["q"])
+    T = q.shape[0]
+    k, pos, qf = torch.randn(T, 2, 128, device="cuda"), torch.arange(T, dtype=torch.int32, device="cuda"), q.float()
+    want, want_q = kv.attend(q), kv.append(k, k, pos, q=qf)
+    want = kv.attend(q)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        torch.cuda._sleep(20_000_000)
+        for like in (want, want_q):
+            busy = torch.empty_like(like)
+            busy.fill_(7)
+            del busy
+        out, got_q = kv.attend(q, stream=side), kv.append(k, k, pos, q=qf, stream=side)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(got_q, want_q)

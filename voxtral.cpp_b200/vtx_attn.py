@@ -259,6 +259,18 @@ def _check(rc: int, what: str = "") -> None:
         raise VtxError(rc, what)
 
 
+def _empty(shape, dtype: torch.dtype, device: torch.device, stream: Optional[torch.cuda.Stream]) -> torch.Tensor:
+    """A tensor that a call on `stream` writes.  It comes from that stream's memory:
+    a block of the current one's may still be in use by work queued there, which
+    `stream` does not wait for.  The current stream counts as a user of it."""
+    if stream is None or device.type != "cuda":
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    t.record_stream(torch.cuda.current_stream(device))
+    return t
+
+
 def workspace_bytes(q, k, v, scale, max_bias=0.0, logit_softcap=0.0, causal=False, window=0,
                     kv_type=None) -> int:
     L = load()
@@ -451,7 +463,9 @@ class PagedKv:
     tighter it is, the better the work is cut).  Workspaces are made here once
     (with a synchronisation, so outside of captures); calls on one PagedKv must
     not overlap on the GPU, and it must live until they are done.  Inputs and
-    outputs stay the caller's and are not copied."""
+    outputs stay the caller's and are not copied.  A call with stream= is queued
+    there and waits for nothing else: its inputs have to be ready on that stream,
+    and a result that it makes is that stream's."""
 
     def __init__(self, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor,
                  q_start: torch.Tensor, n_head_q: int, *, n_tokens: int, max_new: int,
@@ -552,12 +566,6 @@ class PagedKv:
         p.scale = self.head_dim ** -0.5 if scale is None else scale
         p.logit_softcap, p.causal, p.window = softcap, 1 if causal else 0, window
 
-    def _made(self, t: torch.Tensor, stream: Optional[torch.cuda.Stream]) -> torch.Tensor:
-        """A result allocated here on the current stream and written on `stream`."""
-        if stream is not None and self.dev.type == "cuda":
-            t.record_stream(stream)
-        return t
-
     def _call(self, fn, args, stream: Optional[torch.cuda.Stream], *ws) -> None:
         dev = self.dev
         if dev.type != "cuda":
@@ -591,7 +599,7 @@ class PagedKv:
             raise VtxError(-3, f"k, v and positions must be on {self.dev}")
         if q is not None:
             if q_out is None:
-                q_out = self._made(torch.empty(q.shape, dtype=torch.float16, device=self.dev), stream)
+                q_out = _empty(q.shape, torch.float16, self.dev, stream)
             if not q.get_device() == q_out.get_device() == self._on:
                 raise VtxError(-3, f"q and q_out must be on {self.dev}")
             qs, os_, kind = q.stride(), q_out.stride(), _ROW_TYPES.get(q_out.dtype)
@@ -621,7 +629,7 @@ class PagedKv:
         optional float32 (n_tokens, n_head_q) that receives ln sum exp.  scale
         defaults to D ** -0.5."""
         if out is None:
-            out = self._made(torch.empty(self._q_shape, dtype=torch.float32, device=self.dev), stream)
+            out = _empty(self._q_shape, torch.float32, self.dev, stream)
         self._rows(q, "q", self._q, self._q_nb, 1, 2)
         self._rows(out, "out", self._dst, self._dst_nb, 2, 1)
         self._set_params(scale, causal, window, logit_softcap)
