@@ -263,7 +263,7 @@ def _empty(shape, dtype: torch.dtype, device: torch.device, stream: Optional[tor
     """A tensor that a call on `stream` writes.  It comes from that stream's memory:
     a block of the current one's may still be in use by work queued there, which
     `stream` does not wait for.  The current stream counts as a user of it."""
-    if stream is None or device.type != "cuda":
+    if stream is None:
         return torch.empty(shape, dtype=dtype, device=device)
     with torch.cuda.stream(stream):
         t = torch.empty(shape, dtype=dtype, device=device)
@@ -297,14 +297,14 @@ def flash_attn_ext(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     B, Hq, n_q = q.shape[0], q.shape[1], q.shape[2]
     Dv = v.shape[-1] if (kv_type or _ggml_type(v, None)) != Q8_0 else v.shape[-1] // Q8_0_BLOCK * QK8_0
     if out is None:
-        out = torch.empty((B, n_q, Hq, Dv), dtype=torch.float32, device=q.device)
+        out = _empty((B, n_q, Hq, Dv), torch.float32, q.device, stream)
     p = params(scale, max_bias, logit_softcap, causal, window)
     dq, dk, dv = desc(q), desc(k, kv_type), desc(v, kv_type)
     need = L.vtx_flash_attn_ext_workspace(ctypes.byref(dq), ctypes.byref(dk), ctypes.byref(dv), ctypes.byref(p))
     if need == ctypes.c_size_t(-1).value:
         raise VtxError(-3, "operands rejected")
     if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        workspace = _empty((need,), torch.uint8, q.device, stream)
     ws_ptr = workspace.data_ptr() if (workspace is not None and need) else None
     ws_len = workspace.numel() * workspace.element_size() if (workspace is not None and need) else 0
     dm = desc(mask, F16) if mask is not None else None
@@ -349,7 +349,7 @@ class DecodeBatchPlan:
     def __call__(self, q: torch.Tensor, out: Optional[torch.Tensor] = None,
                  stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
         if out is None:
-            out = torch.empty_like(q, dtype=torch.float32)
+            out = _empty(q.shape, torch.float32, q.device, stream)
         self.batch.q = q.data_ptr()
         self.batch.dst = out.data_ptr()
         s = stream if stream is not None else torch.cuda.current_stream(q.device)
@@ -374,15 +374,16 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: 
         if t.dtype != torch.float32 or t.stride(2) != 1 or t.stride(1) != D:
             raise VtxError(-4, "q/k/v must be float32 with heads contiguous")
     if q is not None and q_out is None:
-        q_out = torch.empty_like(q)
+        q_out = _empty(q.shape, q.dtype, q.device, stream)
     a = KvAppendArgs()
     a.n_tokens, a.n_head_kv, a.head_dim, a.kv_type, a.freq_base = T, Hkv, D, kv_type, freq_base
     if q is not None:
         a.n_head_q, a.q, a.q_nb1 = q.shape[1], q.data_ptr(), q.stride(0) * 4
         a.q_out, a.q_out_nb1 = q_out.data_ptr(), q_out.stride(0) * 4
     a.k, a.k_nb1, a.v, a.v_nb1 = k.data_ptr(), k.stride(0) * 4, v.data_ptr(), v.stride(0) * 4
-    pos = positions.to(torch.int32).contiguous()
-    sl = slots.to(torch.int32).contiguous()
+    with torch.cuda.stream(stream):                # copies, if any, are made and freed where they are read
+        pos = positions.to(torch.int32).contiguous()
+        sl = slots.to(torch.int32).contiguous()
     a.positions, a.slots = pos.data_ptr(), sl.data_ptr()
     a.k_cache = k_cache.data_ptr() if k_cache is not None else None
     a.v_cache = v_cache.data_ptr() if v_cache is not None else None
@@ -433,7 +434,7 @@ class DecodeLayerPlan:
             if t.dtype != torch.float32 or t.stride(2) != 1 or t.stride(1) != t.shape[2]:
                 raise VtxError(-4, "q/k/v must be float32 with heads contiguous")
         if out is None:
-            out = torch.empty_like(q)
+            out = _empty(q.shape, q.dtype, q.device, stream)
         a = self.args
         a.q, a.q_nb1 = q.data_ptr(), q.stride(0) * 4
         a.k, a.k_nb1 = k.data_ptr(), k.stride(0) * 4
@@ -806,7 +807,7 @@ def out_proj(attn: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] =
         raise VtxError(-3, "one batch, unit-stride head dim")
     N, K = w.shape
     if out is None:
-        out = torch.empty((n, N), dtype=torch.float32, device=attn.device)
+        out = _empty((n, N), torch.float32, attn.device, stream)
     a = _raw_tensor(F32 if es == 4 else F16, [Dv, Hq, n, 1], [es, head_nb, tok_nb, tok_nb * n], attn.data_ptr())
     wd = _raw_tensor(F16, [K, N, 1, 1], [2, w.stride(0) * 2], w.data_ptr())
     yd = _raw_tensor(F32, [N, n, 1, 1], [4, out.stride(0) * 4], out.data_ptr())
