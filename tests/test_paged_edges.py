@@ -1,4 +1,7 @@
 """The paged decoder cache at the edges of what its header allows."""
+import threading
+import time
+
 import numpy as np
 import pytest
 
@@ -346,3 +349,54 @@ def test_results_made_for_another_stream_are_their_own():
         out, got_q = kv.attend(q, stream=side), kv.append(k, k, pos, q=qf, stream=side)
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(got_q, want_q)
+
+
+# ---- calls from several host threads ------------------------------------------------------------
+
+def test_calls_of_two_host_threads_do_not_mix():
+    """Every call reaches the library with its own arguments, before and after a while inside it."""
+    seen = []
+
+    def tensors(a):
+        if isinstance(a, V.KvAppendPagedArgs):
+            return a.k, a.q_out or 0
+        if isinstance(a, V.KvEvictPagedArgs):
+            return a.score, a.keep
+        q = V.VtxTensor.from_address(a.q).data
+        return (q, V.VtxTensor.from_address(a.dst).data) if isinstance(a, V.FlashAttnPagedArgs) else (q, a.score)
+
+    def call(args, *_):
+        before = tensors(args._obj)
+        time.sleep(0.003)
+        seen.append((before, tensors(args._obj)))
+        return 0
+
+    kv = host_kv(call)
+    pos, stream = torch.zeros(2, dtype=torch.int32), SideStream()
+    want, fails = [], []
+
+    def work(n):
+        q, out, lse, k, score = torch.zeros(2, 4, 64), torch.zeros(2, 4, 64), torch.zeros(2, 4), torch.zeros(2, 2, 64), torch.zeros(1, 2, 32)
+        keep.append((q, out, lse, k, score))
+        try:
+            for _ in range(5):
+                kv.attend(q, out=out, stream=stream)
+                if n == 0:
+                    kv.append(k, k, pos, stream=stream)
+                else:
+                    kv.append(k, k, pos, q=q, q_out=out, stream=stream)
+                kv.score(q, lse, score, stream=stream)
+                kv.evict(score, n + 3, stream=stream)
+        except Exception as e:  # noqa: BLE001
+            fails.append(e)
+        want.extend(5 * [(q.data_ptr(), out.data_ptr()), (k.data_ptr(), out.data_ptr() if n else 0),
+                         (q.data_ptr(), score.data_ptr()), (score.data_ptr(), n + 3)])
+
+    keep = []
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not fails and all(a == b for a, b in seen)
+    assert sorted(a for a, _ in seen) == sorted(want)

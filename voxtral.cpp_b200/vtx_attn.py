@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 from typing import Optional, Sequence
 
 import torch
@@ -462,11 +463,12 @@ class PagedKv:
     they may change between calls (and between replays of a captured call)
     within n_tokens, max_new and max_kv_len (default: the table's capacity; the
     tighter it is, the better the work is cut).  Workspaces are made here once
-    (with a synchronisation, so outside of captures); calls on one PagedKv must
-    not overlap on the GPU, and it must live until they are done.  Inputs and
-    outputs stay the caller's and are not copied.  A call with stream= is queued
-    there and waits for nothing else: its inputs have to be ready on that stream,
-    and a result that it makes is that stream's."""
+    (with a synchronisation, so outside of captures); calls on one PagedKv may
+    come from several host threads, but must not overlap on the GPU, and it must
+    live until they are done.  Inputs and outputs stay the caller's and are not
+    copied.  A call with stream= is queued there and waits for nothing else: its
+    inputs have to be ready on that stream, and a result that it makes is that
+    stream's."""
 
     def __init__(self, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor,
                  q_start: torch.Tensor, n_head_q: int, *, n_tokens: int, max_new: int,
@@ -520,6 +522,7 @@ class PagedKv:
         self._score, self._evict = KvScorePagedArgs(), KvEvictPagedArgs()
         for a in (self._append, self._attend, self._score, self._evict):
             a.kv = adr
+        self._lock = threading.Lock()               # a call fills its block and reads it, another thread's waits
         self._refs = [ctypes.byref(a) for a in (self._append, self._attend, self._score, self._evict)]
         self._attend.q, self._attend.dst, self._attend.params = at(self._q), at(self._dst), at(self._params)
         self._score.q, self._score.params = at(self._q), at(self._params)
@@ -607,19 +610,21 @@ class PagedKv:
             if q.shape != self._q_shape or q_out.shape != self._q_shape or qs[2] != 1 or qs[1] != D or os_[2] != 1 or \
                     os_[1] != D or q.dtype != torch.float32 or kind is None:
                 raise VtxError(-4, f"q (float32) and q_out must be {self._q_shape} with heads contiguous")
-            a.n_head_q, (a.q_out_type, es) = self.n_head_q, kind
-            a.q, a.q_nb1, a.q_out, a.q_out_nb1 = q.data_ptr(), qs[0] * 4, q_out.data_ptr(), os_[0] * es
         elif q_out is not None:
             raise VtxError(-1, "q_out without q")
-        else:
-            a.q = a.q_out = None
-        a.freq_base = freq_base
-        a.k, a.k_nb1, a.v, a.v_nb1 = k.data_ptr(), ks[0] * 4, v.data_ptr(), vs[0] * 4
-        a.positions = positions.data_ptr()
-        a.row_cap = self._array(score, torch.float32, "score", self._array(row_pos, torch.int32, "row_pos", None)) or 0
-        a.row_pos = row_pos.data_ptr() if row_pos is not None else None
-        a.score = score.data_ptr() if score is not None else None
-        self._call(self._lib.vtx_kv_append_paged, self._refs[0], stream)
+        cap = self._array(score, torch.float32, "score", self._array(row_pos, torch.int32, "row_pos", None)) or 0
+        with self._lock:
+            if q is not None:
+                a.n_head_q, (a.q_out_type, es) = self.n_head_q, kind
+                a.q, a.q_nb1, a.q_out, a.q_out_nb1 = q.data_ptr(), qs[0] * 4, q_out.data_ptr(), os_[0] * es
+            else:
+                a.q = a.q_out = None
+            a.freq_base, a.row_cap = freq_base, cap
+            a.k, a.k_nb1, a.v, a.v_nb1 = k.data_ptr(), ks[0] * 4, v.data_ptr(), vs[0] * 4
+            a.positions = positions.data_ptr()
+            a.row_pos = row_pos.data_ptr() if row_pos is not None else None
+            a.score = score.data_ptr() if score is not None else None
+            self._call(self._lib.vtx_kv_append_paged, self._refs[0], stream)
         return q_out
 
     def attend(self, q: torch.Tensor, out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, *,
@@ -631,11 +636,12 @@ class PagedKv:
         defaults to D ** -0.5."""
         if out is None:
             out = _empty(self._q_shape, torch.float32, self.dev, stream)
-        self._rows(q, "q", self._q, self._q_nb, 1, 2)
-        self._rows(out, "out", self._dst, self._dst_nb, 2, 1)
-        self._set_params(scale, causal, window, logit_softcap)
-        self._attend.lse = self._check_lse(lse) if lse is not None else None
-        self._call(self._lib.vtx_flash_attn_paged, self._refs[1], stream, *self._ws)
+        with self._lock:
+            self._rows(q, "q", self._q, self._q_nb, 1, 2)
+            self._rows(out, "out", self._dst, self._dst_nb, 2, 1)
+            self._set_params(scale, causal, window, logit_softcap)
+            self._attend.lse = self._check_lse(lse) if lse is not None else None
+            self._call(self._lib.vtx_flash_attn_paged, self._refs[1], stream, *self._ws)
         return out
 
     def _check_lse(self, lse: torch.Tensor) -> int:
@@ -653,12 +659,13 @@ class PagedKv:
         score_out.  q and lse as attend read and wrote them."""
         out = score if score_out is None else score_out
         cap = self._array(out, torch.float32, "score_out", self._array(score, torch.float32, "score", None))
-        self._rows(q, "q", self._q, self._q_nb, 1, 2)
-        self._set_params(scale, causal, window, logit_softcap)
         a = self._score
-        a.lse, a.score, a.score_out = self._check_lse(lse), score.data_ptr(), out.data_ptr()
-        a.row_cap, a.observe, a.decay = cap, observe, decay
-        self._call(self._lib.vtx_kv_score_paged, self._refs[2], stream)
+        with self._lock:
+            self._rows(q, "q", self._q, self._q_nb, 1, 2)
+            self._set_params(scale, causal, window, logit_softcap)
+            a.lse, a.score, a.score_out = self._check_lse(lse), score.data_ptr(), out.data_ptr()
+            a.row_cap, a.observe, a.decay = cap, observe, decay
+            self._call(self._lib.vtx_kv_score_paged, self._refs[2], stream)
         return out
 
     def evict(self, score: torch.Tensor, keep: int, kv_len_out: Optional[torch.Tensor] = None, *, n_sink: int = 0,
@@ -677,14 +684,15 @@ class PagedKv:
                                   t.get_device() != self._on):
                 raise VtxError(-3, f"{what} must be contiguous int32 on {self.dev}, one per stream")
         a = self._evict
-        a.row_cap = self._array(row_pos, torch.int32, "row_pos", self._array(score, torch.float32, "score", None))
+        rows = self._array(row_pos, torch.int32, "row_pos", self._array(score, torch.float32, "score", None))
         cap = self._array(pos_out, torch.int32, "pos_out", self._array(score_out, torch.float32, "score_out", None))
-        a.out_cap = self._array(src_out, torch.int32, "src_out", cap) or 0
+        cap = self._array(src_out, torch.int32, "src_out", cap) or 0
         ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-        a.score, a.row_pos, a.next_pos, a.kv_len_out = score.data_ptr(), ptr(row_pos), ptr(next_pos), kv_len_out.data_ptr()
-        a.score_out, a.pos_out, a.src_out = ptr(score_out), ptr(pos_out), ptr(src_out)
-        a.keep, a.n_sink, a.n_recent = keep, n_sink, n_recent
-        self._call(self._lib.vtx_kv_evict_paged, self._refs[3], stream, *self._evict_ws)
+        with self._lock:
+            a.score, a.row_pos, a.next_pos, a.kv_len_out = score.data_ptr(), ptr(row_pos), ptr(next_pos), kv_len_out.data_ptr()
+            a.score_out, a.pos_out, a.src_out = ptr(score_out), ptr(pos_out), ptr(src_out)
+            a.keep, a.n_sink, a.n_recent, a.row_cap, a.out_cap = keep, n_sink, n_recent, rows, cap
+            self._call(self._lib.vtx_kv_evict_paged, self._refs[3], stream, *self._evict_ws)
         return kv_len_out
 
 
