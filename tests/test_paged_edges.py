@@ -400,3 +400,50 @@ def test_calls_of_two_host_threads_do_not_mix():
         t.join()
     assert not fails and all(a == b for a, b in seen)
     assert sorted(a for a, _ in seen) == sorted(want)
+
+
+# ---- axes of one element --------------------------------------------------------------------------
+
+def one_token(h, dtype=torch.float32, device="cpu", kind=0):
+    """A (1, h, 64) view of one token whose first stride is not a token's."""
+    x = torch.randn(h, 64, device=device, dtype=dtype)
+    if kind == 0:
+        return x.unsqueeze(1).transpose(0, 1)              # head-major: strides (64, 64, 1)
+    return x.unsqueeze(2).permute(2, 0, 1)                 # strides (1, 64, 1)
+
+
+@pytest.mark.parametrize("kind", [0, 1])
+def test_strides_of_one_token_are_its_own(kind):
+    """The stride of an axis with one element means nothing and is not passed on."""
+    got = []
+
+    def call(args, *_):
+        a = args._obj
+        if isinstance(a, V.KvAppendPagedArgs):
+            got.append((a.k_nb1, a.v_nb1, a.q_nb1, a.q_out_nb1))
+        else:
+            q, d = (V.VtxTensor.from_address(x) for x in (a.q, a.dst))
+            got.append((q.nb[1], q.nb[2], d.nb[2], d.nb[1]))
+        return 0
+
+    kv, side = host_kv(call, n_tokens=1), SideStream()
+    q, k, pos = one_token(4, kind=kind), one_token(2, kind=kind), torch.zeros(1, dtype=torch.int32)
+    kv.append(k, k, pos, q=q, q_out=one_token(4, torch.float16, kind=kind), stream=side)
+    kv.attend(q, out=one_token(4, torch.float16, kind=kind), stream=side)
+    assert got == [(512, 512, 1024, 512), (1024, 256, 512, 128)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [0, 1])
+def test_one_token_of_any_stride(kind):
+    c = R.build(97, "f16", [(1, 40)], 4, 1, 64)
+    kv, kv2 = device_kv(c), device_kv(c)
+    q, k, pos = one_token(4, device="cuda", kind=kind), one_token(1, device="cuda", kind=kind), torch.full((1,), 9, dtype=torch.int32, device="cuda")
+    q16 = kv.append(k, k, pos, q=q)
+    want = kv.attend(q16)
+    out, half = one_token(4, device="cuda", kind=kind), one_token(4, torch.float16, "cuda", kind)
+    plain = lambda x: x.clone(memory_format=torch.contiguous_format)  # noqa: E731
+    kv2.append(plain(k), plain(k), pos, q=plain(q), q_out=half)
+    kv2.attend(half, out=out)
+    assert torch.equal(half, q16) and torch.equal(out, want)
+    assert torch.equal(kv.k_pool.view(torch.int16), kv2.k_pool.view(torch.int16))

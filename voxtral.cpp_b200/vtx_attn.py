@@ -511,6 +511,7 @@ class PagedKv:
         # argument blocks, made once: a call only sets its tensors
         self._q_shape = (n_tokens, n_head_q, self.head_dim)
         self._kv_shape = (n_tokens, self.n_head_kv, self.head_dim)
+        self._ones = 1 in (n_tokens, n_head_q, self.n_head_kv)
         self._q, self._dst, self._params = VtxTensor(), VtxTensor(), FaParams()
         for d in (self._q, self._dst):
             d.ne[0], d.ne[3] = self.head_dim, 1
@@ -545,9 +546,17 @@ class PagedKv:
         d.data = t.data_ptr()
         return d
 
+    def _strides(self, t: torch.Tensor):
+        """Strides, those of axes with one element (which may be anything) as if contiguous."""
+        st = t.stride()
+        if not self._ones or len(st) != 3:
+            return st
+        head = st[1] if t.shape[1] > 1 else t.shape[2]
+        return st[0] if t.shape[0] > 1 else head * t.shape[1], head, st[2]
+
     def _rows(self, t: torch.Tensor, what: str, d: VtxTensor, nb, token: int, head: int) -> None:
         """Puts a (n_tokens, n_head_q, D) float32 / float16 view into descriptor d."""
-        st, kind = t.stride(), _ROW_TYPES.get(t.dtype)
+        st, kind = self._strides(t), _ROW_TYPES.get(t.dtype)
         if t.shape != self._q_shape or st[2] != 1 or t.get_device() != self._on:
             raise VtxError(-3, f"{what} must be {self._q_shape} on {self.dev}, last axis contiguous")
         if kind is None:
@@ -593,7 +602,7 @@ class PagedKv:
         float16 when not given).  row_pos (int32) and score (float32),
         (n_seq, n_head_kv, rows): the new rows' entries are set."""
         D, a = self.head_dim, self._append
-        ks, vs = k.stride(), v.stride()
+        ks, vs = self._strides(k), self._strides(v)
         if k.shape != self._kv_shape or v.shape != self._kv_shape or ks[2] != 1 or ks[1] != D or vs[2] != 1 or \
                 vs[1] != D or k.dtype != torch.float32 or v.dtype != torch.float32:
             raise VtxError(-4, f"k and v must be {self._kv_shape} float32 with heads contiguous")
@@ -606,7 +615,7 @@ class PagedKv:
                 q_out = _empty(q.shape, torch.float16, self.dev, stream)
             if not q.get_device() == q_out.get_device() == self._on:
                 raise VtxError(-3, f"q and q_out must be on {self.dev}")
-            qs, os_, kind = q.stride(), q_out.stride(), _ROW_TYPES.get(q_out.dtype)
+            qs, os_, kind = self._strides(q), self._strides(q_out), _ROW_TYPES.get(q_out.dtype)
             if q.shape != self._q_shape or q_out.shape != self._q_shape or qs[2] != 1 or qs[1] != D or os_[2] != 1 or \
                     os_[1] != D or q.dtype != torch.float32 or kind is None:
                 raise VtxError(-4, f"q (float32) and q_out must be {self._q_shape} with heads contiguous")
