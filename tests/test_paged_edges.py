@@ -447,3 +447,45 @@ def test_one_token_of_any_stride(kind):
     kv2.attend(half, out=out)
     assert torch.equal(half, q16) and torch.equal(out, want)
     assert torch.equal(kv.k_pool.view(torch.int16), kv2.k_pool.view(torch.int16))
+
+
+# ---- chunks next to single tokens, replayed -----------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_type", ["f16", "q8_0"])
+def test_mixed_steps_replayed_with_other_lengths(kv_type):
+    """A captured step whose single tokens run beside its chunks: every replay
+    goes by the lengths, pages and queries written just before it."""
+    rng = np.random.default_rng(3)
+    streams = [(40, 600), (1, 900), (2, 500), (20, 300), (1, 40)]
+    c = R.build(98, kv_type, streams, 8, 2, poison=False)
+    kv = device_kv(c)
+    q = up(c["q"])
+    out, lse = torch.empty(q.shape, device="cuda"), torch.empty(q.shape[:2], device="cuda")
+    new_len, new_table, new_q = kv.kv_len.clone(), kv.page_table.clone(), q.clone()
+
+    def step():
+        kv.kv_len.copy_(new_len)
+        kv.page_table.copy_(new_table)
+        q.copy_(new_q)
+        kv.attend(q, out=out, lse=lse)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    pages = c["k_pool"].shape[0]
+    for _ in range(8):
+        c["len"] = [int(rng.integers(n, most + 1)) for n, most in streams]
+        c["table"] = rng.integers(0, pages, c["table"].shape).astype(np.int32)
+        c["q"] = rng.standard_normal(c["q"].shape).astype(np.float16)
+        new_len.copy_(torch.tensor(c["len"], dtype=torch.int32))
+        new_table.copy_(up(c["table"]))
+        new_q.copy_(up(c["q"]))
+        graph.replay()
+        ref = R.attend(c)
+        tol, ltol = R.attend_tolerance(ref, 1)
+        close(out, ref[0], tol + ref[4] * 2.0 ** -22)
+        close(lse, ref[1], ltol)
+    assert V.read_device_error() == 0
