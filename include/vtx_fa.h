@@ -538,7 +538,11 @@ VTX_API int vtx_kv_score_paged(const vtx_kv_score_paged_args *args, void *stream
  *   (out_cap >= keep): score, position and old row index of the m rows;
  *   entries behind m are left alone.  score_out may be score and pos_out
  *   row_pos (then out_cap = row_cap), no other overlap.
- * - kv_len_out: [n_seq], receives m (may be kv_len).
+ * - kv_len_out: [n_seq], receives m.  It may be kv_len, but only where no other
+ *   cache goes by that array: the caches of several layers that share it are all
+ *   evicted with its old lengths, the new ones in an array of their own that
+ *   replaces it after the last of them.  (Evicted again with lengths already cut
+ *   to keep, a cache would lose the rows behind it, its best ones among them.)
  * q_start is not used.  n_sink + n_recent <= keep. */
 typedef struct vtx_kv_evict_paged_args {
     const vtx_paged_kv *kv;

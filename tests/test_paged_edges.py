@@ -489,3 +489,32 @@ def test_mixed_steps_replayed_with_other_lengths(kv_type):
         close(out, ref[0], tol + ref[4] * 2.0 ** -22)
         close(lse, ref[1], ltol)
     assert V.read_device_error() == 0
+
+
+# ---- layers that share their lengths ---------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [300, 1500])
+def test_layers_with_one_kv_len_evict_by_the_old_lengths(n):
+    """Each layer's eviction reads the shared lengths and writes the new ones
+    elsewhere; every layer keeps its own best rows."""
+    cases = [R.build(110 + i, "f16", [(0, n), (0, 40), (0, n - 90)], 4, 2, 64, 16, poison=False) for i in range(3)]
+    kvs = [device_kv(c, n_tokens=0, max_new=0) for c in cases]
+    kv_len, left = kvs[0].kv_len.clone(), torch.zeros(3, dtype=torch.int32, device="cuda")
+    kvs = [V.PagedKv(kv.k_pool, kv.v_pool, kv.page_table, kv_len, kv.q_start, 4, n_tokens=0, max_new=0, max_kv_len=n) for kv in kvs]
+    rng = np.random.default_rng(4)
+    scores = [rng.random((3, 2, n)).astype(np.float32) for _ in cases]
+    srcs = [torch.full((3, 2, 100), -1, dtype=torch.int32, device="cuda") for _ in cases]
+    for kv, sc, src in zip(kvs, scores, srcs):
+        kv.evict(up(sc), 100, left, n_sink=4, n_recent=20, src_out=src)
+    kv_len.copy_(left)
+    assert kv_len.tolist() == [100, 40, 100]
+    for c, kv, sc, src in zip(cases, kvs, scores, srcs):
+        want, _ = R.evict(c, sc, 100, 4, 20)
+        pools = [(c[p], getattr(kv, p).cpu().numpy()) for p in ("k_pool", "v_pool")]
+        for (s, h), rows in want.items():
+            assert np.array_equal(src[s, h, :len(rows)].cpu().numpy(), rows)
+            for old, now in pools:
+                kept = R.rows_of(now, c["table"][s], len(rows))[h]
+                assert np.array_equal(kept, R.rows_of(old, c["table"][s], c["len"][s])[h][rows])
+    assert V.read_device_error() == 0

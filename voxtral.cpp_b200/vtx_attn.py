@@ -683,7 +683,10 @@ class PagedKv:
               src_out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
         """vtx_kv_evict_paged: every (stream, KV head) keeps its ``keep`` best rows,
         moved together in place; kv_len_out (default: kv_len itself) receives
-        the new lengths.  score_out, pos_out, src_out: optional
+        the new lengths.  Where several caches (layers) share one kv_len, give
+        each call another kv_len_out and copy it to kv_len after the last one:
+        a shorter kv_len cuts off what the next cache still had to choose from.
+        score_out, pos_out, src_out: optional
         (n_seq, n_head_kv, >= keep) arrays of the kept rows' scores, positions
         and old row indices; score_out may be score and pos_out row_pos."""
         if kv_len_out is None:
