@@ -518,3 +518,53 @@ def test_layers_with_one_kv_len_evict_by_the_old_lengths(n):
                 kept = R.rows_of(now, c["table"][s], len(rows))[h]
                 assert np.array_equal(kept, R.rows_of(old, c["table"][s], c["len"][s])[h][rows])
     assert V.read_device_error() == 0
+
+
+# ---- shared workspaces ---------------------------------------------------------------------------------
+
+def test_share_takes_the_workspaces_of_another():
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.float16)
+
+    def make(n_seq, max_pages, **kw):
+        return V.PagedKv(k, k.clone(), i32(n_seq, max_pages), i32(n_seq), i32(n_seq + 1), 4, n_tokens=40, max_new=40, **kw)
+
+    big = make(8, 64)
+    small = make(1, 20, share=big)
+    assert small.workspace is big.workspace and small._ws == big._ws and small._evict_ws == big._evict_ws
+    assert make(8, 64, share=small).workspace is big.workspace
+    own = make(1, 20)
+    assert own.workspace is not big.workspace and own.workspace.numel() < big.workspace.numel()
+    with pytest.raises(V.VtxError) as e:
+        make(8, 64, share=own)
+    assert e.value.status == -6
+    with pytest.raises(V.VtxError) as e:                  # more counters than their fixed place holds
+        make(1, 1, share=make(40000, 2))
+    assert e.value.status == -6
+
+
+@pytest.mark.gpu
+def test_layers_and_steps_share_one_set():
+    """A prompt and then single tokens through three layers over one set of workspaces."""
+    cases = [R.build(120 + i, "q8_0", [(60, 700), (33, 600)], 8, 2, poison=False) for i in range(3)]
+    first, layers = None, []
+    for c in cases:
+        kv = device_kv(c, share=first)
+        first = first or kv
+        one = dict(c, start=np.array([0, 1, 2], np.int32), q=c["q"][:2])
+        layers.append((c, kv, one, V.PagedKv(kv.k_pool, kv.v_pool, kv.page_table, kv.kv_len, up(one["start"]), 8,
+                                             n_tokens=2, max_new=1, max_kv_len=700, share=first)))
+    for _ in range(2):
+        for what in (0, 2):
+            for l in layers:
+                c, kv = l[what], l[what + 1]
+                out = kv.attend(up(c["q"]))
+                ref = R.attend(c)
+                close(out, ref[0], R.attend_tolerance(ref, 1)[0] + ref[4] * 2.0 ** -22)
+    for i, (c, kv, _, _) in enumerate(layers):
+        sc = np.random.default_rng(i).random((2, 2, 700)).astype(np.float32)
+        src = torch.empty(2, 2, 200, dtype=torch.int32, device="cuda")
+        kv.evict(up(sc), 200, torch.zeros(2, dtype=torch.int32, device="cuda"), src_out=src)
+        for (s, h), rows in R.evict(c, sc, 200)[0].items():
+            assert np.array_equal(src[s, h].cpu().numpy(), rows)
+    assert V.read_device_error() == 0

@@ -463,16 +463,18 @@ class PagedKv:
     they may change between calls (and between replays of a captured call)
     within n_tokens, max_new and max_kv_len (default: the table's capacity; the
     tighter it is, the better the work is cut).  Workspaces are made here once
-    (with a synchronisation, so outside of captures); calls on one PagedKv may
-    come from several host threads, but must not overlap on the GPU, and it must
-    live until they are done.  Inputs and outputs stay the caller's and are not
+    (with a synchronisation, so outside of captures), up to 4 GiB where chunks
+    meet a Q8_0 cache; share= takes those of another PagedKv, no smaller ones, so
+    that layers, or prompts and single tokens, have one set between them.  Calls
+    on one PagedKv, or on those that share, may come from several host threads,
+    but must not overlap on the GPU, and it must live until they are done.  Inputs and outputs stay the caller's and are not
     copied.  A call with stream= is queued there and waits for nothing else: its
     inputs have to be ready on that stream, and a result that it makes is that
     stream's."""
 
     def __init__(self, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor,
                  q_start: torch.Tensor, n_head_q: int, *, n_tokens: int, max_new: int,
-                 max_kv_len: Optional[int] = None):
+                 max_kv_len: Optional[int] = None, share: Optional["PagedKv"] = None):
         if k_pool.dim() != 4 or v_pool.shape != k_pool.shape or v_pool.dtype != k_pool.dtype or \
                 v_pool.device != k_pool.device:
             raise VtxError(-3, "k_pool and v_pool must be (n_pages, n_head_kv, page_size, D) alike")
@@ -502,11 +504,18 @@ class PagedKv:
                     self._lib.vtx_kv_evict_paged_workspace(ctypes.byref(c))]
         if ctypes.c_size_t(-1).value in need:
             raise VtxError(-3, "paged cache rejected")
-        # attention's holds arrival counters: zero once, left zeroed by every call
-        self.workspace = torch.zeros(max(need[0], 256), dtype=torch.uint8, device=self.dev)
-        self.evict_workspace = torch.empty(max(need[1], 256), dtype=torch.uint8, device=self.dev)
-        if self.dev.type == "cuda":                 # the first call may be on another stream
-            torch.cuda.current_stream(self.dev).synchronize()
+        if share is not None:
+            pairs = (n_seq * self.n_head_kv, share.n_seq * share.n_head_kv)
+            if share.dev != self.dev or share.workspace.numel() < need[0] or share.evict_workspace.numel() < need[1] or \
+                    (max(pairs) > 65536 and pairs[0] != pairs[1]):              # counters beyond their fixed place
+                raise VtxError(-6, "the shared workspaces are too small, or on another device")
+            self.workspace, self.evict_workspace = share.workspace, share.evict_workspace
+        else:
+            # attention's holds arrival counters: zero once, left zeroed by every call
+            self.workspace = torch.zeros(max(need[0], 256), dtype=torch.uint8, device=self.dev)
+            self.evict_workspace = torch.empty(max(need[1], 256), dtype=torch.uint8, device=self.dev)
+            if self.dev.type == "cuda":             # the first call may be on another stream
+                torch.cuda.current_stream(self.dev).synchronize()
         self._ws, self._evict_ws = ((w.data_ptr(), w.numel()) for w in (self.workspace, self.evict_workspace))
         # argument blocks, made once: a call only sets its tensors
         self._q_shape = (n_tokens, n_head_q, self.head_dim)
