@@ -7,13 +7,19 @@ import pytest
 
 import paged_ref as R
 import vtx_attn as V
-from test_paged import BASE, device_kv
+from test_paged import ATTEND, BASE, device_kv
 
 torch = pytest.importorskip("torch")
 
 
 def up(x):
     return torch.from_numpy(np.ascontiguousarray(x)).cuda()
+
+
+# Q8_0: P carries V's scale d when it is rounded, so a subnormal loses 2^-25 of a product
+# whose largest is 16 d or more; with the cases' scales of 1/127 and more that is 2^-22 of
+# what a whole weight would give
+SUBNORMAL = 2.0 ** -22
 
 
 def close(got, want, tol):
@@ -84,7 +90,7 @@ def test_attend_and_score_beyond_the_table(i):
     assert V.read_device_error() == 41
     ref = R.attend(c, **opt)
     tol, ltol = R.attend_tolerance(ref, 1)
-    close(out, ref[0], tol + ref[4] * 2.0 ** -22)
+    close(out, ref[0], tol + ref[4] * SUBNORMAL)
     close(lse, ref[1], ltol)
     c["len"] = [min(n, cap) for n in c["len"]]                # rows that the sums run over
     for x in (q, q.float()):
@@ -133,7 +139,7 @@ def finite_case(i):
     c = R.build(80 + i, kv_type, streams, Hq, Hkv, D, 16)
     ref = R.attend(c)
     tol, ltol = R.attend_tolerance(ref, 1)
-    return c, ref, tol + ref[4] * 2.0 ** -22, ltol
+    return c, ref, tol + ref[4] * SUBNORMAL, ltol
 
 
 def check_finite(c, kv, q, ref, tol, ltol, nan, what):
@@ -225,7 +231,7 @@ def test_infinite_scores(i):
         nan = np.zeros(q.shape[:2], bool)
         t = slice(c["start"][s], c["start"][s + 1])
         nan[t] = (row <= n - new + np.arange(new))[:, None] & (c["q"][t, :, 0] > 0)
-        check_finite(c, kv, q, ref, tol + ref[4] * 2.0 ** -22, ltol, nan, f"{FINITE[i]} row {row}")
+        check_finite(c, kv, q, ref, tol + ref[4] * SUBNORMAL, ltol, nan, f"{FINITE[i]} row {row}")
         undo()
     assert V.read_device_error() == 0
 
@@ -251,7 +257,7 @@ def test_one_workspace_for_prompts_and_steps(kv_type):
             out, lse = torch.full(q.shape, 7.0, device="cuda"), torch.full(q.shape[:2], 7.0, device="cuda")
             kv.attend(q, out=out, lse=lse)
             tol, ltol = R.attend_tolerance(ref, 1)
-            close(out, ref[0], tol + ref[4] * 2.0 ** -22)
+            close(out, ref[0], tol + ref[4] * SUBNORMAL)
             close(lse, ref[1], ltol)
     assert V.read_device_error() == 0
 
@@ -486,7 +492,7 @@ def test_mixed_steps_replayed_with_other_lengths(kv_type):
         graph.replay()
         ref = R.attend(c)
         tol, ltol = R.attend_tolerance(ref, 1)
-        close(out, ref[0], tol + ref[4] * 2.0 ** -22)
+        close(out, ref[0], tol + ref[4] * SUBNORMAL)
         close(lse, ref[1], ltol)
     assert V.read_device_error() == 0
 
@@ -560,7 +566,7 @@ def test_layers_and_steps_share_one_set():
                 c, kv = l[what], l[what + 1]
                 out = kv.attend(up(c["q"]))
                 ref = R.attend(c)
-                close(out, ref[0], R.attend_tolerance(ref, 1)[0] + ref[4] * 2.0 ** -22)
+                close(out, ref[0], R.attend_tolerance(ref, 1)[0] + ref[4] * SUBNORMAL)
     for i, (c, kv, _, _) in enumerate(layers):
         sc = np.random.default_rng(i).random((2, 2, 700)).astype(np.float32)
         src = torch.empty(2, 2, 200, dtype=torch.int32, device="cuda")
@@ -568,3 +574,46 @@ def test_layers_and_steps_share_one_set():
         for (s, h), rows in R.evict(c, sc, 200)[0].items():
             assert np.array_equal(src[s, h].cpu().numpy(), rows)
     assert V.read_device_error() == 0
+
+
+# ---- Q8_0 caches: P is all that is rounded ----------------------------------------------------------------
+
+Q8_CASES = [i for i, x in enumerate(ATTEND) if x[0] == "q8_0"]
+
+
+def q8_tolerance(c, ref):
+    """Bounds with one rounding to half, P's, which carries V's scale d: relative 2^-11, and
+    2^-25 for a subnormal, of a product whose largest is 16 d or more in the streaming
+    kernel, 64 d over short caches, 1 over an unpacked one (whose V is exact to 2^-25)."""
+    tol, ltol = R.attend_tolerance(ref, 1)
+    scales = R.half_bits_to_f64(c["v_pool"].reshape(*c["v_pool"].shape[:-1], -1, R.QB)[..., :2])
+    low = np.abs(scales[np.isfinite(scales)]).min()
+    return tol + ref[4] * 2.0 ** -25 / min(1.0, 16 * low) + 2.0 ** -25, ltol
+
+
+def test_q8_bounds_notice_a_rounded_key():
+    """K rounded to half would move a score by 2^-12 of its products' sum: more than lse's bound."""
+    c = R.build(100 + Q8_CASES[1], "q8_0", [(1, 1), (1, 15), (1, 64)], 8, 2, 128, 32)
+    ref = R.attend(c)
+    _, ltol = q8_tolerance(c, ref)
+    out = np.zeros(ref[1].shape)
+    for s, n in enumerate(c["len"]):
+        k = R.values(R.rows_of(c["k_pool"], c["table"][s], n)).astype(np.float16).astype(np.float64)
+        for h in range(8):
+            x = k[h // 4] @ c["q"][s, h].astype(np.float64) * 128 ** -0.5
+            out[s, h] = np.log(np.exp(x - x.max()).sum()) + x.max()
+    assert (np.abs(out - ref[1]) > ltol).mean() > 0.25
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", Q8_CASES)
+def test_attend_over_q8_rounds_p_alone(i):
+    kv_type, streams, Hq, Hkv, D, page, opt = ATTEND[i]
+    c = R.build(100 + i, kv_type, streams, Hq, Hkv, D, page)
+    ref = R.attend(c, **opt)
+    tol, ltol = q8_tolerance(c, ref)
+    q = up(c["q"])
+    out, lse = torch.empty(q.shape, device="cuda"), torch.empty(q.shape[:2], device="cuda")
+    device_kv(c).attend(q, out=out, lse=lse, **{("logit_softcap" if k == "softcap" else k): v for k, v in opt.items()})
+    close(out, ref[0], tol)
+    close(lse, ref[1], ltol)
