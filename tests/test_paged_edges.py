@@ -617,3 +617,82 @@ def test_attend_over_q8_rounds_p_alone(i):
     device_kv(c).attend(q, out=out, lse=lse, **{("logit_softcap" if k == "softcap" else k): v for k, v in opt.items()})
     close(out, ref[0], tol)
     close(lse, ref[1], ltol)
+
+
+# ---- all four calls in one captured step ---------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_type", ["f16", "q8_0"])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_captured_step_with_its_eviction(kv_type, in_place):
+    """A step of append, attention, score and eviction captured once and replayed:
+    single tokens next to a chunk, each stream brought back to its budget."""
+    Hq, Hkv, D, page, cap, keep = 8, 2, 128, 16, 128, 70
+    rng = np.random.default_rng(6)
+    new, length = [1, 30, 1], [60, 50, 69]
+    c = R.build(130, kv_type, [(n, cap) for n in new], Hq, Hkv, D, page, poison=False)
+    c["table"], c["len"], T = np.ascontiguousarray(c["table"][:, :cap // page]), length, sum(new)
+    kv = device_kv(c, max_kv_len=cap)
+    f = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float32)).cuda()  # noqa: E731
+    k, v, qf = (torch.zeros(T, h, D, device="cuda") for h in (Hkv, Hkv, Hq))
+    q16, out, lse = torch.zeros(T, Hq, D, dtype=torch.float16, device="cuda"), torch.zeros(T, Hq, D, device="cuda"), torch.zeros(T, Hq, device="cuda")
+    score, row_pos = torch.zeros(3, Hkv, cap, device="cuda"), torch.arange(cap, dtype=torch.int32, device="cuda").repeat(3, Hkv, 1)
+    score += f(3, Hkv, cap).abs()
+    n_new, positions = torch.tensor(new, dtype=torch.int32, device="cuda"), torch.zeros(T, dtype=torch.int32, device="cuda")
+    next_pos, left = torch.tensor(length, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    src = torch.zeros(3, Hkv, cap, dtype=torch.int32, device="cuda")
+    within = torch.cat([torch.arange(n, dtype=torch.int32) for n in new]).cuda()
+    which = torch.repeat_interleave(torch.arange(3), torch.tensor(new)).cuda()
+    state = {}
+
+    def step():
+        positions.copy_(next_pos[which] + within)
+        kv.kv_len.add_(n_new)
+        next_pos.add_(n_new)
+        kv.append(k, v, positions, BASE, q=qf, q_out=q16, row_pos=row_pos, score=score)
+        kv.attend(q16, out=out, lse=lse)
+        kv.score(q16, lse, score, observe=8)
+        for name, x in (("k_pool", kv.k_pool), ("v_pool", kv.v_pool), ("score", score), ("pos", row_pos), ("len", kv.kv_len)):
+            state.setdefault(name, torch.zeros_like(x)).copy_(x)          # before the eviction
+        kv.evict(score, keep, None if in_place else left, n_sink=4, n_recent=40, row_pos=row_pos, next_pos=next_pos,
+                 score_out=score, pos_out=row_pos, src_out=src)
+        if not in_place:
+            kv.kv_len.copy_(left)
+
+    graph = None
+    for turn in range(8):
+        for x in (k, v, qf):
+            x.copy_(f(*x.shape))
+        if graph is None:
+            step()
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                step()
+        else:
+            old = score.clone()
+            graph.replay()
+        host = {n: x.cpu().numpy() for n, x in state.items()}
+        now = dict(c, len=host["len"].tolist(), q=q16.cpu().numpy(), k_pool=host["k_pool"], v_pool=host["v_pool"])
+        ref = R.attend(now)
+        tol, ltol = R.attend_tolerance(ref, 1)
+        close(out, ref[0], tol + ref[4] * SUBNORMAL)
+        close(lse, ref[1], ltol)
+        if turn:
+            before = old.cpu().numpy()
+            for s, n in enumerate(now["len"]):
+                before[s, :, n - new[s]:n] = 0.0
+            want, stol = R.score(now, lse.cpu().numpy(), before, cap, observe=8)
+            for s, n in enumerate(now["len"]):
+                assert (np.abs(host["score"][s, :, :n] - want[s, :, :n]) <= stol[s, :, :n]).all()
+        rows, lens = R.evict(now, host["score"], keep, 4, 40, host["pos"], next_pos.tolist())
+        assert kv.kv_len.tolist() == lens
+        after = [(host[p], getattr(kv, p).cpu().numpy()) for p in ("k_pool", "v_pool")]
+        for (s, h), r in rows.items():
+            assert np.array_equal(src[s, h, :len(r)].cpu().numpy(), r)
+            assert np.array_equal(score[s, h, :len(r)].cpu().numpy(), host["score"][s, h, r])
+            assert np.array_equal(row_pos[s, h, :len(r)].cpu().numpy(), host["pos"][s, h, r])
+            for was, is_ in after:
+                assert np.array_equal(R.rows_of(is_, c["table"][s], len(r))[h],
+                                      R.rows_of(was, c["table"][s], now["len"][s])[h][r])
+    assert V.read_device_error() == 0
