@@ -470,6 +470,7 @@ VTX_API int vtx_kv_append_paged(const vtx_kv_append_paged_args *args, void *stre
  * V may also spoil tokens of its stream that do not see it.  A row with a score
  * of NaN or +inf has NaN in dst and in lse; one of -inf counts nothing.  dst must
  * not overlap q.
+ * dst and lse of tokens of no stream, and of what exceeds max_new, are left alone.
  * Rounded to half: P (times the scale of V for a Q8_0 cache) and a F32 q.
  * Everything else is F32, the values of a Q8_0 cache included.  Its scales may
  * reach 511 (larger ones overflow a half); below 2^-14 those of V cost bits of

@@ -15,7 +15,10 @@
 // integers (exact halves): K's scales are applied to each block's f32 sum, V's to P
 // before its one rounding to half, 64-fold so that a small scale keeps P out of the
 // subnormals.  So only P (and a F32 q) is rounded.  Loads are not overlapped with
-// the products: over 95 keys there is little to overlap.
+// the products: over the 95 keys at most that it is meant for there is little to
+// overlap.  Chunks over longer caches come here too where their unpacked copy would
+// be too large (vtx_paged.cu), and pay for it: 128 tokens at 14k keys 1630 us, 109 on
+// the tensor-core kernel.
 #pragma once
 #include <cuda_fp16.h>
 #include <cstdint>

@@ -28,8 +28,9 @@
 // 502 over F16 pages, for twice the products.
 //
 // D = 64, twice the exponentials per flop: a quarter of them runs on the FMA pipe
-// (2048 tokens at 14k keys 446 -> 430 us; D = 128 gained nothing, 519 us either way,
-// and under the power cap it costs, 569 against 562 us).  2^x = 2^j p(f), j = round(x),
+// (2048 tokens at 14k keys 496-506 us without, 449-500 with, by how warm the board is;
+// over Q8_0 652 and 631; D = 128 gained nothing, 519 us either way, and under the power
+// cap it costs, 569 against 562 us).  2^x = 2^j p(f), j = round(x),
 // with p the degree-4 polynomial of least relative error (2.6e-6) on
 // [-1/2, 1/2], fitted here by an exchange.  The row sums are taken of the f32
 // P, so lse carries neither P's rounding to half nor more than that error.

@@ -651,7 +651,8 @@ class PagedKv:
         """vtx_flash_attn_paged: q (n_tokens, n_head_q, D) float16 / float32 ->
         out, same shape (float32, or the type of the given tensor).  lse:
         optional float32 (n_tokens, n_head_q) that receives ln sum exp.  scale
-        defaults to D ** -0.5."""
+        defaults to D ** -0.5.  Rows of tokens of no stream are left as they are
+        (not initialised, in a result made here)."""
         if out is None:
             out = _empty(self._q_shape, torch.float32, self.dev, stream)
         with self._lock:
