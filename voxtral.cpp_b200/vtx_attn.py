@@ -467,10 +467,10 @@ class PagedKv:
     meet a Q8_0 cache; share= takes those of another PagedKv, no smaller ones, so
     that layers, or prompts and single tokens, have one set between them.  Calls
     on one PagedKv, or on those that share, may come from several host threads,
-    but must not overlap on the GPU, and it must live until they are done.  Inputs and outputs stay the caller's and are not
-    copied.  A call with stream= is queued there and waits for nothing else: its
-    inputs have to be ready on that stream, and a result that it makes is that
-    stream's."""
+    but must not overlap on the GPU, and it must live until they are done.  Inputs
+    and outputs stay the caller's and are not copied.  A call with stream= is
+    queued there and waits for nothing else: its inputs have to be ready on that
+    stream, and a result that it makes is that stream's."""
 
     def __init__(self, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor,
                  q_start: torch.Tensor, n_head_q: int, *, n_tokens: int, max_new: int,
